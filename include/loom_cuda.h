@@ -41,6 +41,7 @@ extern "C" {
 
 enum {
     LOOM_F32 = 0,
+    LOOM_F16 = 1,
     LOOM_Q4_0 = 2,
     LOOM_Q4_1 = 3,
     LOOM_Q5_0 = 6,
@@ -50,7 +51,8 @@ enum {
     LOOM_Q3_K = 11,
     LOOM_Q4_K = 12,
     LOOM_Q5_K = 13,
-    LOOM_Q6_K = 14
+    LOOM_Q6_K = 14,
+    LOOM_BF16 = 30
 };
 
 /* WeightRef, src/compute/cpu.zig:21: a weight tensor as the fused entries take it. */
@@ -512,6 +514,82 @@ int loom_cuda_ep_a2a_forward(const loom_moe_desc *desc, const float *d_x, size_t
  * API: no counterpart in the reference's seam. */
 int loom_cuda_ep_a2a_forward_cap(const loom_moe_desc *desc, const float *d_x, size_t T, size_t t_cap, float *d_out,
                                  const float *d_residual, const float *d_logits, uint32_t *d_ids, void *stream);
+/* ---- batched serving: shared prompts, adapters, drafted tokens ---------------
+ * No counterpart in the reference: the operators that one step of many requests
+ * needs when they share a prompt, bring their own adapters and draft tokens. The
+ * three share one row layout: the rows of sequence b are d_seq_rows[b] ..
+ * d_seq_rows[b + 1] - 1 (device u32 [n_seqs + 1], rising from 0 to n_rows): its
+ * last accepted token, then its drafts in order. All work on device buffers, on
+ * `stream`, and only launch: scratch is the caller's workspace (16-byte aligned, at
+ * least loom_cuda_*_workspace(desc) bytes, not shared by calls that overlap; its
+ * contents need not be kept), so they can be captured in a CUDA graph. Strides
+ * count elements; element types are LOOM_F32, LOOM_F16 and LOOM_BF16, sums are
+ * f32 or wider. Device-side indices that lie outside the call's sizes are held to
+ * them: the result is then meaningless, but nothing outside the buffers is
+ * touched. Outputs may not overlap inputs, except where said. */
+
+/* Softmax attention of every row over a prefix cache that all sequences share and
+ * its sequence's own cache: row j of the n rows of sequence b sees the prefix's
+ * prefix_len positions and own positions 0 .. d_seq_len[b] - (n - 1 - j) - 1, so
+ * that d_seq_len counts the rows of this step, whose keys and values are in the
+ * own cache already. q is [n_rows][n_heads][head_dim] (rows q_stride apart), out
+ * likewise; key (or value) i of KV head h is at i * pos_stride + h * head_stride,
+ * plus b * own_seq_stride in the own caches, which hold own_cap positions each. One
+ * type for q, caches and out. head_dim 1..256; query head h reads KV head
+ * h / (n_heads / n_kv_heads). A row that sees nothing gives zeros. */
+typedef struct {
+    int type;
+    float scale; /* scores = scale * q.k */
+    size_t n_seqs, n_rows, n_heads, n_kv_heads, head_dim;
+    size_t q_stride, out_stride;
+    size_t prefix_len, prefix_pos_stride, prefix_head_stride;
+    size_t own_cap, own_pos_stride, own_head_stride, own_seq_stride;
+} loom_attn_shared_desc;
+size_t loom_cuda_attn_shared_workspace(const loom_attn_shared_desc *desc);
+int loom_cuda_attn_shared(const loom_attn_shared_desc *desc, const void *d_q, const void *d_prefix_k,
+                          const void *d_prefix_v, const void *d_own_k, const void *d_own_v, const uint32_t *d_seq_rows,
+                          const uint32_t *d_seq_len, void *d_out, void *d_ws, size_t ws_bytes, void *stream);
+
+/* out[r] = base[r] + d_scales[a] * B_a (A_a x[r]) with a = d_ids[r]; a row whose id
+ * is outside 0 .. n_adapters - 1 keeps its base. x, base and out are f32, A
+ * [n_adapters][max_rank][n_in] and B [n_adapters][n_out][max_rank] of `type`, of
+ * which adapter a uses its first d_ranks[a] rows (columns of B); the rest is not
+ * read. base NULL reads as zeros; out may be base (same rows). */
+typedef struct {
+    int type; /* of A and B */
+    size_t n_rows, n_in, n_out, n_adapters, max_rank;
+    size_t x_stride, base_stride, out_stride;
+    size_t a_row_stride, a_adapter_stride, b_row_stride, b_adapter_stride;
+} loom_lora_desc;
+size_t loom_cuda_lora_workspace(const loom_lora_desc *desc);
+int loom_cuda_lora(const loom_lora_desc *desc, const float *d_x, const void *d_a, const void *d_b,
+                   const int32_t *d_ranks, const float *d_scales, const int32_t *d_ids, const float *d_base,
+                   float *d_out, void *d_ws, size_t ws_bytes, void *stream);
+
+/* Verification of drafted tokens. Row r's logits (type, [n_rows][vocab]) are the
+ * target's for the token after row r; that token's draft, if row r is not its
+ * sequence's last, is d_tokens[r + 1], and d_draft_probs[r] (f32 [vocab], NULL: a
+ * drafter without chance, probability 1 at its draft) is what it was drawn from.
+ * With p = softmax(logits[r] / T), T = d_temperature[b] (NULL: 1), drafts are
+ * accepted in order while d_u[r] * q(draft) < p(draft); at T <= 0 while the draft
+ * is the argmax. Then one more token is chosen: after a refusal from max(p - q, 0)
+ * (from p when that is zero everywhere), after the last draft from p, at the first
+ * index where the running sum exceeds d_u[last row of b] times the whole; at T <= 0
+ * the argmax (first maximum, NaN never taken, 0 when nothing is above -inf). d_u is
+ * f32 [n_rows] in [0, 1). A draft outside the vocabulary is refused.
+ * d_out[r]: the token after row r, for the accepted drafts and the chosen token,
+ * -1 in the sequence's other rows; d_n_out[b]: how many there are (0 for a sequence
+ * without rows); d_logprobs[r]: their log p (at T <= 0 of softmax(logits)), else 0. */
+typedef struct {
+    int type; /* of the logits */
+    size_t n_seqs, n_rows, vocab;
+    size_t logits_stride, probs_stride;
+} loom_verify_desc;
+size_t loom_cuda_verify_workspace(const loom_verify_desc *desc);
+int loom_cuda_verify(const loom_verify_desc *desc, const void *d_logits, const float *d_draft_probs,
+                     const int32_t *d_tokens, const uint32_t *d_seq_rows, const float *d_u, const float *d_temperature,
+                     int32_t *d_out, int32_t *d_n_out, float *d_logprobs, void *d_ws, size_t ws_bytes, void *stream);
+
 /* Greedy sampling (sampler.zig:7-15 argmax) of device logits into *d_index
  * (device u32): the first maximum; NaN never taken; 0 when nothing is above
  * -inf. Asynchronous on `stream`; calls on one device share a 16-byte scratch,

@@ -82,6 +82,24 @@ class Shard(C.Structure):  # loom_shard
     _fields_ = [("ext", Weight * 4), ("n_ext", C.c_int), ("digest", C.c_uint8 * 32)]
 
 
+class AttnSharedDesc(C.Structure):  # loom_attn_shared_desc
+    _fields_ = [("type", C.c_int), ("scale", C.c_float)] + [(n, C.c_size_t) for n in (
+        "n_seqs", "n_rows", "n_heads", "n_kv_heads", "head_dim", "q_stride", "out_stride",
+        "prefix_len", "prefix_pos_stride", "prefix_head_stride",
+        "own_cap", "own_pos_stride", "own_head_stride", "own_seq_stride")]
+
+
+class LoraDesc(C.Structure):  # loom_lora_desc
+    _fields_ = [("type", C.c_int)] + [(n, C.c_size_t) for n in (
+        "n_rows", "n_in", "n_out", "n_adapters", "max_rank", "x_stride", "base_stride", "out_stride",
+        "a_row_stride", "a_adapter_stride", "b_row_stride", "b_adapter_stride")]
+
+
+class VerifyDesc(C.Structure):  # loom_verify_desc
+    _fields_ = [("type", C.c_int)] + [(n, C.c_size_t) for n in (
+        "n_seqs", "n_rows", "vocab", "logits_stride", "probs_stride")]
+
+
 def header_symbols() -> list[str]:
     """Every function the public header declares."""
     src = open(HEADER).read()
@@ -185,6 +203,12 @@ def lib() -> C.CDLL:
         "loom_gguf_get_string": (i, [vp, C.c_char_p, C.POINTER(C.c_void_p), C.POINTER(sz)]),
         "loom_gguf_get_bool": (i, [vp, C.c_char_p, C.POINTER(i)]),
         "loom_gguf_resolve": (i, [vp, C.c_char_p, C.POINTER(GgufView)]),
+        "loom_cuda_attn_shared_workspace": (sz, [C.POINTER(AttnSharedDesc)]),
+        "loom_cuda_attn_shared": (i, [C.POINTER(AttnSharedDesc)] + [vp] * 9 + [sz, vp]),
+        "loom_cuda_lora_workspace": (sz, [C.POINTER(LoraDesc)]),
+        "loom_cuda_lora": (i, [C.POINTER(LoraDesc)] + [vp] * 9 + [sz, vp]),
+        "loom_cuda_verify_workspace": (sz, [C.POINTER(VerifyDesc)]),
+        "loom_cuda_verify": (i, [C.POINTER(VerifyDesc)] + [vp] * 10 + [sz, vp]),
         "loom_cuda_verify_shards": (i, [C.POINTER(Shard), sz, vp, C.POINTER(sz)]),
         "loom_cuda_sha256_device": (i, [vp, sz, vp]),
         "loom_cuda_tensor_sha256": (i, [u64, u64, u64, vp]),

@@ -1,0 +1,67 @@
+"""CPU checks of the batched-serving entries: struct layout, refusals that need no device."""
+import ctypes as C
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from loom_b200 import LoomCudaError, _lib, serve
+
+
+def test_descriptors_match_the_header(tmp_path):
+    """Size of each descriptor and the offset of each field."""
+    if not shutil.which("gcc"):
+        pytest.skip("no C compiler")
+    names = {"loom_attn_shared_desc": _lib.AttnSharedDesc, "loom_lora_desc": _lib.LoraDesc,
+             "loom_verify_desc": _lib.VerifyDesc}
+    lines, want = [], []
+    for n, cls in names.items():
+        lines.append('printf("%%zu\\n", sizeof(%s));' % n)
+        want.append(C.sizeof(cls))
+        for f, _ in cls._fields_:
+            lines.append('printf("%%zu\\n", offsetof(%s, %s));' % (n, f))
+            want.append(getattr(cls, f).offset)
+    src = tmp_path / "sz.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "%s"\nint main(void){%s return 0;}\n' % (
+        _lib.HEADER, " ".join(lines)))
+    exe = tmp_path / "sz"
+    subprocess.run(["gcc", "-o", str(exe), str(src)], check=True)
+    assert [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()] == want
+
+
+def test_workspace_sizes_and_bad_descriptors():
+    L = _lib.lib()
+    good = dict(type=30, scale=0.1, n_seqs=4, n_rows=9, n_heads=32, n_kv_heads=4, head_dim=128, q_stride=4096,
+                out_stride=4096, prefix_len=1000, prefix_pos_stride=512, prefix_head_stride=128, own_cap=300,
+                own_pos_stride=512, own_head_stride=128, own_seq_stride=300 * 512)
+    ws = lambda **kw: L.loom_cuda_attn_shared_workspace(C.byref(_lib.AttnSharedDesc(**{**good, **kw})))  # noqa: E731
+    assert ws() > 0
+    assert ws(type=0) > 0 and ws(type=8) == 0 and ws(n_kv_heads=5) == 0 and ws(head_dim=257) == 0
+    assert ws(n_heads=0) == 0 and ws(prefix_len=1 << 40) == 0 and ws(n_rows=1 << 40) == 0
+    lora = lambda **kw: L.loom_cuda_lora_workspace(C.byref(_lib.LoraDesc(**{**dict(  # noqa: E731
+        type=1, n_rows=5, n_in=64, n_out=32, n_adapters=2, max_rank=8, x_stride=64, base_stride=32, out_stride=32,
+        a_row_stride=64, a_adapter_stride=512, b_row_stride=8, b_adapter_stride=256), **kw})))
+    assert lora() > 0 and lora(type=12) == 0 and lora(n_in=0) == 0 and lora(max_rank=5000) == 0
+    ver = lambda **kw: L.loom_cuda_verify_workspace(C.byref(_lib.VerifyDesc(**{**dict(  # noqa: E731
+        type=0, n_seqs=2, n_rows=5, vocab=100, logits_stride=100, probs_stride=0), **kw})))
+    assert ver() > 0 and ver(type=2) == 0 and ver(vocab=0) == 0 and ver(vocab=1 << 30) == 0
+
+
+def test_entries_decline_before_init():
+    L = _lib.lib()
+    d = _lib.VerifyDesc(0, 1, 1, 4, 4, 0)
+    assert L.loom_cuda_verify(C.byref(d), *[None] * 10, 0, None) == _lib.DECLINED
+    assert "init" in _lib.last_error()
+    assert L.loom_cuda_lora(C.byref(_lib.LoraDesc()), *[None] * 9, 0, None) == _lib.DECLINED
+    assert L.loom_cuda_attn_shared(C.byref(_lib.AttnSharedDesc()), *[None] * 9, 0, None) == _lib.DECLINED
+
+
+def test_host_tensors_are_refused():
+    z, i = torch.zeros, torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(LoomCudaError, match="cuda"):
+        serve.attn_shared(z(1, 2, 8), z(4, 1, 8), z(4, 1, 8), z(1, 4, 1, 8), z(1, 4, 1, 8), i, i[:1], 1.0)
+    with pytest.raises(LoomCudaError, match="cuda"):
+        serve.lora(z(1, 4), z(1, 2, 4), z(1, 3, 2), i[:1], z(1), i[:1])
+    with pytest.raises(LoomCudaError, match="cuda"):
+        serve.verify(z(1, 4), i[:1], i, z(1))
