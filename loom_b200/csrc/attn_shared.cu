@@ -21,6 +21,7 @@
 #include <cfloat>
 
 #include "../../include/loom_cuda.h"
+#include "mma.cuh"
 #include "serve.cuh"
 
 namespace loom {
@@ -40,7 +41,7 @@ struct AttnArgs {
     int64_t q_stride, out_stride, ppos, phead, opos, ohead, oseq;
     int n_seqs, n_rows, nh, nkv, group, hd;
     int prefix, cap;
-    int pre_chunk, own_chunk, n_pre, n_own, pre_tiles;
+    int pre_chunk, own_chunk, n_pre, n_own, pre_tiles, pre_rows;
     float scale;  // of the scores in base 2: scale * log2(e)
 };
 
@@ -59,6 +60,43 @@ __device__ __forceinline__ SeqView seq_view(const AttnArgs &a, int b) {
     return s;
 }
 
+// A CTA's work: query rows r0 .. r1-1 (row * group + head of the group) of one KV
+// head against positions p0 .. p1-1 of a cache, and the slot for the parts.
+template <class T> struct Item {
+    int slot, r0, r1, p0, p1;
+    const T *k, *v;
+    int64_t pos_stride;
+};
+template <class T> __device__ __forceinline__ Item<T> item_of(const AttnArgs &a, int item, int kvh) {
+    Item<T> o;
+    if (item < a.n_pre * a.pre_tiles) {
+        o.slot = item / a.pre_tiles;
+        o.r0 = (item % a.pre_tiles) * a.pre_rows;
+        o.r1 = min(o.r0 + a.pre_rows, a.n_rows * a.group);
+        o.p0 = o.slot * a.pre_chunk;
+        o.p1 = min(o.p0 + a.pre_chunk, a.prefix);
+        o.pos_stride = a.ppos;
+        o.k = static_cast<const T *>(a.pk) + kvh * a.phead;
+        o.v = static_cast<const T *>(a.pv) + kvh * a.phead;
+    } else {
+        item -= a.n_pre * a.pre_tiles;
+        const int b = item / a.n_own, c = item % a.n_own;
+        const SeqView s = seq_view(a, b);
+        o.slot = a.n_pre + c;
+        o.r0 = s.row0 * a.group;
+        o.r1 = o.r0 + s.rows * a.group;
+        o.p0 = c * a.own_chunk;
+        o.p1 = min(o.p0 + a.own_chunk, s.common);
+        o.pos_stride = a.opos;
+        o.k = static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead;
+        o.v = static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead;
+    }
+    return o;
+}
+__device__ __forceinline__ size_t part_at(const AttnArgs &a, int slot, int hr, int kvh) {
+    return ((size_t)slot * a.n_rows + hr / a.group) * a.nh + kvh * a.group + hr % a.group;
+}
+
 // ---- any shape ---------------------------------------------------------------
 // One CTA per chunk of positions and KV head. 32 positions at a time go to
 // shared memory as f32; 16 query rows (row, head of the group) share them, a
@@ -70,32 +108,10 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
     extern __shared__ float sm[];
     const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     float *sq = sm, *sk = sq + G_TR * hd, *sv = sk + G_TP * (hd + 1), *ss = sv + G_TP * hd;
-    int item = blockIdx.x, slot, r0, r1, p0, p1;
-    const T *kb, *vb;
-    int64_t ps;
-    if (item < a.n_pre * a.pre_tiles) {
-        slot = item / a.pre_tiles;
-        const int rows = a.n_rows * a.group, per = (rows + a.pre_tiles - 1) / a.pre_tiles;
-        r0 = (item % a.pre_tiles) * per;
-        r1 = min(r0 + per, rows);
-        p0 = slot * a.pre_chunk;
-        p1 = min(p0 + a.pre_chunk, a.prefix);
-        ps = a.ppos;
-        kb = static_cast<const T *>(a.pk) + kvh * a.phead;
-        vb = static_cast<const T *>(a.pv) + kvh * a.phead;
-    } else {
-        item -= a.n_pre * a.pre_tiles;
-        const int b = item / a.n_own, c = item % a.n_own;
-        const SeqView s = seq_view(a, b);
-        slot = a.n_pre + c;
-        r0 = s.row0 * a.group;
-        r1 = r0 + s.rows * a.group;
-        p0 = c * a.own_chunk;
-        p1 = min(p0 + a.own_chunk, s.common);
-        ps = a.opos;
-        kb = static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead;
-        vb = static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead;
-    }
+    const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
+    const int slot = it.slot, r0 = it.r0, r1 = it.r1, p0 = it.p0, p1 = it.p1;
+    const T *kb = it.k, *vb = it.v;
+    const int64_t ps = it.pos_stride;
     if (p0 >= p1) return;  // the join does not read this slot
     for (int t0 = r0; t0 < r1; t0 += G_TR) {
         __syncthreads();
@@ -158,11 +174,303 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
         for (int j = 0; j < 4; j++) {
             const int hr = t0 + warp * 4 + j;
             if (hr >= r1) break;
-            const size_t at = ((size_t)slot * a.n_rows + hr / a.group) * a.nh + kvh * a.group + hr % a.group;
+            const size_t at = part_at(a, slot, hr, kvh);
             if (lane == 0) a.ml[at] = make_float2(m[j], l[j]);
 #pragma unroll
             for (int d = 0; d < MAX_HD / 32; d++)
                 if (d * 32 + lane < hd) a.acc[at * hd + d * 32 + lane] = acc[j][d];
+        }
+    }
+}
+
+// ---- tensor cores, a few query rows per tile ------------------------------------
+// Four warps over up to 64 query rows: a warp has 16 of them, and warps that are
+// left over when the rows are fewer share the rows and split the positions (a
+// decode step's 8 heads of a group: all four do), joining at the end. Positions
+// come in tiles through two shared-memory stages (16-byte asynchronous copies).
+// Scores, maxima and sums are f32. The weights are rounded to the element type for
+// their product with the values (2^-9 or 2^-12 of each, the size of the output's
+// own rounding) and summed as rounded, so that they still add up to one; f32
+// operands go as three tf32 products (mma.cuh), and each step's leading products
+// are added to the running sums by f32 additions: the tensor core truncates its
+// own, which along a row of 128 dimensions cost 2.1e-6 of the result, not 1e-6.
+template <class T> constexpr int mma_tp() { return sizeof(T) == 4 ? 32 : 64; }
+template <class T, int HDP> constexpr int mma_kstride() { return sizeof(T) == 4 ? HDP + 8 : HDP + 8; }
+template <class T, int HDP> constexpr int mma_vstride() { return sizeof(T) == 4 ? HDP + 4 : HDP + 8; }
+template <class T, int HDP> constexpr size_t mma_stage() {
+    return (size_t)mma_tp<T>() * (mma_kstride<T, HDP>() + mma_vstride<T, HDP>()) * sizeof(T);
+}
+constexpr size_t maxz(size_t a, size_t b) { return a > b ? a : b; }
+template <class T, int HDP> constexpr size_t mma_smem() {  // stages (or the warps' sums), then f32 queries
+    return maxz(2 * mma_stage<T, HDP>(), (size_t)64 * HDP * 4) + (sizeof(T) == 4 ? (size_t)64 * (HDP + 8) * 4 : 0);
+}
+
+template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a) {
+    constexpr int TP = mma_tp<T>(), KST = mma_kstride<T, HDP>(), VST = mma_vstride<T, HDP>();
+    constexpr bool F = sizeof(T) == 4;
+    constexpr int SUB = F ? 8 : 16;            // positions of one step of a warp
+    constexpr int KS = F ? 1 : HDP / 16;       // query fragments held in registers (16-bit types)
+    extern __shared__ __align__(16) uint8_t smb[];
+    __shared__ float s_m[4][16], s_l[4][16];
+    const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int kvh = blockIdx.y;
+    const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
+    if (it.p0 >= it.p1) return;  // the join does not read this slot
+    auto stage_k = [&](int s) { return reinterpret_cast<T *>(smb + s * mma_stage<T, HDP>()); };
+    auto stage_v = [&](int s) { return stage_k(s) + TP * KST; };
+    float *sq = reinterpret_cast<float *>(smb + maxz(2 * mma_stage<T, HDP>(), (size_t)64 * HDP * 4));
+    constexpr int QST = HDP + 8;
+    const int wide = (hd + SUB - 1) / SUB * SUB;  // the head dimension rounded up to a product's depth
+    if (wide > hd)                                // its rest holds zeros, which the copies leave alone
+        for (int i = tid; i < 2 * TP * (wide - hd); i += 128) {
+            const int s = i / (TP * (wide - hd)), j = i / (wide - hd) % TP, d = hd + i % (wide - hd);
+            stage_k(s)[j * KST + d] = from_f32<T>(0.0f);
+            stage_v(s)[j * VST + d] = from_f32<T>(0.0f);
+        }
+    const int cpr = hd * (int)sizeof(T) / 16;  // 16-byte pieces of a row
+    const int drow = 128 / cpr, dcol = 128 % cpr;
+    auto fetch = [&](int s, int p) {
+        int j = tid / cpr, c = tid % cpr;
+        const uint32_t k0 = smem_u32(stage_k(s)), v0 = smem_u32(stage_v(s));
+        while (j < TP) {
+            const bool in = p + j < it.p1;
+            const int64_t src = (int64_t)(in ? p + j : it.p0) * it.pos_stride + c * (16 / (int)sizeof(T));
+            cp_async16(k0 + j * (KST * (int)sizeof(T)) + c * 16, it.k + src, in);
+            cp_async16(v0 + j * (VST * (int)sizeof(T)) + c * 16, it.v + src, in);
+            j += drow;
+            c += dcol;
+            if (c >= cpr) {
+                c -= cpr;
+                j++;
+            }
+        }
+    };
+    for (int rb = it.r0; rb < it.r1; rb += 64) {
+        const int rows = min(64, it.r1 - rb);
+        const int nps = rows <= 16 ? 4 : rows <= 32 ? 2 : 1;  // warps that share 16 rows
+        const int rt = warp / nps, ps = warp % nps;
+        const int row_a = rb + rt * 16 + g, row_b = row_a + 8;
+        const bool in_a = row_a < it.r1, in_b = row_b < it.r1, busy = rt * 16 < rows;
+        auto q_row = [&](int hr) {
+            return static_cast<const T *>(a.q) + (int64_t)(hr / a.group) * a.q_stride +
+                   (int64_t)(kvh * a.group + hr % a.group) * hd;
+        };
+        __syncthreads();  // the last block's joined sums have been read
+        fetch(0, it.p0);
+        cp_async_commit();
+        fetch(1, it.p0 + TP);
+        cp_async_commit();
+        uint32_t qf[KS][4];
+        if constexpr (F) {
+            for (int i = tid; i < 64 * wide; i += 128) {
+                const int j = i / wide, d = i % wide;
+                sq[j * QST + d] = j < rows && d < hd ? reinterpret_cast<const float *>(q_row(rb + j))[d] : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int d = k * 16 + 2 * t;
+                auto two = [&](bool in, int hr, int dd) -> uint32_t {
+                    if (!in || dd >= hd) return 0u;
+                    const uint16_t *p = reinterpret_cast<const uint16_t *>(q_row(hr) + dd);
+                    return (uint32_t)p[0] | ((uint32_t)p[1] << 16);  // hd is even
+                };
+                qf[k][0] = two(in_a, row_a, d);
+                qf[k][1] = two(in_b, row_b, d);
+                qf[k][2] = two(in_a, row_a, d + 8);
+                qf[k][3] = two(in_b, row_b, d + 8);
+            }
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        float o[HDP / 8][4];
+#pragma unroll
+        for (int i = 0; i < HDP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        int s = 0;
+        for (int p = it.p0; p < it.p1; p += TP, s ^= 1) {
+            cp_async_wait<1>();
+            __syncthreads();
+            const T *sk = stage_k(s), *sv = stage_v(s);
+            for (int sub = ps * SUB; busy && sub < TP && p + sub < it.p1; sub += nps * SUB) {
+                constexpr int NT = SUB / 8;
+                float c[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
+                if constexpr (F) {
+                    float small[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+                    for (int d = 0; d < wide; d += 8) {
+                        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const float2 qa = *reinterpret_cast<const float2 *>(sq + (rt * 16 + g) * QST + d + 2 * t);
+                        const float2 qb = *reinterpret_cast<const float2 *>(sq + (rt * 16 + g + 8) * QST + d + 2 * t);
+                        const float2 kk = *reinterpret_cast<const float2 *>(
+                            reinterpret_cast<const float *>(sk) + (sub + g) * KST + d + 2 * t);
+                        uint32_t ah[4], al[4], bh[2], bl[2];
+                        split_tf32(qa.x, ah[0], al[0]);
+                        split_tf32(qb.x, ah[1], al[1]);
+                        split_tf32(qa.y, ah[2], al[2]);
+                        split_tf32(qb.y, ah[3], al[3]);
+                        split_tf32(kk.x, bh[0], bl[0]);
+                        split_tf32(kk.y, bh[1], bl[1]);
+                        mma_tf32(small, al, bh[0], bh[1]);
+                        mma_tf32(small, ah, bl[0], bl[1]);
+                        mma_tf32(e, ah, bh[0], bh[1]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) c[0][j] += e[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) c[0][j] += small[j];
+                } else {
+                    const uint32_t at = smem_u32(sk + (sub + (lane >> 4) * 8 + (lane & 7)) * KST + ((lane >> 3) & 1) * 8);
+#pragma unroll
+                    for (int k = 0; k < KS; k++) {
+                        if (k * 16 < wide) {
+                            uint32_t b[4];
+                            ldmatrix_x4(b, at + k * 32);
+                            mma_k16<T>(c[0], qf[k], b[0], b[1]);
+                            mma_k16<T>(c[1], qf[k], b[2], b[3]);
+                        }
+                    }
+                }
+                float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        c[n][j] *= a.scale;
+                        if (p + sub + n * 8 + 2 * t + (j & 1) >= it.p1) c[n][j] = -INFINITY;
+                        float &x = j < 2 ? x0 : x1;
+                        x = fmaxf(x, c[n][j]);
+                    }
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
+                if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {  // the maxima settle after a few tiles
+                    const float f0 = ex2(m0 - b0), f1 = ex2(m1 - b1);
+                    l0 *= f0;
+                    l1 *= f1;
+#pragma unroll
+                    for (int i = 0; i < HDP / 8; i++) {
+                        o[i][0] *= f0;
+                        o[i][1] *= f0;
+                        o[i][2] *= f1;
+                        o[i][3] *= f1;
+                    }
+                    m0 = n0;
+                    m1 = n1;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    c[n][0] = ex2(c[n][0] - b0);
+                    c[n][1] = ex2(c[n][1] - b0);
+                    c[n][2] = ex2(c[n][2] - b1);
+                    c[n][3] = ex2(c[n][3] - b1);
+                }
+                if constexpr (F) {
+                    uint32_t ah[4], al[4];
+                    split_tf32(c[0][0], ah[0], al[0]);  // depth t is position 2t, depth t + 4 is 2t + 1
+                    split_tf32(c[0][2], ah[1], al[1]);
+                    split_tf32(c[0][1], ah[2], al[2]);
+                    split_tf32(c[0][3], ah[3], al[3]);
+                    l0 += c[0][0] + c[0][1];
+                    l1 += c[0][2] + c[0][3];
+                    const float *v0 = reinterpret_cast<const float *>(sv) + (sub + 2 * t) * VST + g;
+#pragma unroll
+                    for (int i = 0; i < HDP / 8; i++) {
+                        if (i * 8 < wide) {
+                            uint32_t bh[2], bl[2];
+                            split_tf32(v0[i * 8], bh[0], bl[0]);
+                            split_tf32(v0[VST + i * 8], bh[1], bl[1]);
+                            float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_tf32(e, al, bh[0], bh[1]);
+                            mma_tf32(e, ah, bl[0], bl[1]);
+                            mma_tf32(e, ah, bh[0], bh[1]);
+                            o[i][0] += e[0];
+                            o[i][1] += e[1];
+                            o[i][2] += e[2];
+                            o[i][3] += e[3];
+                        }
+                    }
+                } else {
+                    uint32_t pf[4];
+                    pf[0] = pack2<T>(c[0][0], c[0][1]);
+                    pf[1] = pack2<T>(c[0][2], c[0][3]);
+                    pf[2] = pack2<T>(c[1][0], c[1][1]);
+                    pf[3] = pack2<T>(c[1][2], c[1][3]);
+                    const float2 r0 = unpack2<T>(pf[0]), r1 = unpack2<T>(pf[1]), r2 = unpack2<T>(pf[2]), r3 = unpack2<T>(pf[3]);
+                    l0 += (r0.x + r0.y) + (r2.x + r2.y);
+                    l1 += (r1.x + r1.y) + (r3.x + r3.y);
+                    const uint32_t at = smem_u32(sv + (sub + ((lane >> 3) & 1) * 8 + (lane & 7)) * VST + (lane >> 4) * 8);
+#pragma unroll
+                    for (int i = 0; i < HDP / 16; i++) {
+                        if (i * 16 < wide) {
+                            uint32_t b[4];
+                            ldmatrix_x4_trans(b, at + i * 32);
+                            mma_k16<T>(o[2 * i], pf, b[0], b[1]);
+                            mma_k16<T>(o[2 * i + 1], pf, b[2], b[3]);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            if (p + 2 * TP < it.p1) fetch(s, p + 2 * TP);
+            cp_async_commit();
+        }
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        cp_async_wait<0>();
+        if (nps == 1) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                if (half ? !in_b : !in_a) continue;
+                const size_t at = part_at(a, it.slot, half ? row_b : row_a, kvh);
+                if (t == 0) a.ml[at] = half ? make_float2(m1, l1) : make_float2(m0, l0);
+                float *dst = a.acc + at * hd;
+#pragma unroll
+                for (int i = 0; i < HDP / 8; i++)
+                    if (i * 8 + 2 * t < hd)  // hd is even
+                        *reinterpret_cast<float2 *>(dst + i * 8 + 2 * t) = make_float2(o[i][2 * half], o[i][2 * half + 1]);
+            }
+            continue;
+        }
+        if (t == 0) {
+            s_m[warp][g] = m0;
+            s_m[warp][g + 8] = m1;
+            s_l[warp][g] = l0;
+            s_l[warp][g + 8] = l1;
+        }
+        __syncthreads();  // the tiles are read: the sums of the warps take their place
+        float *so = reinterpret_cast<float *>(smb) + warp * 16 * HDP;
+        {
+            float t0 = -INFINITY, t1 = -INFINITY;
+            for (int w = rt * nps; w < (rt + 1) * nps; w++) {
+                t0 = fmaxf(t0, s_m[w][g]);
+                t1 = fmaxf(t1, s_m[w][g + 8]);
+            }
+            const float f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - t0), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - t1);
+#pragma unroll
+            for (int i = 0; i < HDP / 8; i++) {
+                *reinterpret_cast<float2 *>(so + g * HDP + i * 8 + 2 * t) = make_float2(o[i][0] * f0, o[i][1] * f0);
+                *reinterpret_cast<float2 *>(so + (g + 8) * HDP + i * 8 + 2 * t) = make_float2(o[i][2] * f1, o[i][3] * f1);
+            }
+        }
+        __syncthreads();
+        for (int j = warp; j < rows; j += 4) {
+            const int w0 = (j / 16) * nps, jr = j % 16;
+            const size_t at = part_at(a, it.slot, rb + j, kvh);
+            float top = -INFINITY, l = 0.0f;
+            for (int w = w0; w < w0 + nps; w++) top = fmaxf(top, s_m[w][jr]);
+            for (int w = w0; w < w0 + nps; w++) l += s_l[w][jr] * (s_m[w][jr] == -INFINITY ? 0.0f : ex2(s_m[w][jr] - top));
+            if (lane == 0) a.ml[at] = make_float2(top, l);
+            for (int d = lane; d < hd; d += 32) {
+                float v = 0.0f;
+                for (int w = w0; w < w0 + nps; w++) v += reinterpret_cast<float *>(smb)[(w * 16 + jr) * HDP + d];
+                a.acc[at * hd + d] = v;
+            }
         }
     }
 }
@@ -260,13 +568,14 @@ void plan(const loom_attn_shared_desc *d, AttnArgs &a) {
     a.ohead = (int64_t)d->own_head_stride;
     a.oseq = (int64_t)d->own_seq_stride;
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int want = 4 * 148;
-    a.pre_tiles = (int)up((int64_t)a.n_rows * a.group, 64);
+    const int want = 6 * 148;
+    a.pre_rows = 64;
+    a.pre_tiles = (int)up((int64_t)a.n_rows * a.group, a.pre_rows);
     const int64_t pre_per = std::max<int64_t>(1, up(want, (int64_t)std::max(a.pre_tiles, 1) * a.nkv));
-    a.pre_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.prefix, 1), pre_per), G_TP) * G_TP);
+    a.pre_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.prefix, 1), pre_per), 64) * 64);
     a.n_pre = (int)up(a.prefix, a.pre_chunk);
     const int64_t own_per = std::max<int64_t>(1, up(want, (int64_t)std::max(a.n_seqs, 1) * a.nkv));
-    a.own_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.cap, 1), own_per), G_TP) * G_TP);
+    a.own_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.cap, 1), own_per), 64) * 64);
     a.n_own = a.n_seqs ? (int)up(a.cap, a.own_chunk) : 0;
 }
 
@@ -277,14 +586,37 @@ size_t ws_bytes_of(const AttnArgs &a) {
     return ml_bytes(a) + (size_t)(a.n_pre + a.n_own) * a.n_rows * a.nh * a.hd * sizeof(float);
 }
 
+// Whether the tensor-core kernels can take the call: whole 16-byte pieces in
+// every cache row, and rows of whole pieces apart.
+bool pieces(const AttnArgs &a, size_t size) {
+    auto whole = [&](int64_t elems) { return elems * (int64_t)size % 16 == 0; };
+    auto ptr = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return whole(a.hd) && whole(a.ppos) && whole(a.phead) && whole(a.opos) && whole(a.ohead) && whole(a.oseq) &&
+           ptr(a.pk) && ptr(a.pv) && ptr(a.ok) && ptr(a.ov);
+}
+
+template <class K> cudaError_t launch_items(K kern, size_t smem, int items, int threads, const AttnArgs &a, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    kern<<<dim3(items, a.nkv), threads, smem, st>>>(a);
+    count_launch();
+    return cudaSuccess;
+}
+
 template <class T> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
-    const size_t smem = (size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * sizeof(float);
     const int items = a.n_pre * a.pre_tiles + a.n_seqs * a.n_own;
     if (items) {
-        cudaError_t e = cudaFuncSetAttribute(k_attn_shared_any<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e;
+        if (!pieces(a, sizeof(T)))
+            e = launch_items(k_attn_shared_any<T>, (size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * 4,
+                             items, G_WARPS * 32, a, st);
+        else if (a.hd <= 64)
+            e = launch_items(k_attn_shared_mma<T, 64>, mma_smem<T, 64>(), items, 128, a, st);
+        else if (a.hd <= 128)
+            e = launch_items(k_attn_shared_mma<T, 128>, mma_smem<T, 128>(), items, 128, a, st);
+        else
+            e = launch_items(k_attn_shared_mma<T, 256>, mma_smem<T, 256>(), items, 128, a, st);
         if (e != cudaSuccess) return e;
-        k_attn_shared_any<T><<<dim3(items, a.nkv), G_WARPS * 32, smem, st>>>(a);
-        count_launch();
     }
     k_attn_shared_join<T><<<(unsigned)(((int64_t)a.n_rows * a.nh + 3) / 4), 128, 0, st>>>(a);
     count_launch();
