@@ -595,12 +595,12 @@ bool pieces(const AttnArgs &a, size_t size) {
            ptr(a.pk) && ptr(a.pv) && ptr(a.ok) && ptr(a.ov);
 }
 
-template <class K> cudaError_t launch_items(K kern, size_t smem, int items, int threads, const AttnArgs &a, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <auto K> cudaError_t launch_items(size_t smem, int items, int threads, const AttnArgs &a, cudaStream_t st) {
+    cudaError_t e = allow_smem<K>(smem);
     if (e != cudaSuccess) return e;
-    kern<<<dim3(items, a.nkv), threads, smem, st>>>(a);
+    K<<<dim3(items, a.nkv), threads, smem, st>>>(a);
     count_launch();
-    return cudaSuccess;
+    return cudaGetLastError();
 }
 
 template <class T> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
@@ -608,14 +608,14 @@ template <class T> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
     if (items) {
         cudaError_t e;
         if (!pieces(a, sizeof(T)))
-            e = launch_items(k_attn_shared_any<T>, (size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * 4,
+            e = launch_items<k_attn_shared_any<T>>((size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * 4,
                              items, G_WARPS * 32, a, st);
         else if (a.hd <= 64)
-            e = launch_items(k_attn_shared_mma<T, 64>, mma_smem<T, 64>(), items, 128, a, st);
+            e = launch_items<k_attn_shared_mma<T, 64>>(mma_smem<T, 64>(), items, 128, a, st);
         else if (a.hd <= 128)
-            e = launch_items(k_attn_shared_mma<T, 128>, mma_smem<T, 128>(), items, 128, a, st);
+            e = launch_items<k_attn_shared_mma<T, 128>>(mma_smem<T, 128>(), items, 128, a, st);
         else
-            e = launch_items(k_attn_shared_mma<T, 256>, mma_smem<T, 256>(), items, 128, a, st);
+            e = launch_items<k_attn_shared_mma<T, 256>>(mma_smem<T, 256>(), items, 128, a, st);
         if (e != cudaSuccess) return e;
     }
     k_attn_shared_join<T><<<(unsigned)(((int64_t)a.n_rows * a.nh + 3) / 4), 128, 0, st>>>(a);

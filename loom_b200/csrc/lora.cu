@@ -314,7 +314,7 @@ template <class T> cudaError_t launch(const LoraArgs &a, cudaStream_t st) {
         if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     }
     const size_t smem = (size_t)L_RB * (a.max_rank + 36) * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(k_lora_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem<k_lora_expand<T>>(smem);
     if (e != cudaSuccess) return e;
     const dim3 grid(blocks, groups, (a.n_out + L_OUT - 1) / L_OUT);
     if (a.n_adapters) return launch_pdl_(k_lora_expand<T>, grid, dim3(128), smem, st, a);

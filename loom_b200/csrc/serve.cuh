@@ -36,6 +36,18 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Let kernel K use `smem` bytes of dynamic shared memory; the driver is asked only
+// when a launch needs more than K's earlier ones on the device did.
+template <auto K> cudaError_t allow_smem(size_t smem) {
+    static size_t most[16] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 16 && most[dev] >= smem)) return e;
+    e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && dev < 16) most[dev] = smem;
+    return e;
+}
+
 // f(T{}) with the element type behind a type id (checked by the caller)
 template <class F> auto by_type(int type, F f) {
     return type == T_F32 ? f(float{}) : type == T_F16 ? f(__half{}) : f(__nv_bfloat16{});

@@ -24,12 +24,29 @@
 namespace loom {
 namespace {
 
-struct RowStat {
-    float top;     // largest logit that is not NaN; -inf when none is above it
-    float z;       // sum of e^((l - top) / T)
-    int arg;       // its first index
-    int pad;
+constexpr int V_C = 8, V_W = 16, V_T = V_W * 32;  // CTAs of a cluster, warps of a CTA
+
+// What a row's cluster leaves: every CTA's part, read as one by row_stat
+struct RowParts {
+    double z[V_C];   // sums of e^((l - top) / T)
+    int arg[V_C];    // first index of the largest logit (greedy rows)
+    float top;       // the largest logit that is not NaN; -inf when none is above it
+    int pad[7];
 };
+struct RowStat {
+    float top, z;
+    int arg;
+};
+__device__ __forceinline__ RowStat row_stat(const RowParts *p) {
+    double z = 0.0;
+    int arg = 0x7FFFFFFF;
+#pragma unroll
+    for (int c = 0; c < V_C; c++) {
+        z += p->z[c];
+        arg = min(arg, p->arg[c]);
+    }
+    return {p->top, (float)z, arg == 0x7FFFFFFF ? 0 : arg};
+}
 
 struct VerifyArgs {
     const void *logits;
@@ -38,7 +55,7 @@ struct VerifyArgs {
     const uint32_t *seq_rows;
     int32_t *out, *n_out;
     float *logprobs;
-    RowStat *stat;
+    RowParts *stat;
     int64_t logits_stride, probs_stride;
     int n_seqs, n_rows, vocab;
 };
@@ -51,6 +68,12 @@ __device__ __forceinline__ float weight(float l, float top, float inv) {
     if (l == top) return top == -INFINITY ? 0.0f : 1.0f;
     const float e = expf(fmul(fsub(l, top), inv));
     return e == e ? e : 0.0f;
+}
+
+// The same where top is finite and inv is too: e^0 is 1 without asking, and the
+// maximum with zero drops a NaN.
+__device__ __forceinline__ float weight_finite(float l, float top, float inv) {
+    return fmaxf(expf(fmul(fsub(l, top), inv)), 0.0f);
 }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -77,7 +100,6 @@ __device__ __forceinline__ int seq_of(const VerifyArgs &a, int r) {
 // row crosses the memory once although the weights need its maximum; longer rows
 // read the rest again. A row that does not start on 16 bytes is shifted: its first
 // piece holds fewer logits.
-constexpr int V_C = 8, V_W = 16, V_T = V_W * 32;
 template <class T> constexpr int v_nv() { return sizeof(T) == 4 ? 10 : 5; }
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -85,8 +107,11 @@ __device__ __forceinline__ unsigned cluster_rank() {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 // the address in CTA `rank` of a variable of this CTA's shared memory
 __device__ __forceinline__ uint32_t peer(const void *p, unsigned rank) {
@@ -94,15 +119,14 @@ __device__ __forceinline__ uint32_t peer(const void *p, unsigned rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
     return r;
 }
-__device__ __forceinline__ uint64_t peer_ld(uint32_t a) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+__device__ __forceinline__ float peer_ldf(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
-
-__device__ __forceinline__ int peer_ld32(uint32_t a) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+__device__ __forceinline__ double peer_ldd(uint32_t a) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
     return v;
 }
 
@@ -151,85 +175,111 @@ template <class T> struct RowPieces {
     }
 };
 
-// One cluster per row: the largest logit and its first index, then the sum of the
-// weights. Bound by reading the logits once.
+// One cluster per row: the largest logit, then every CTA's sum of the weights (the
+// parts meet in row_stat, so the cluster meets once, for the maximum). Reading the
+// logits once would take 14 us for 366 rows of 129,281 bf16; what bounds it is
+// issuing about 20 instructions per logit, half of them e^x.
+//
+// A thread's sum is as exact as a 64-bit one without its conversions: a weight in
+// [0, 1] is cut at 2^-16; its 40 upper parts add exactly in f32 (below 2^8), the
+// lower ones, 2^-17 each, with an error below 2^-31.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_rows(VerifyArgs a) {
-    __shared__ uint64_t s_best[V_W], s_cta;
-    __shared__ double s_sum[V_W], s_z;
-    constexpr int V_NV = v_nv<T>();
+    __shared__ float s_best[V_W], s_cta;
+    __shared__ double s_sum[V_W];
+    __shared__ int s_arg;
+    constexpr int V_NV = v_nv<T>(), N = Piece<T>::N;
     pdl_trigger_();
     const int r = blockIdx.x / V_C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const RowPieces<T> row(static_cast<const T *>(a.logits) + r * a.logits_stride, a.vocab);
-    const float inv = inv_temp(temp_of(a, seq_of(a, r)));
     Piece<T> keep[V_NV];
     const int steps = row.steps();
 #pragma unroll
     for (int j = 0; j < V_NV; j++)
         if (j < steps) keep[j] = row.load(j);
-    // the best of (logit, lowest index) as one number: order-preserving bits of the
-    // logit above the complement of the index
+    const float temp = temp_of(a, seq_of(a, r)), inv = inv_temp(temp);
     float top = -INFINITY;
-    int arg = -1;
-    auto look = [&](const Piece<T> &p, int j) {
+    auto look = [&](const Piece<T> &p) {
 #pragma unroll
-        for (int k = 0; k < Piece<T>::N; k++) {
-            const float v = p.get(k);
-            if (v > top) {
-                top = v;
-                arg = row.base(j) + k;
-            }
-        }
+        for (int k = 0; k < N; k++) top = fmaxf(top, p.get(k));  // of a NaN and a number, the number
     };
 #pragma unroll
     for (int j = 0; j < V_NV; j++)
-        if (j < steps) look(keep[j], j);
-    for (int j = V_NV; j < steps; j++) look(row.load(j), j);
-    const uint32_t bits = __float_as_uint(top + 0.0f);  // -0 and 0 are equal
-    uint64_t best = arg < 0 ? 0 : ((uint64_t)(bits & 0x80000000u ? ~bits : bits | 0x80000000u) << 32) | (uint32_t)~arg;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)best, o));
-    if (lane == 0) s_best[warp] = best;
+        if (j < steps) look(keep[j]);
+    for (int j = V_NV; j < steps; j++) look(row.load(j));
+    top = warp_max(top);
+    if (lane == 0) s_best[warp] = top;
+    if (tid == 0) s_arg = 0x7FFFFFFF;
     __syncthreads();
-    best = s_best[0];
-    for (int w = 1; w < V_W; w++) best = max(best, s_best[w]);
-    if (tid == 0) s_cta = best;
+    if (warp == 0) {
+        top = warp_max(lane < V_W ? s_best[lane] : -INFINITY);
+        if (lane == 0) s_cta = top;
+    }
     cluster_sync();
-    for (unsigned c = 0; c < V_C; c++) best = max(best, peer_ld(peer(&s_cta, c)));
-    const uint32_t hi = (uint32_t)(best >> 32);
-    top = best ? __uint_as_float(hi & 0x80000000u ? hi & 0x7FFFFFFFu : ~hi) : -INFINITY;
+    top = warp_max(peer_ldf(peer(&s_cta, lane % V_C)));
+    cluster_arrive();  // a peer leaves once all have read its shared memory
+    float hi = 0.0f, lo = 0.0f;
     double z = 0.0;
-    auto add = [&](const Piece<T> &p) {
+    if (isfinite(top) && isfinite(inv)) {
+        auto add = [&](const Piece<T> &p) {
 #pragma unroll
-        for (int k = 0; k < Piece<T>::N; k++) z += weight(p.get(k), top, inv);
-    };
+            for (int k = 0; k < N; k++) {
+                const float e = weight_finite(p.get(k), top, inv);
+                const float up = fsub(fadd(e, 128.0f), 128.0f);  // e rounded to a multiple of 2^-16
+                hi += up;
+                lo += e - up;
+            }
+        };
 #pragma unroll
-    for (int j = 0; j < V_NV; j++)
-        if (j < steps) add(keep[j]);
-    for (int j = V_NV; j < steps; j++) add(row.load(j));
+        for (int j = 0; j < V_NV; j++)
+            if (j < steps) add(keep[j]);
+        z = (double)hi + lo;
+        for (int j = V_NV; j < steps; j++) {
+            hi = lo = 0.0f;
+            add(row.load(j));
+            z += (double)hi + lo;
+        }
+    } else {  // nothing above -inf, an infinite logit, a temperature without a finite inverse
+        for (int j = 0; j < steps; j++) {
+            const Piece<T> p = row.load(j);
+#pragma unroll
+            for (int k = 0; k < N; k++) z += weight(p.get(k), top, inv);
+        }
+    }
+    if (temp <= 0.0f && top > -INFINITY) {  // greedy: the first index of the largest
+        int arg = 0x7FFFFFFF;
+        auto find = [&](const Piece<T> &p, int j) {
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (p.get(k) == top) arg = min(arg, row.base(j) + k);
+        };
+#pragma unroll
+        for (int j = 0; j < V_NV; j++)
+            if (j < steps) find(keep[j], j);
+        for (int j = V_NV; j < steps; j++) find(row.load(j), j);
+        if (arg != 0x7FFFFFFF) atomicMin(&s_arg, arg);
+    }
     z = warp_sum_d(z);
     if (lane == 0) s_sum[warp] = z;
     __syncthreads();
     if (tid == 0) {
         z = 0.0;
+#pragma unroll
         for (int w = 0; w < V_W; w++) z += s_sum[w];
-        s_z = z;
+        RowParts &o = a.stat[r];
+        o.z[cluster_rank()] = z;
+        o.arg[cluster_rank()] = s_arg;
+        if (cluster_rank() == 0) o.top = top;
     }
-    cluster_sync();
-    if (tid == 0 && cluster_rank() == 0) {
-        z = 0.0;
-        for (unsigned c = 0; c < V_C; c++) z += __longlong_as_double((long long)peer_ld(peer(&s_z, c)));
-        a.stat[r] = RowStat{top, (float)z, best ? (int)~(uint32_t)best : 0, 0};
-    }
-    cluster_sync();  // the others' shared memory is being read
+    cluster_wait();
 }
 
 // One cluster per sequence: the accepted drafts, then one token. The weights of the
-// row at the refusal are kept in registers while their sums say in which warp's run,
-// which group of 32 pieces and which lane the chosen index lies.
+// row at the refusal stay in registers while the sums of all the cluster's warps
+// say in whose run the chosen index lies; that warp alone looks for it.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 1) k_verify_pick(VerifyArgs a) {
-    __shared__ double s_sum[V_W], s_cta;
-    __shared__ int s_stop, s_first, s_last;
-    constexpr int V_NV = v_nv<T>();
+    __shared__ double s_sum[V_W], s_all[V_C * V_W];
+    __shared__ int s_stop;
+    constexpr int V_NV = v_nv<T>(), N = Piece<T>::N;
     const int b = blockIdx.x / V_C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cluster_rank();
     pdl_wait_();
@@ -241,8 +291,7 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     const float t = temp_of(a, b), inv = inv_temp(t);
     const bool greedy = t <= 0.0f;
     auto row_at = [&](int r) { return static_cast<const T *>(a.logits) + r * a.logits_stride; };
-    auto logp = [&](int r, int tok) {
-        const RowStat s = a.stat[r];
+    auto logp = [&](const RowStat &s, int r, int tok) {
         if (s.z == 0.0f) return -INFINITY;  // a row with nothing above -inf
         const float l = to_f32(row_at(r)[tok]);
         return fsub(l == s.top ? 0.0f : fmul(fsub(l, s.top), inv), logf(s.z));
@@ -255,7 +304,7 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
             bool no = false;
             if (r < r1 - 1) {
                 const int d = a.tokens[r + 1];
-                const RowStat s = a.stat[r];
+                const RowStat s = row_stat(a.stat + r);
                 if (d < 0 || d >= a.vocab)
                     no = true;
                 else if (greedy)
@@ -263,9 +312,9 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
                 else
                     no = !(fmul(a.u[r], a.probs ? a.probs[r * a.probs_stride + d] : 1.0f) <
                            __fdiv_rn(weight(to_f32(row_at(r)[d]), s.top, inv), s.z));
-                if (rank == 0 && !no) {  // a row after a refusal is written again below
+                if (rank == 0 && !no) {  // rows after a refusal are written again below
                     a.out[r] = d;
-                    a.logprobs[r] = logp(r, d);
+                    a.logprobs[r] = logp(s, r, d);
                 }
             }
             const uint32_t m = __ballot_sync(0xffffffffu, no);
@@ -274,134 +323,143 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
                 break;
             }
         }
-        if (lane == 0) {
-            s_stop = stop;
-            s_first = 0x7FFFFFFF;
-            s_last = -1;
-        }
+        if (lane == 0) s_stop = stop;
     }
     __syncthreads();
     const int stop = s_stop;
-    const RowStat s = a.stat[stop];
-    int tok = s.arg;
-    if (!greedy) {
-        const bool full = stop == r1 - 1;
-        const RowPieces<T> row(row_at(stop), a.vocab);
-        const float *q = !full && a.probs ? a.probs + stop * a.probs_stride : nullptr;
-        const int d = full ? -1 : a.tokens[stop + 1];
-        const int steps = row.steps();
-        bool rest = !full;
-        // weight of element i with logit l: max(p - q, 0), or without probabilities
-        // every token but the draft, or (after the last draft, or when the rest is
-        // empty) the target's own
-        auto w_of = [&](float l, int i) {
-            const float e = weight(l, s.top, inv);
-            if (!rest || i < 0 || i >= a.vocab) return e;
-            if (!q) return i == d ? 0.0f : e;
-            const float left = fsub(__fdiv_rn(e, s.z), __ldg(q + i));
-            return left > 0.0f ? left : 0.0f;
-        };
-        constexpr int N = Piece<T>::N;
-        float w[V_NV][N];
-        double mine = 0.0, total = 0.0, before = 0.0;
-        for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
-            mine = 0.0;
+    if (rank == 0)
+        for (int r = stop + 1 + tid; r < r1; r += V_T) {
+            a.out[r] = -1;
+            a.logprobs[r] = 0.0f;
+        }
+    const RowStat s = row_stat(a.stat + stop);
+    auto emit = [&](int tok) {
+        a.out[stop] = tok;
+        a.logprobs[stop] = logp(s, stop, tok);
+        a.n_out[b] = stop - r0 + 1;
+    };
+    if (greedy) {
+        if (tid == 0 && rank == 0) emit(s.arg);
+        return;
+    }
+    const bool full = stop == r1 - 1;
+    const RowPieces<T> row(row_at(stop), a.vocab);
+    const float *q = !full && a.probs ? a.probs + stop * a.probs_stride : nullptr;
+    const int d = full ? -1 : a.tokens[stop + 1];
+    const int steps = row.steps();
+    bool rest = !full;
+    // weight of element i with logit l: max(p - q, 0), or without probabilities every
+    // token but the draft; after the last draft, and when that rest is empty, the
+    // target's own
+    auto w_of = [&](float l, int i) {
+        const float e = weight(l, s.top, inv);
+        if (!rest || i < 0 || i >= a.vocab) return e;
+        if (!q) return i == d ? 0.0f : e;
+        const float left = fsub(__fdiv_rn(e, s.z), __ldg(q + i));
+        return left > 0.0f ? left : 0.0f;
+    };
+    float w[V_NV][N];
+    double upto = 0.0, total = 0.0;  // of the sums of warps 4 lane .. 4 lane + 3, and of all
+    for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
+        double mine = 0.0;
 #pragma unroll
-            for (int j = 0; j < V_NV; j++)
-                if (j < steps) {
-                    const Piece<T> p = row.load(j);
-#pragma unroll
-                    for (int k = 0; k < N; k++) mine += w[j][k] = w_of(p.get(k), row.base(j) + k);
-                }
-            for (int j = V_NV; j < steps; j++) {
+        for (int j = 0; j < V_NV; j++)
+            if (j < steps) {
                 const Piece<T> p = row.load(j);
 #pragma unroll
-                for (int k = 0; k < N; k++) mine += w_of(p.get(k), row.base(j) + k);
+                for (int k = 0; k < N; k++) mine += w[j][k] = w_of(p.get(k), row.base(j) + k);
             }
-            mine = warp_sum_d(mine);
-            __syncthreads();
-            if (lane == 0) s_sum[warp] = mine;
-            __syncthreads();
-            if (tid == 0) {
-                double c = 0.0;
-                for (int k = 0; k < V_W; k++) c += s_sum[k];
-                s_cta = c;
-            }
-            cluster_sync();
-            total = before = 0.0;
-            for (unsigned c = 0; c < V_C; c++) {
-                const double v = __longlong_as_double((long long)peer_ld(peer(&s_cta, c)));
-                if (c < rank) before += v;
-                total += v;
-            }
-            for (int k = 0; k < warp; k++) before += s_sum[k];
-            cluster_sync();  // s_cta has been read
-            if (total > 0.0 || !rest) break;
-            rest = false;
+        for (int j = V_NV; j < steps; j++) {
+            const Piece<T> p = row.load(j);
+#pragma unroll
+            for (int k = 0; k < N; k++) mine += w_of(p.get(k), row.base(j) + k);
         }
-        // The first index whose running sum exceeds the threshold, and the last one
-        // with any weight, which is taken when rounding leaves no such index.
-        const double want = (double)a.u[r1 - 1] * total;
-        int first = 0x7FFFFFFF, last = -1;
-        if (mine > 0.0) {  // the warp has weight; `before` precedes its run
-            double c = before;
-            for (int j = 0; j < steps; j++) {
-                float e[N];
-                if (j < V_NV) {
-#pragma unroll
-                    for (int jj = 0; jj < V_NV; jj++)
-                        if (jj == j) {
-#pragma unroll
-                            for (int k = 0; k < N; k++) e[k] = w[jj][k];
-                        }
-                } else {
-                    const Piece<T> p = row.load(j);
-#pragma unroll
-                    for (int k = 0; k < N; k++) e[k] = w_of(p.get(k), row.base(j) + k);
-                }
-                double sum = 0.0;
-#pragma unroll
-                for (int k = 0; k < N; k++) sum += e[k];
-                double upto = sum;  // over the lanes
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double v = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += v;
-                }
-                double run = c + (upto - sum);
-#pragma unroll
-                for (int k = 0; k < N; k++) {
-                    run += e[k];
-                    if (e[k] > 0.0f) {
-                        last = row.base(j) + k;
-                        if (run > want) first = min(first, last);
-                    }
-                }
-                c += __shfl_sync(0xffffffffu, upto, 31);
-            }
-        }
-        if (first != 0x7FFFFFFF) atomicMin(&s_first, first);
-        if (last >= 0) atomicMax(&s_last, last);
+        mine = warp_sum_d(mine);
+        if (lane == 0) s_sum[warp] = mine;
         cluster_sync();
-        int lo = 0x7FFFFFFF, hi = -1;
-        for (unsigned c = 0; c < V_C && rank == 0; c++) {
-            lo = min(lo, peer_ld32(peer(&s_first, c)));
-            hi = max(hi, peer_ld32(peer(&s_last, c)));
+        if (tid < V_C * V_W) s_all[tid] = peer_ldd(peer(&s_sum[tid % V_W], tid / V_W));
+        cluster_sync();
+        double four = 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) four += s_all[4 * lane + k];
+        upto = four;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
-        tok = lo != 0x7FFFFFFF ? lo : hi >= 0 ? hi : 0;
-        cluster_sync();  // the others' shared memory has been read
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        if (total > 0.0 || !rest) break;
+        rest = false;
     }
-    if (rank != 0) return;
-    __syncthreads();
-    if (tid == 0) {
-        a.out[stop] = tok;
-        a.logprobs[stop] = logp(stop, tok);
-        a.n_out[b] = stop - r0 + 1;
+    // the run with the chosen index: the first whose end exceeds the threshold; the
+    // last one with weight, should none (a random number of 1)
+    const double want = (double)a.u[r1 - 1] * total;
+    double c = __shfl_up_sync(0xffffffffu, upto, 1), before = 0.0;
+    if (lane == 0) c = 0.0;
+    int pick = -1, heavy = -1;
+    double start = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const double v = s_all[4 * lane + k];
+        if (v > 0.0) heavy = 4 * lane + k;
+        if (pick < 0 && v > 0.0 && c + v > want) {
+            pick = 4 * lane + k;
+            start = c;
+        }
+        c += v;
     }
-    for (int r = stop + 1 + tid; r < r1; r += V_T) {
-        a.out[r] = -1;
-        a.logprobs[r] = 0.0f;
+    const uint32_t m = __ballot_sync(0xffffffffu, pick >= 0);
+    if (m) {
+        pick = __shfl_sync(0xffffffffu, pick, __ffs(m) - 1);
+        before = __shfl_sync(0xffffffffu, start, __ffs(m) - 1);
+    } else {
+        pick = __reduce_max_sync(0xffffffffu, heavy);
+        before = total;
     }
+    if (pick < 0) {  // no weight at all
+        if (tid == 0 && rank == 0) emit(0);
+        return;
+    }
+    if (pick != (int)rank * V_W + warp) return;
+    int first = -1, last = -1;
+    auto look = [&](const float (&e)[N], int j) {
+        if (first >= 0) return;
+        double sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < N; k++) sum += e[k];
+        double run = sum;  // over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
+        double at = before + (run - sum);
+        before += __shfl_sync(0xffffffffu, run, 31);
+        int mine = 0x7FFFFFFF;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            at += e[k];
+            if (e[k] > 0.0f) {
+                last = max(last, row.base(j) + k);
+                if (at > want) mine = min(mine, row.base(j) + k);
+            }
+        }
+        mine = __reduce_min_sync(0xffffffffu, mine);
+        if (mine != 0x7FFFFFFF) first = mine;
+    };
+#pragma unroll
+    for (int j = 0; j < V_NV; j++)
+        if (j < steps) look(w[j], j);
+    for (int j = V_NV; j < steps; j++) {
+        const Piece<T> p = row.load(j);
+        float e[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) e[k] = w_of(p.get(k), row.base(j) + k);
+        look(e, j);
+    }
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) emit(first >= 0 ? first : max(last, 0));
 }
 
 const char *check(const loom_verify_desc *d) {
@@ -412,7 +470,7 @@ const char *check(const loom_verify_desc *d) {
     return nullptr;
 }
 
-size_t ws_bytes_of(const loom_verify_desc *d) { return d->n_rows * sizeof(RowStat); }
+size_t ws_bytes_of(const loom_verify_desc *d) { return d->n_rows * sizeof(RowParts); }
 
 template <class T> cudaError_t launch(const VerifyArgs &a, cudaStream_t st) {
     k_verify_rows<T><<<(unsigned)a.n_rows * V_C, V_T, 0, st>>>(a);
@@ -451,7 +509,7 @@ int loom_cuda_verify(const loom_verify_desc *d, const void *d_logits, const floa
     a.out = d_out;
     a.n_out = d_n_out;
     a.logprobs = d_logprobs;
-    a.stat = static_cast<RowStat *>(d_ws);
+    a.stat = static_cast<RowParts *>(d_ws);
     a.logits_stride = (int64_t)d->logits_stride;
     a.probs_stride = (int64_t)d->probs_stride;
     a.n_seqs = (int)d->n_seqs;

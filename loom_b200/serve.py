@@ -12,7 +12,7 @@ in a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -22,41 +22,52 @@ from ._lib import LoomCudaError
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
+_device = -1  # the device a call here brought the backend up on
+
+
 def _need(ok: bool, why: str) -> None:
     if not ok:
         raise LoomCudaError(why)
 
 
-def _typed(op: str, name: str, t, dtype, shape, like, dense: bool = True) -> None:
-    """t is a tensor of this dtype and shape on like's device (dense: contiguous)."""
-    if t.dtype is not dtype or t.shape != shape or t.device != like.device or (dense and not t.is_contiguous()):
-        raise LoomCudaError(f"{op}: {name} must be {'a contiguous ' if dense else ''}{dtype} {tuple(shape)} on "
-                            f"{like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-
-_device = None  # the device the backend was brought up on by a call here
-
-
-def _on(op: str, t) -> None:
+def _on(op: str, t) -> int:
+    """The cuda device of t, on which the backend is up."""
     global _device
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{op}: tensors must be on a cuda device")
-    if t.device != _device:  # bring-up, or the refusal of a second device
-        _lib.must(_lib.lib().loom_cuda_init(t.device.index), op)
-        _device = t.device
-    _need(t.dtype in TYPES, f"{op}: type must be float32, float16 or bfloat16, got {t.dtype}")
+    dev = t.get_device() if isinstance(t, torch.Tensor) else -1
+    _need(dev >= 0, f"{op}: tensors must be on a cuda device")
+    if dev != _device:  # bring-up, or the refusal of a second device
+        _lib.must(_lib.lib().loom_cuda_init(dev), op)
+        _device = dev
+    return dev
 
 
-def _stream(stream, like):
-    cur = torch.cuda.current_stream(like.device).cuda_stream
-    return cur if stream is None else stream, cur
+def _refuse(op: str, dev: int, want: Sequence[tuple]) -> None:
+    """Name the first tensor that is not as wanted: (name, tensor, dtype, shape, strides it must have or None)."""
+    for name, t, dtype, shape, strides in want:
+        if t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == dev and
+                         (strides is None or _laid(t, strides))):
+            continue
+        raise LoomCudaError(f"{op}: {name} must be {dtype} {tuple(shape)} on cuda:{dev}"
+                            f"{'' if strides is None else f' with strides {strides}'}, got {t.dtype} "
+                            f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+    raise LoomCudaError(f"{op}: arguments do not fit together")
 
 
-def _workspace(n: int, like, stream: int, cur: int):
-    """Scratch from torch's allocator, kept from reuse until the call's stream is done with it."""
-    ws = torch.empty(n, dtype=torch.uint8, device=like.device)
-    if stream != cur and n:
-        ws.record_stream(torch.cuda.ExternalStream(stream, device=like.device))
-    return ws
+def _laid(t, strides) -> bool:
+    """The strides of t are these (None: any), where a dimension of more than one element has a say."""
+    return t.numel() == 0 or all(w is None or s == w or n == 1 for s, w, n in zip(t.stride(), strides, t.shape))
+
+
+def _workspace(n: int, dev: int, stream: Optional[int]):
+    """Scratch from torch's allocator (kept from reuse until a stream other than the current one is done with it), and
+    the stream of the call."""
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    cur = torch.cuda.current_stream(dev).cuda_stream
+    if stream is None or stream == cur:
+        return ws, cur
+    if n:
+        ws.record_stream(torch.cuda.ExternalStream(stream, device=dev))
+    return ws, stream
 
 
 def attn_shared(q, prefix_k, prefix_v, own_k, own_v, seq_rows, seq_len, scale: float, out=None,
@@ -64,38 +75,52 @@ def attn_shared(q, prefix_k, prefix_v, own_k, own_v, seq_rows, seq_len, scale: f
     """Attention over a shared prefix cache and each sequence's own cache.
 
     q [rows, heads, hd]; prefix_k/v [prefix, kv_heads, hd]; own_k/v [seqs, cap, kv_heads, hd], all of one type
-    (float32, float16, bfloat16), any strides but a last dimension of 1 (q, out: heads side by side). seq_len (cuda
-    int32 [seqs]) counts each sequence's own positions, this step's rows included: row j of n sees seq_len - (n - 1 - j)
-    of them. Returns out [rows, heads, hd]."""
-    _on("attn_shared", q)
-    n, h, hd = q.shape if q.dim() == 3 else (0, 0, 0)
-    _need(h > 0 and hd > 0 and own_k.dim() == 4 and prefix_k.dim() == 3,
+    (float32, float16, bfloat16), any strides but a last dimension of 1 (q, out: heads side by side; keys and values
+    laid out alike). seq_len (cuda int32 [seqs]) counts each sequence's own positions, this step's rows included: row j
+    of n sees seq_len - (n - 1 - j) of them. Returns out [rows, heads, hd]."""
+    dev = _on("attn_shared", q)
+    _need(q.dim() == 3 and own_k.dim() == 4 and prefix_k.dim() == 3 and q.shape[1] > 0 and q.shape[2] > 0,
           "attn_shared: q [rows, heads, hd], prefix_k/v [prefix, kv, hd], own_k/v [seqs, cap, kv, hd]")
+    ty, qs = q.dtype, q.shape
+    n, h, hd = qs
     seqs, cap, kv, _ = own_k.shape
     pre = prefix_k.shape[0]
-    ty, pst, ost = q.dtype, prefix_k.stride(), own_k.stride()
-    _typed("attn_shared", "prefix_k", prefix_k, ty, (pre, kv, hd), q, False)
-    _typed("attn_shared", "prefix_v", prefix_v, ty, (pre, kv, hd), q, False)
-    _typed("attn_shared", "own_k", own_k, ty, (seqs, cap, kv, hd), q, False)
-    _typed("attn_shared", "own_v", own_v, ty, (seqs, cap, kv, hd), q, False)
-    _typed("attn_shared", "seq_rows", seq_rows, torch.int32, (seqs + 1,), q)
-    _typed("attn_shared", "seq_len", seq_len, torch.int32, (seqs,), q)
+    _need(ty in TYPES, f"attn_shared: type must be float32, float16 or bfloat16, got {ty}")
     if out is None:
-        out = torch.empty((n, h, hd), dtype=ty, device=q.device)
-    _typed("attn_shared", "out", out, ty, (n, h, hd), q, False)
-    qst, dst = q.stride(), out.stride()
-    _need(prefix_v.stride() == pst and own_v.stride() == ost, "attn_shared: keys and values must be laid out alike")
-    _need((pst[2] == 1 or hd == 1) and (ost[3] == 1 or hd == 1) and (qst[2] == 1 or hd == 1) and (dst[2] == 1 or hd == 1)
-          and (qst[1] == hd or h == 1) and (dst[1] == hd or h == 1),
-          "attn_shared: the last dimension must be contiguous, and the heads of q and out side by side")
-    d = _lib.AttnSharedDesc(TYPES[ty], scale, seqs, n, h, kv, hd, qst[0], dst[0], pre, pst[0], pst[1], cap, ost[1],
-                            ost[2], ost[0])
-    L, (st, cur) = _lib.lib(), _stream(stream, q)
-    ref = C.byref(d)
-    ws = _workspace(L.loom_cuda_attn_shared_workspace(ref), q, st, cur)
-    _lib.must(L.loom_cuda_attn_shared(ref, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), own_k.data_ptr(),
-                                      own_v.data_ptr(), seq_rows.data_ptr(), seq_len.data_ptr(), out.data_ptr(),
-                                      ws.data_ptr(), ws.numel(), st), "attn_shared")
+        out = torch.empty(qs, dtype=ty, device=dev)
+    pshape, oshape, i32 = (pre, kv, hd), (seqs, cap, kv, hd), torch.int32
+    pst, ost, qst, dst = prefix_k.stride(), own_k.stride(), q.stride(), out.stride()
+    if not (prefix_k.dtype is ty and prefix_v.dtype is ty and own_k.dtype is ty and own_v.dtype is ty and
+            out.dtype is ty and seq_rows.dtype is i32 and seq_len.dtype is i32 and prefix_k.shape == pshape and
+            prefix_v.shape == pshape and own_k.shape == oshape and own_v.shape == oshape and out.shape == qs and
+            seq_rows.shape == (seqs + 1,) and seq_len.shape == (seqs,) and
+            dev == prefix_k.get_device() == prefix_v.get_device() == own_k.get_device() == own_v.get_device() ==
+            out.get_device() == seq_rows.get_device() == seq_len.get_device() and
+            pst[2] == ost[3] == qst[2] == dst[2] == 1 and qst[1] == dst[1] == hd and prefix_v.stride() == pst and
+            own_v.stride() == ost and seq_rows.is_contiguous() and seq_len.is_contiguous()):
+        heads, one = (None, hd, 1), (1,)
+        like = lambda t, u: _laid(u, t.stride()) and _laid(t, u.stride())  # noqa: E731
+        if not (_laid(q, heads) and _laid(out, heads) and _laid(prefix_k, (None, None, 1)) and
+                _laid(own_k, (None, None, None, 1)) and like(prefix_k, prefix_v) and like(own_k, own_v) and
+                all(t.dtype is d and t.shape == s and t.get_device() == dev for t, d, s in (
+                    (prefix_k, ty, pshape), (prefix_v, ty, pshape), (own_k, ty, oshape), (own_v, ty, oshape),
+                    (out, ty, qs), (seq_rows, i32, (seqs + 1,)), (seq_len, i32, (seqs,)))) and
+                _laid(seq_rows, one) and _laid(seq_len, one)):
+            _refuse("attn_shared", dev, (
+                ("q", q, ty, qs, heads), ("out", out, ty, qs, heads), ("prefix_k", prefix_k, ty, pshape, (None, None, 1)),
+                ("prefix_v", prefix_v, ty, pshape, pst), ("own_k", own_k, ty, oshape, (None, None, None, 1)),
+                ("own_v", own_v, ty, oshape, ost), ("seq_rows", seq_rows, i32, (seqs + 1,), one),
+                ("seq_len", seq_len, i32, (seqs,), one)))
+    ref = C.byref(_lib.AttnSharedDesc(TYPES[ty], scale, seqs, n, h, kv, hd, qst[0], dst[0], pre, pst[0], pst[1], cap,
+                                      ost[1], ost[2], ost[0]))
+    L = _lib.lib()
+    need = L.loom_cuda_attn_shared_workspace(ref)
+    ws, st = _workspace(need, dev, stream)
+    rc = L.loom_cuda_attn_shared(ref, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), own_k.data_ptr(),
+                                 own_v.data_ptr(), seq_rows.data_ptr(), seq_len.data_ptr(), out.data_ptr(),
+                                 ws.data_ptr(), need, st)
+    if rc:
+        _lib.must(rc, "attn_shared")
     return out
 
 
@@ -105,32 +130,42 @@ def lora(x, a, b, ranks, scales, ids, base=None, out=None, stream: Optional[int]
     x [rows, n_in] float32; a [adapters, max_rank, n_in], b [adapters, n_out, max_rank] of one type (float32, float16,
     bfloat16); ranks (int32) and scales (float32) [adapters]; ids int32 [rows]; base, out [rows, n_out] float32 (base
     None: zeros; out may be base). Last dimensions contiguous. Returns out."""
-    _on("lora", a)
+    dev = _on("lora", a)
     _need(a.dim() == 3 and b.dim() == 3 and x.dim() == 2, "lora: x [rows, n_in], a [n, rank, n_in], b [n, n_out, rank]")
+    ty, f32, i32 = a.dtype, torch.float32, torch.int32
     na, rank, nin = a.shape
     n, nout = x.shape[0], b.shape[1]
-    f32 = torch.float32
-    _typed("lora", "x", x, f32, (n, nin), a, False)
-    _typed("lora", "b", b, a.dtype, (na, nout, rank), a, False)
-    _typed("lora", "ranks", ranks, torch.int32, (na,), a)
-    _typed("lora", "scales", scales, f32, (na,), a)
-    _typed("lora", "ids", ids, torch.int32, (n,), a)
-    if base is not None:
-        _typed("lora", "base", base, f32, (n, nout), a, False)
+    _need(ty in TYPES, f"lora: type must be float32, float16 or bfloat16, got {ty}")
     if out is None:
-        out = torch.empty((n, nout), dtype=f32, device=a.device)
-    _typed("lora", "out", out, f32, (n, nout), a, False)
+        out = torch.empty((n, nout), dtype=f32, device=dev)
     xst, ast, bst, dst = x.stride(), a.stride(), b.stride(), out.stride()
     cst = dst if base is None else base.stride()
-    _need((xst[1] == 1 or nin == 1) and (ast[2] == 1 or nin == 1) and (bst[2] == 1 or rank == 1) and
-          ((dst[1] == 1 and cst[1] == 1) or nout == 1), "lora: the last dimension must be contiguous")
-    d = _lib.LoraDesc(TYPES[a.dtype], n, nin, nout, na, rank, xst[0], cst[0], dst[0], ast[1], ast[0], bst[1], bst[0])
-    L, (st, cur) = _lib.lib(), _stream(stream, a)
-    ref = C.byref(d)
-    ws = _workspace(L.loom_cuda_lora_workspace(ref), a, st, cur)
-    _lib.must(L.loom_cuda_lora(ref, x.data_ptr(), a.data_ptr(), b.data_ptr(), ranks.data_ptr(), scales.data_ptr(),
-                               ids.data_ptr(), None if base is None else base.data_ptr(), out.data_ptr(),
-                               ws.data_ptr(), ws.numel(), st), "lora")
+    bshape, oshape = (na, nout, rank), (n, nout)
+    if not (x.dtype is f32 and b.dtype is ty and ranks.dtype is i32 and scales.dtype is f32 and ids.dtype is i32 and
+            out.dtype is f32 and x.shape == (n, nin) and b.shape == bshape and ranks.shape == (na,) and
+            scales.shape == (na,) and ids.shape == (n,) and out.shape == oshape and
+            dev == x.get_device() == b.get_device() == ranks.get_device() == scales.get_device() == ids.get_device() ==
+            out.get_device() and
+            (base is None or (base.dtype is f32 and base.shape == oshape and base.get_device() == dev)) and
+            xst[1] == ast[2] == bst[2] == dst[1] == cst[1] == 1 and ranks.is_contiguous() and scales.is_contiguous() and
+            ids.is_contiguous()):
+        want = (("x", x, f32, (n, nin), (None, 1)), ("a", a, ty, (na, rank, nin), (None, None, 1)),
+                ("b", b, ty, bshape, (None, None, 1)), ("ranks", ranks, i32, (na,), (1,)),
+                ("scales", scales, f32, (na,), (1,)), ("ids", ids, i32, (n,), (1,)),
+                ("base", base, f32, oshape, (None, 1)), ("out", out, f32, oshape, (None, 1)))
+        if not all(t is None or (t.dtype is d and t.shape == s and t.get_device() == dev and _laid(t, w))
+                   for _, t, d, s, w in want):
+            _refuse("lora", dev, want)
+    ref = C.byref(_lib.LoraDesc(TYPES[ty], n, nin, nout, na, rank, xst[0], cst[0], dst[0], ast[1], ast[0], bst[1],
+                                bst[0]))
+    L = _lib.lib()
+    need = L.loom_cuda_lora_workspace(ref)
+    ws, st = _workspace(need, dev, stream)
+    rc = L.loom_cuda_lora(ref, x.data_ptr(), a.data_ptr(), b.data_ptr(), ranks.data_ptr(), scales.data_ptr(),
+                          ids.data_ptr(), None if base is None else base.data_ptr(), out.data_ptr(), ws.data_ptr(),
+                          need, st)
+    if rc:
+        _lib.must(rc, "lora")
     return out
 
 
@@ -143,36 +178,46 @@ def verify(logits, tokens, seq_rows, u, temperature=None, draft_probs=None, out=
     float32 [rows, vocab], row r what the token after row r was drawn from (None: drafts without chance).
     Returns (token after each row or -1 [rows] int32, tokens per sequence [seqs] int32, log-probabilities [rows]);
     `out` gives those three buffers."""
-    _on("verify", logits)
-    _need(logits.dim() == 2, "verify: logits must be [rows, vocab]")
+    dev = _on("verify", logits)
+    _need(logits.dim() == 2 and seq_rows.numel() > 0, "verify: logits [rows, vocab], seq_rows [seqs + 1]")
+    ty, f32, i32 = logits.dtype, torch.float32, torch.int32
     n, v = logits.shape
     seqs = seq_rows.numel() - 1
-    _need(seqs >= 0, "verify: seq_rows must be [seqs + 1]")
-    f32, i32 = torch.float32, torch.int32
-    _typed("verify", "tokens", tokens, i32, (n,), logits)
-    _typed("verify", "seq_rows", seq_rows, i32, (seqs + 1,), logits)
-    _typed("verify", "u", u, f32, (n,), logits)
-    if temperature is not None:
-        _typed("verify", "temperature", temperature, f32, (seqs,), logits)
-    if draft_probs is not None:
-        _typed("verify", "draft_probs", draft_probs, f32, (n, v), logits, False)
-        _need(draft_probs.stride(1) == 1 or v == 1, "verify: the last dimension must be contiguous")
-    _need(logits.stride(1) == 1 or v == 1, "verify: the last dimension must be contiguous")
+    _need(ty in TYPES, f"verify: type must be float32, float16 or bfloat16, got {ty}")
     if out is None:
-        dev = logits.device
         out = (torch.empty(n, dtype=i32, device=dev), torch.empty(seqs, dtype=i32, device=dev),
                torch.empty(n, dtype=f32, device=dev))
     tok, cnt, lp = out
-    _typed("verify", "out tokens", tok, i32, (n,), logits)
-    _typed("verify", "out counts", cnt, i32, (seqs,), logits)
-    _typed("verify", "out logprobs", lp, f32, (n,), logits)
-    d = _lib.VerifyDesc(TYPES[logits.dtype], seqs, n, v, logits.stride(0),
-                        0 if draft_probs is None else draft_probs.stride(0))
-    L, (st, cur) = _lib.lib(), _stream(stream, logits)
-    ref = C.byref(d)
-    ws = _workspace(L.loom_cuda_verify_workspace(ref), logits, st, cur)
-    _lib.must(L.loom_cuda_verify(ref, logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
-                                 tokens.data_ptr(), seq_rows.data_ptr(), u.data_ptr(),
-                                 None if temperature is None else temperature.data_ptr(), tok.data_ptr(),
-                                 cnt.data_ptr(), lp.data_ptr(), ws.data_ptr(), ws.numel(), st), "verify")
+    lst = logits.stride()
+    pst = (0, 1) if draft_probs is None else draft_probs.stride()
+    rows, per = (n,), (seqs,)
+    if not (tokens.dtype is i32 and seq_rows.dtype is i32 and u.dtype is f32 and tok.dtype is i32 and cnt.dtype is i32 and
+            lp.dtype is f32 and tokens.shape == rows and seq_rows.dim() == 1 and u.shape == rows and tok.shape == rows and
+            cnt.shape == per and lp.shape == rows and
+            dev == tokens.get_device() == seq_rows.get_device() == u.get_device() == tok.get_device() ==
+            cnt.get_device() == lp.get_device() and
+            (temperature is None or (temperature.dtype is f32 and temperature.shape == per and
+                                     temperature.get_device() == dev and temperature.is_contiguous())) and
+            (draft_probs is None or (draft_probs.dtype is f32 and draft_probs.shape == (n, v) and
+                                     draft_probs.get_device() == dev)) and
+            lst[1] == pst[1] == 1 and tokens.is_contiguous() and seq_rows.is_contiguous() and u.is_contiguous() and
+            tok.is_contiguous() and cnt.is_contiguous() and lp.is_contiguous()):
+        want = (("logits", logits, ty, (n, v), (None, 1)), ("tokens", tokens, i32, rows, (1,)),
+                ("seq_rows", seq_rows, i32, (seqs + 1,), (1,)), ("u", u, f32, rows, (1,)),
+                ("temperature", temperature, f32, per, (1,)), ("draft_probs", draft_probs, f32, (n, v), (None, 1)),
+                ("out tokens", tok, i32, rows, (1,)), ("out counts", cnt, i32, per, (1,)),
+                ("out logprobs", lp, f32, rows, (1,)))
+        if not all(t is None or (t.dtype is d and t.shape == s and t.get_device() == dev and _laid(t, w))
+                   for _, t, d, s, w in want):
+            _refuse("verify", dev, want)
+    ref = C.byref(_lib.VerifyDesc(TYPES[ty], seqs, n, v, lst[0], pst[0]))
+    L = _lib.lib()
+    need = L.loom_cuda_verify_workspace(ref)
+    ws, st = _workspace(need, dev, stream)
+    rc = L.loom_cuda_verify(ref, logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
+                            tokens.data_ptr(), seq_rows.data_ptr(), u.data_ptr(),
+                            None if temperature is None else temperature.data_ptr(), tok.data_ptr(), cnt.data_ptr(),
+                            lp.data_ptr(), ws.data_ptr(), need, st)
+    if rc:
+        _lib.must(rc, "verify")
     return out
