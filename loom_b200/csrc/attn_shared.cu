@@ -106,6 +106,7 @@ constexpr int G_TP = 32, G_TR = 16, G_WARPS = 4;
 template <class T>
 __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
     extern __shared__ float sm[];
+    pdl_trigger_();
     const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     float *sq = sm, *sk = sq + G_TR * hd, *sv = sk + G_TP * (hd + 1), *ss = sv + G_TP * hd;
     const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
@@ -212,6 +213,7 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
     constexpr int KS = F ? 1 : HDP / 16;       // query fragments held in registers (16-bit types)
     extern __shared__ __align__(16) uint8_t smb[];
     __shared__ float s_m[4][16], s_l[4][16];
+    pdl_trigger_();
     const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kvh = blockIdx.y;
     const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
@@ -262,9 +264,9 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
         cp_async_commit();
         uint32_t qf[KS][4];
         if constexpr (F) {
-            for (int i = tid; i < 64 * wide; i += 128) {
-                const int j = i / wide, d = i % wide;
-                sq[j * QST + d] = j < rows && d < hd ? reinterpret_cast<const float *>(q_row(rb + j))[d] : 0.0f;
+            for (int j = warp; j < (rows + 15) / 16 * 16; j += 4) {
+                const float *src = reinterpret_cast<const float *>(q_row(min(rb + j, it.r1 - 1)));
+                for (int d = lane; d < wide; d += 32) sq[j * QST + d] = j < rows && d < hd ? src[d] : 0.0f;
             }
         } else {
 #pragma unroll
@@ -476,61 +478,111 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
 }
 
 // ---- join ----------------------------------------------------------------------
-// One warp per (row, head): the parts of the chunks, then the own rows that not
-// every row of the sequence sees, then the division. A row that sees nothing
-// gives zeros.
-template <class T> __global__ void __launch_bounds__(128) k_attn_shared_join(AttnArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t rh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (rh >= (int64_t)a.n_rows * a.nh) return;
+// WPH warps per (row, head), one warp where the parts are few: their maxima and
+// sums a lane each, then the parts weighted by e^(m - M), eight in flight; then the
+// own rows that not every row of the sequence sees, and the division. A row that
+// sees nothing gives zeros. Bound by reading the parts.
+template <class T, int WPH> __global__ void __launch_bounds__(128) k_attn_shared_join(AttnArgs a) {
+    constexpr int ND = MAX_HD / 32;
+    __shared__ float s_acc[WPH > 1 ? 4 : 1][MAX_HD];
+    __shared__ float2 s_ml[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPH;
+    const int64_t rh = (int64_t)blockIdx.x * (4 / WPH) + warp / WPH;
+    if (rh >= (int64_t)a.n_rows * a.nh) {
+        pdl_wait_();
+        return;
+    }
     const int r = (int)(rh / a.nh), h = (int)(rh % a.nh), kvh = h / a.group;
     // the sequence of row r: the last b with seq_rows[b] <= r
     int lo = 0, hi = a.n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if ((int)min(a.seq_rows[mid], 0x7FFFFFFFu) <= r) lo = mid; else hi = mid;
+        if (a.seq_rows[mid] <= (uint32_t)r) lo = mid; else hi = mid;
     }
     const int b = lo;
     SeqView s = {0, 0, 0, 0};
     if (a.n_seqs) s = seq_view(a, b);
     const bool mine = r >= s.row0 && r < s.row0 + s.rows;
-    const int own = mine ? (s.common + a.own_chunk - 1) / a.own_chunk : 0;
-    const int tail = mine ? max(s.len - (s.row0 + s.rows - 1 - r), 0) : 0;  // own positions this row sees
-    float m = -INFINITY, l = 0.0f, acc[MAX_HD / 32];
+    const int n = a.n_pre + (mine ? (s.common + a.own_chunk - 1) / a.own_chunk : 0);
+    const int see = mine ? max(s.len - (s.row0 + s.rows - 1 - r), 0) : 0;  // own positions this row sees
+    float acc[ND], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int d = 0; d < MAX_HD / 32; d++) acc[d] = 0.0f;
-    const int n = a.n_pre + own;
-    for (int i = 0; i < n; i++) {
-        const size_t at = ((size_t)i * a.n_rows + r) * a.nh + h;
-        const float2 p = a.ml[at];
-        if (p.y == 0.0f) continue;  // nothing but weights of zero (a NaN goes on)
-        const float mn = fmaxf(m, p.x), fa = exp2f(m - mn), fb = exp2f(p.x - mn);
-        l = l * fa + p.y * fb;
-        m = mn;
+    for (int d = 0; d < ND; d++) acc[d] = 0.0f;
+    const int64_t step = (int64_t)a.n_rows * a.nh;  // (row, head) pairs from part to part
+    pdl_wait_();
+    for (int i0 = 0; i0 < n; i0 += 32 * WPH) {
+        const int i = i0 + lane * WPH + part;
+        const float2 p = i < n ? a.ml[i * step + rh] : make_float2(-INFINITY, 0.0f);
+        const float top = fmaxf(m, warp_max(p.y == 0.0f ? -INFINITY : p.x));
+        const float base = top == -INFINITY ? 0.0f : top;
+        // a part of zero weight counts for nothing; a NaN goes on
+        const float f = p.y == 0.0f ? 0.0f : ex2(p.x - base), fix = ex2(m - base);
+        l = l * fix + warp_sum(p.y * f);
+        m = top;
 #pragma unroll
-        for (int d = 0; d < MAX_HD / 32; d++)
-            if (d * 32 + lane < a.hd) acc[d] = acc[d] * fa + a.acc[at * a.hd + d * 32 + lane] * fb;
+        for (int d = 0; d < ND; d++) acc[d] *= fix;
+        const int here = min(32, (n - i0 - part + WPH - 1) / WPH);
+        const float *src = a.acc + ((i0 + part) * step + rh) * a.hd + lane;
+        for (int j0 = 0; j0 < here; j0 += 8) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                if (d * 32 >= a.hd) break;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const bool in = j0 + j < here && d * 32 + lane < a.hd;
+                    v[j] = in ? __ldcg(src + (int64_t)(j0 + j) * WPH * step * a.hd + d * 32) : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+                    if (j0 + j < here && w != 0.0f) acc[d] = fmaf(v[j], w, acc[d]);
+                }
+            }
+        }
+    }
+    if constexpr (WPH > 1) {
+        if (lane == 0) s_ml[warp] = make_float2(m, l);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            if (d * 32 + lane < a.hd) s_acc[warp][d * 32 + lane] = acc[d];
+        __syncthreads();
+        if (part) return;
+        float top = -INFINITY;
+        for (int w = 0; w < WPH; w++) top = fmaxf(top, s_ml[w].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        m = top;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) acc[d] = 0.0f;
+        for (int w = 0; w < WPH; w++) {
+            const float f = s_ml[w].y == 0.0f ? 0.0f : ex2(s_ml[w].x - base);
+            l += s_ml[w].y * f;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                if (d * 32 + lane < a.hd) acc[d] += s_acc[w][d * 32 + lane] * f;
+        }
     }
     const T *q = static_cast<const T *>(a.q) + r * a.q_stride + (int64_t)h * a.hd;
-    for (int p = s.common; p < tail; p++) {
+    for (int p = s.common; p < see; p++) {
         const T *k = static_cast<const T *>(a.ok) + b * a.oseq + p * a.opos + kvh * a.ohead;
         const T *v = static_cast<const T *>(a.ov) + b * a.oseq + p * a.opos + kvh * a.ohead;
         float x = 0.0f;
 #pragma unroll
-        for (int d = 0; d < MAX_HD / 32; d++)
+        for (int d = 0; d < ND; d++)
             if (d * 32 + lane < a.hd) x = fmaf(to_f32(q[d * 32 + lane]) * a.scale, to_f32(k[d * 32 + lane]), x);
         x = warp_sum(x);
         if (x == -INFINITY) continue;
-        const float mn = fmaxf(m, x), fa = exp2f(m - mn), fb = exp2f(x - mn);
+        const float mn = fmaxf(m, x), fa = ex2(m - mn), fb = ex2(x - mn);
         l = l * fa + fb;
         m = mn;
 #pragma unroll
-        for (int d = 0; d < MAX_HD / 32; d++)
+        for (int d = 0; d < ND; d++)
             if (d * 32 + lane < a.hd) acc[d] = acc[d] * fa + to_f32(v[d * 32 + lane]) * fb;
     }
     T *out = static_cast<T *>(a.out) + r * a.out_stride + (int64_t)h * a.hd;
 #pragma unroll
-    for (int d = 0; d < MAX_HD / 32; d++)
+    for (int d = 0; d < ND; d++)
         if (d * 32 + lane < a.hd) out[d * 32 + lane] = from_f32<T>(l != 0.0f ? acc[d] / l : 0.0f);
 }
 
@@ -618,7 +670,15 @@ template <class T> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
             e = launch_items<k_attn_shared_mma<T, 256>>(mma_smem<T, 256>(), items, 128, a, st);
         if (e != cudaSuccess) return e;
     }
-    k_attn_shared_join<T><<<(unsigned)(((int64_t)a.n_rows * a.nh + 3) / 4), 128, 0, st>>>(a);
+    // Four warps share a (row, head) where one would read many parts in turn and the
+    // rows alone leave SMs idle.
+    const int64_t pairs = (int64_t)a.n_rows * a.nh;
+    const bool four = a.n_pre + a.n_own > 16 && pairs < 4 * 4 * 148;
+    const dim3 grid((unsigned)(four ? pairs : (pairs + 3) / 4));
+    if (items)
+        return four ? launch_pdl_(k_attn_shared_join<T, 4>, grid, dim3(128), 0, st, a)
+                    : launch_pdl_(k_attn_shared_join<T, 1>, grid, dim3(128), 0, st, a);
+    k_attn_shared_join<T, 1><<<grid, 128, 0, st>>>(a);  // reads seq_rows before its wait: only behind its own kernel
     count_launch();
     return cudaGetLastError();
 }

@@ -70,12 +70,6 @@ __device__ __forceinline__ float weight(float l, float top, float inv) {
     return e == e ? e : 0.0f;
 }
 
-// The same where top is finite and inv is too: e^0 is 1 without asking, and the
-// maximum with zero drops a NaN.
-__device__ __forceinline__ float weight_finite(float l, float top, float inv) {
-    return fmaxf(expf(fmul(fsub(l, top), inv)), 0.0f);
-}
-
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -130,6 +124,47 @@ __device__ __forceinline__ double peer_ldd(uint32_t a) {
     return v;
 }
 
+// two f32 at once (one issue slot, each half rounded as by itself)
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+// A sum of weights in [0, 1] as exact as a 64-bit one, without its conversions:
+// each is cut at 2^-16; the upper parts, up to 256 of them, add exactly in f32, the
+// lower ones, 2^-17 at most, with an error below 2^-31.
+struct Sum01 {
+    F2 hi = f2(0.0f, 0.0f), lo = f2(0.0f, 0.0f);
+    __device__ __forceinline__ void add(F2 e) {
+        const F2 up = (e + f2(128.0f, 128.0f)) + f2(-128.0f, -128.0f);
+        hi = hi + up;
+        lo = lo + (e + up * f2(-1.0f, -1.0f));
+    }
+    __device__ __forceinline__ double get() const {
+        const float2 h = split(hi), l = split(lo);
+        return ((double)h.x + h.y) + ((double)l.x + l.y);
+    }
+};
+
 template <class T> struct Piece {
     static constexpr int N = 16 / sizeof(T);
     uint4 raw;
@@ -142,7 +177,18 @@ template <class T> struct Piece {
             if constexpr (std::is_same<T, __half>::value)
                 return __half2float(__ushort_as_half(h));
             else
-                return __bfloat162float(__ushort_as_bfloat16(h));
+                return __uint_as_float(k % 2 ? w[k / 2] & 0xFFFF0000u : w[k / 2] << 16);
+        }
+    }
+    // the largest, of a NaN and a number the number
+    __device__ __forceinline__ float max(float top) const {
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(top, fmaxf(get(0), get(1))), fmaxf(get(2), get(3)));
+        } else {
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            auto two = [](uint32_t v) { return *reinterpret_cast<const T2 *>(&v); };
+            const T2 m = __hmax2(__hmax2(two(raw.x), two(raw.y)), __hmax2(two(raw.z), two(raw.w)));
+            return fmaxf(top, fmaxf(to_f32(m.x), to_f32(m.y)));
         }
     }
 };
@@ -179,10 +225,6 @@ template <class T> struct RowPieces {
 // parts meet in row_stat, so the cluster meets once, for the maximum). Reading the
 // logits once would take 14 us for 366 rows of 129,281 bf16; what bounds it is
 // issuing about 20 instructions per logit, half of them e^x.
-//
-// A thread's sum is as exact as a 64-bit one without its conversions: a weight in
-// [0, 1] is cut at 2^-16; its 40 upper parts add exactly in f32 (below 2^8), the
-// lower ones, 2^-17 each, with an error below 2^-31.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_rows(VerifyArgs a) {
     __shared__ float s_best[V_W], s_cta;
     __shared__ double s_sum[V_W];
@@ -198,14 +240,10 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         if (j < steps) keep[j] = row.load(j);
     const float temp = temp_of(a, seq_of(a, r)), inv = inv_temp(temp);
     float top = -INFINITY;
-    auto look = [&](const Piece<T> &p) {
-#pragma unroll
-        for (int k = 0; k < N; k++) top = fmaxf(top, p.get(k));  // of a NaN and a number, the number
-    };
 #pragma unroll
     for (int j = 0; j < V_NV; j++)
-        if (j < steps) look(keep[j]);
-    for (int j = V_NV; j < steps; j++) look(row.load(j));
+        if (j < steps) top = keep[j].max(top);
+    for (int j = V_NV; j < steps; j++) top = row.load(j).max(top);
     top = warp_max(top);
     if (lane == 0) s_best[warp] = top;
     if (tid == 0) s_arg = 0x7FFFFFFF;
@@ -217,26 +255,25 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     cluster_sync();
     top = warp_max(peer_ldf(peer(&s_cta, lane % V_C)));
     cluster_arrive();  // a peer leaves once all have read its shared memory
-    float hi = 0.0f, lo = 0.0f;
     double z = 0.0;
-    if (isfinite(top) && isfinite(inv)) {
-        auto add = [&](const Piece<T> &p) {
+    if (isfinite(top) && isfinite(inv)) {  // then e^0 is 1 without asking
+        const F2 top2 = f2(-top, -top), inv2 = f2(inv, inv);
+        auto add = [&](Sum01 &s, const Piece<T> &p) {
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                const float e = weight_finite(p.get(k), top, inv);
-                const float up = fsub(fadd(e, 128.0f), 128.0f);  // e rounded to a multiple of 2^-16
-                hi += up;
-                lo += e - up;
+            for (int k = 0; k < N; k += 2) {
+                const float2 x = split((f2(p.get(k), p.get(k + 1)) + top2) * inv2);
+                s.add(f2(fmaxf(expf(x.x), 0.0f), fmaxf(expf(x.y), 0.0f)));  // the maximum drops a NaN
             }
         };
+        Sum01 s;
 #pragma unroll
         for (int j = 0; j < V_NV; j++)
-            if (j < steps) add(keep[j]);
-        z = (double)hi + lo;
+            if (j < steps) add(s, keep[j]);
+        z = s.get();
         for (int j = V_NV; j < steps; j++) {
-            hi = lo = 0.0f;
-            add(row.load(j));
-            z += (double)hi + lo;
+            Sum01 rest;
+            add(rest, row.load(j));
+            z += rest.get();
         }
     } else {  // nothing above -inf, an infinite logit, a temperature without a finite inverse
         for (int j = 0; j < steps; j++) {
@@ -273,13 +310,13 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     cluster_wait();
 }
 
-// One cluster per sequence: the accepted drafts, then one token. The weights of the
-// row at the refusal stay in registers while the sums of all the cluster's warps
-// say in whose run the chosen index lies; that warp alone looks for it.
-template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 1) k_verify_pick(VerifyArgs a) {
+// One cluster per sequence: the accepted drafts, then one token. The sums of the
+// weights over the runs of all the cluster's warps say in whose run the chosen
+// index lies; that warp alone goes through its run again, and finds it.
+template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_pick(VerifyArgs a) {
     __shared__ double s_sum[V_W], s_all[V_C * V_W];
     __shared__ int s_stop;
-    constexpr int V_NV = v_nv<T>(), N = Piece<T>::N;
+    constexpr int N = Piece<T>::N;
     const int b = blockIdx.x / V_C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cluster_rank();
     pdl_wait_();
@@ -358,21 +395,23 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         const float left = fsub(__fdiv_rn(e, s.z), __ldg(q + i));
         return left > 0.0f ? left : 0.0f;
     };
-    float w[V_NV][N];
     double upto = 0.0, total = 0.0;  // of the sums of warps 4 lane .. 4 lane + 3, and of all
     for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
         double mine = 0.0;
+        for (int j0 = 0; j0 < steps; j0 += 4) {
+            Piece<T> p[4];
 #pragma unroll
-        for (int j = 0; j < V_NV; j++)
-            if (j < steps) {
-                const Piece<T> p = row.load(j);
+            for (int j = 0; j < 4; j++) p[j] = row.load(j0 + j);  // past the run: past the row, or unused
+            Sum01 s;
 #pragma unroll
-                for (int k = 0; k < N; k++) mine += w[j][k] = w_of(p.get(k), row.base(j) + k);
-            }
-        for (int j = V_NV; j < steps; j++) {
-            const Piece<T> p = row.load(j);
+            for (int j = 0; j < 4; j++)
+                if (j0 + j < steps)
 #pragma unroll
-            for (int k = 0; k < N; k++) mine += w_of(p.get(k), row.base(j) + k);
+                    for (int k = 0; k < N; k += 2) {
+                        const int i = row.base(j0 + j) + k;
+                        s.add(f2(w_of(p[j].get(k), i), w_of(p[j].get(k + 1), i + 1)));
+                    }
+            mine += s.get();
         }
         mine = warp_sum_d(mine);
         if (lane == 0) s_sum[warp] = mine;
@@ -424,7 +463,6 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     if (pick != (int)rank * V_W + warp) return;
     int first = -1, last = -1;
     auto look = [&](const float (&e)[N], int j) {
-        if (first >= 0) return;
         double sum = 0.0;
 #pragma unroll
         for (int k = 0; k < N; k++) sum += e[k];
@@ -448,10 +486,7 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         mine = __reduce_min_sync(0xffffffffu, mine);
         if (mine != 0x7FFFFFFF) first = mine;
     };
-#pragma unroll
-    for (int j = 0; j < V_NV; j++)
-        if (j < steps) look(w[j], j);
-    for (int j = V_NV; j < steps; j++) {
+    for (int j = 0; j < steps && first < 0; j++) {
         const Piece<T> p = row.load(j);
         float e[N];
 #pragma unroll
