@@ -18,84 +18,17 @@
 // row. The chunk kernels then have one length for a whole sequence and no mask
 // but that length, and a cache row that a query may not see never meets it, not
 // even as 0 times infinity.
-#include <cfloat>
+#include <algorithm>
+#include <type_traits>
 
 #include "../../include/loom_cuda.h"
-#include "mma.cuh"
-#include "serve.cuh"
+#include "attn_shared.cuh"
 
 namespace loom {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_HD = 256;
-
-struct AttnArgs {
-    const void *q, *pk, *pv, *ok, *ov;
-    void *out;
-    const uint32_t *seq_rows, *seq_len;
-    // parts: [slot][row][head] (m, l) pairs and [slot][row][head][hd] sums; the
-    // prefix's n_pre slots come first, then the n_own slots of the row's own cache
-    float2 *ml;
-    float *acc;
-    int64_t q_stride, out_stride, ppos, phead, opos, ohead, oseq;
-    int n_seqs, n_rows, nh, nkv, group, hd;
-    int prefix, cap;
-    int pre_chunk, own_chunk, n_pre, n_own, pre_tiles, pre_rows;
-    float scale;  // of the scores in base 2: scale * log2(e)
-};
-
-// A sequence's rows and the own positions that all of them see; every value is
-// held to the call's sizes, so wrong device arrays give wrong numbers, not
-// addresses outside the tensors.
-struct SeqView {
-    int row0, rows, len, common;
-};
-__device__ __forceinline__ SeqView seq_view(const AttnArgs &a, int b) {
-    SeqView s;
-    s.row0 = (int)min(a.seq_rows[b], (uint32_t)a.n_rows);
-    s.rows = max((int)min(a.seq_rows[b + 1], (uint32_t)a.n_rows) - s.row0, 0);
-    s.len = (int)min(a.seq_len[b], (uint32_t)a.cap);
-    s.common = max(s.len - max(s.rows - 1, 0), 0);
-    return s;
-}
-
-// A CTA's work: query rows r0 .. r1-1 (row * group + head of the group) of one KV
-// head against positions p0 .. p1-1 of a cache, and the slot for the parts.
-template <class T> struct Item {
-    int slot, r0, r1, p0, p1;
-    const T *k, *v;
-    int64_t pos_stride;
-};
-template <class T> __device__ __forceinline__ Item<T> item_of(const AttnArgs &a, int item, int kvh) {
-    Item<T> o;
-    if (item < a.n_pre * a.pre_tiles) {
-        o.slot = item / a.pre_tiles;
-        o.r0 = (item % a.pre_tiles) * a.pre_rows;
-        o.r1 = min(o.r0 + a.pre_rows, a.n_rows * a.group);
-        o.p0 = o.slot * a.pre_chunk;
-        o.p1 = min(o.p0 + a.pre_chunk, a.prefix);
-        o.pos_stride = a.ppos;
-        o.k = static_cast<const T *>(a.pk) + kvh * a.phead;
-        o.v = static_cast<const T *>(a.pv) + kvh * a.phead;
-    } else {
-        item -= a.n_pre * a.pre_tiles;
-        const int b = item / a.n_own, c = item % a.n_own;
-        const SeqView s = seq_view(a, b);
-        o.slot = a.n_pre + c;
-        o.r0 = s.row0 * a.group;
-        o.r1 = o.r0 + s.rows * a.group;
-        o.p0 = c * a.own_chunk;
-        o.p1 = min(o.p0 + a.own_chunk, s.common);
-        o.pos_stride = a.opos;
-        o.k = static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead;
-        o.v = static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead;
-    }
-    return o;
-}
-__device__ __forceinline__ size_t part_at(const AttnArgs &a, int slot, int hr, int kvh) {
-    return ((size_t)slot * a.n_rows + hr / a.group) * a.nh + kvh * a.group + hr % a.group;
-}
 
 // ---- any shape ---------------------------------------------------------------
 // One CTA per chunk of positions and KV head. 32 positions at a time go to
@@ -109,11 +42,14 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
     pdl_trigger_();
     const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     float *sq = sm, *sk = sq + G_TR * hd, *sv = sk + G_TP * (hd + 1), *ss = sv + G_TP * hd;
-    const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
+    const Item<T> it = item_of<T>(a, a.first + blockIdx.x, kvh);
     const int slot = it.slot, r0 = it.r0, r1 = it.r1, p0 = it.p0, p1 = it.p1;
     const T *kb = it.k, *vb = it.v;
     const int64_t ps = it.pos_stride;
-    if (p0 >= p1) return;  // the join does not read this slot
+    if (p0 >= p1) {  // the join does not read this slot
+        pdl_wait_();
+        return;
+    }
     for (int t0 = r0; t0 < r1; t0 += G_TR) {
         __syncthreads();
         for (int i = tid; i < G_TR * hd; i += G_WARPS * 32) {
@@ -182,6 +118,7 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
                 if (d * 32 + lane < hd) a.acc[at * hd + d * 32 + lane] = acc[j][d];
         }
     }
+    pdl_wait_();
 }
 
 // ---- tensor cores, a few query rows per tile ------------------------------------
@@ -216,8 +153,11 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
     pdl_trigger_();
     const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kvh = blockIdx.y;
-    const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
-    if (it.p0 >= it.p1) return;  // the join does not read this slot
+    const Item<T> it = item_of<T>(a, a.first + blockIdx.x, kvh);
+    if (it.p0 >= it.p1) {  // the join does not read this slot
+        pdl_wait_();
+        return;
+    }
     auto stage_k = [&](int s) { return reinterpret_cast<T *>(smb + s * mma_stage<T, HDP>()); };
     auto stage_v = [&](int s) { return stage_k(s) + TP * KST; };
     float *sq = reinterpret_cast<float *>(smb + maxz(2 * mma_stage<T, HDP>(), (size_t)64 * HDP * 4));
@@ -475,6 +415,7 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
             }
         }
     }
+    pdl_wait_();  // the join waits for this kernel, and through it for the prefix's
 }
 
 // ---- join ----------------------------------------------------------------------
@@ -600,6 +541,13 @@ const char *check(const loom_attn_shared_desc *d) {
     return nullptr;
 }
 
+// Whether the prefix goes to attn_prefix.cu, as far as the call's sizes say: 16-bit
+// types, dimensions that fit its tiles, and rows enough for them.
+bool prefix_tc(const loom_attn_shared_desc *d) {
+    return d->type != T_F32 && d->head_dim <= 128 && d->head_dim % 8 == 0 && d->scale >= 0.0f && d->prefix_len &&
+           d->n_rows * (d->n_heads / d->n_kv_heads) > 64;
+}
+
 // The cut of the positions. Chunks are sized so that prefix and own items
 // together give the GPU a few CTAs per SM, no smaller than 64 positions.
 void plan(const loom_attn_shared_desc *d, AttnArgs &a) {
@@ -621,10 +569,18 @@ void plan(const loom_attn_shared_desc *d, AttnArgs &a) {
     a.oseq = (int64_t)d->own_seq_stride;
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     const int want = 6 * 148;
-    a.pre_rows = 64;
-    a.pre_tiles = (int)up((int64_t)a.n_rows * a.group, a.pre_rows);
-    const int64_t pre_per = std::max<int64_t>(1, up(want, (int64_t)std::max(a.pre_tiles, 1) * a.nkv));
-    a.pre_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.prefix, 1), pre_per), 64) * 64);
+    const int64_t rows = std::max<int64_t>((int64_t)a.n_rows * a.group, 1);
+    if (prefix_tc(d)) {  // one CTA per SM, one round of them
+        a.pre_tiles = (int)up(rows, 256);
+        a.pre_rows = (int)up(rows, a.pre_tiles);
+        const int64_t per = std::max<int64_t>(1, 148 / ((int64_t)a.pre_tiles * a.nkv));
+        a.pre_chunk = (int)(up(up(std::max(a.prefix, 1), per), 128) * 128);
+    } else {
+        a.pre_rows = 64;
+        a.pre_tiles = (int)up(rows, a.pre_rows);
+        const int64_t per = up(want, (int64_t)a.pre_tiles * a.nkv);
+        a.pre_chunk = (int)(up(up(std::max(a.prefix, 1), per), 64) * 64);
+    }
     a.n_pre = (int)up(a.prefix, a.pre_chunk);
     const int64_t own_per = std::max<int64_t>(1, up(want, (int64_t)std::max(a.n_seqs, 1) * a.nkv));
     a.own_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.cap, 1), own_per), 64) * 64);
@@ -650,18 +606,26 @@ bool pieces(const AttnArgs &a, size_t size) {
 template <auto K> cudaError_t launch_items(size_t smem, int items, int threads, const AttnArgs &a, cudaStream_t st) {
     cudaError_t e = allow_smem<K>(smem);
     if (e != cudaSuccess) return e;
+    // beside the prefix's kernel where that came before (neither reads what the other writes)
+    if (a.first) return launch_pdl_(K, dim3(items, a.nkv), dim3(threads), smem, st, a);
     K<<<dim3(items, a.nkv), threads, smem, st>>>(a);
     count_launch();
     return cudaGetLastError();
 }
 
-template <class T> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
-    const int items = a.n_pre * a.pre_tiles + a.n_seqs * a.n_own;
-    if (items) {
-        cudaError_t e;
-        if (!pieces(a, sizeof(T)))
+template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
+    const int all = a.n_pre * a.pre_tiles + a.n_seqs * a.n_own;
+    const bool whole = pieces(a, sizeof(T));
+    cudaError_t e = cudaSuccess;
+    if constexpr (sizeof(T) == 2)
+        if (tc && whole && attn_prefix_run(std::is_same<T, __half>::value ? T_F16 : T_BF16, a, st, &e)) {
+            if (e != cudaSuccess) return e;
+            a.first = a.n_pre * a.pre_tiles;
+        }
+    if (const int items = all - a.first) {
+        if (!whole)
             e = launch_items<k_attn_shared_any<T>>((size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * 4,
-                             items, G_WARPS * 32, a, st);
+                                                   items, G_WARPS * 32, a, st);
         else if (a.hd <= 64)
             e = launch_items<k_attn_shared_mma<T, 64>>(mma_smem<T, 64>(), items, 128, a, st);
         else if (a.hd <= 128)
@@ -675,7 +639,7 @@ template <class T> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
     const int64_t pairs = (int64_t)a.n_rows * a.nh;
     const bool four = a.n_pre + a.n_own > 16 && pairs < 4 * 4 * 148;
     const dim3 grid((unsigned)(four ? pairs : (pairs + 3) / 4));
-    if (items)
+    if (all)
         return four ? launch_pdl_(k_attn_shared_join<T, 4>, grid, dim3(128), 0, st, a)
                     : launch_pdl_(k_attn_shared_join<T, 1>, grid, dim3(128), 0, st, a);
     k_attn_shared_join<T, 1><<<grid, 128, 0, st>>>(a);  // reads seq_rows before its wait: only behind its own kernel
@@ -721,7 +685,7 @@ int loom_cuda_attn_shared(const loom_attn_shared_desc *d, const void *d_q, const
     a.seq_len = d_seq_len;
     a.ml = static_cast<float2 *>(d_ws);
     a.acc = reinterpret_cast<float *>(static_cast<uint8_t *>(d_ws) + ml_bytes(a));
-    const cudaError_t e = by_type(d->type, [&](auto t) { return launch<decltype(t)>(a, rt_stream(stream)); });
+    const cudaError_t e = by_type(d->type, [&](auto t) { return launch<decltype(t)>(a, prefix_tc(d), rt_stream(stream)); });
     return e == cudaSuccess ? LOOM_CUDA_OK : rt_fail("attn_shared", e);
 }
 

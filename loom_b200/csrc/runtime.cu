@@ -17,6 +17,7 @@
 
 #include "../../include/loom_cuda.h"
 #include "attn.cuh"
+#include "attn_shared.cuh"
 #include "gemv.cuh"
 #include "decode.cuh"
 #include "ep.cuh"
@@ -845,10 +846,11 @@ size_t loom_cuda_trace_read(uint64_t *out, size_t n_kernels) {
 }
 
 int loom_cuda_device_error(void) {
-    if (!g_inited || !S.counters.p) return 0;
-    int v = 0;
-    // the error word sits after the counters of the last layer shape reserved
+    if (!g_inited) return 0;
     if (cudaStreamSynchronize(g_stream) != cudaSuccess) return -1;
+    int v = attn_prefix_error();
+    if (v < 0 || !S.counters.p) return v;
+    // the error word sits after the counters of the last layer shape reserved
     std::vector<int> all(S.counters.cap / 4);
     if (cudaMemcpy(all.data(), S.counters.p, all.size() * 4, cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
     for (int x : all) v |= x;
