@@ -5,24 +5,28 @@
 // values (512 bytes of a KV head) meet all the batch's query rows of the head's
 // group, so beyond about 100 rows the arithmetic, not the memory, takes the time.
 // A CTA has up to 256 query rows (two tiles of 128, the height of an MMA) and a
-// chunk of positions, 128 at a time:
+// chunk of positions, 64 at a time:
 //
-//   S = Q K^T   both from shared memory, into TMEM (128 lanes = rows, 128 columns)
+//   S = Q K^T   both from shared memory, into TMEM (128 lanes = rows, 64 columns)
 //   P = 2^(scale S - m)   by the row's thread: maximum, exponentials, sum, P in the
 //               element type back into TMEM in S's place
 //   O += P V    P from TMEM, V from shared memory as it lies (positions x
 //               dimensions: the operand with the summed dimension outermost)
 //
-// The two tiles take turns: while the threads of one are at their exponentials, the
-// tensor core has the other's products, each about 1,024 cycles of either. O stays
-// in TMEM; it is scaled when a row's maximum has grown by more than 2^8 over the
-// one in use (the quotient by the sum undoes any common factor, and f32 has room),
-// so after the first positions hardly ever.
+// A tile has two S (and a barrier of each kind for each: its threads may be a step
+// ahead of the products), so the products of the next positions are made while its
+// threads are at their exponentials (64 a row and step, 16 an SM and cycle: the
+// bound, beside the products' own 2,048 cycles per 128 positions of two tiles). O
+// stays in TMEM; it is scaled when a row's maximum has grown by more than 2^8 over
+// the one in use (the quotient by the sum undoes any common factor, and f32 has
+// room), so after the first positions hardly ever.
 //
 // Roles (320 threads, one CTA per SM: all 512 TMEM columns): warps 0-3 and 4-7 the
-// rows of tile 0 and 1, warp 8 the copies (TMA, keys and values in turn through a
-// ring of four 32 KB stages), warp 9 the MMAs. P is rounded to the element type as
-// in attn_shared.cu. Every wait is bounded; one that gives up sets an error word
+// rows of tile 0 and 1, warp 8 the copies (TMA, 64 positions of keys or values
+// each, through a ring of six 16 KB stages), warp 9 the MMAs. The ring's size and
+// 112 registers a thread leave room on the SM for a CTA of the own caches' kernel,
+// which is bound by memory where this one is not. P is rounded to the element type
+// as in attn_shared.cu. Every wait is bounded; one that gives up sets an error word
 // (bit 128 of loom_cuda_device_error), leaves NaN in the CTA's rows and ends.
 #include <cuda.h>  // CUtensorMap (the encoder is reached through the runtime's driver entry point)
 
@@ -34,13 +38,14 @@
 namespace loom {
 namespace {
 
-constexpr int AP_THREADS = 320, AP_N = 128, AP_STAGES = 4;
-constexpr size_t AP_BLOCK = 128 * 128;           // 128 rows of 64 elements, swizzled in 128-byte rows
-constexpr uint32_t AP_POLLS = 1u << 20;
+constexpr int AP_THREADS = 320, AP_N = 64, AP_STAGES = 6;
+constexpr size_t AP_QBLOCK = 128 * 128;          // 128 rows of 64 elements, swizzled in 128-byte rows
+constexpr size_t AP_BLOCK = AP_N * 128;          // the same of 64 positions
+constexpr uint32_t AP_POLLS = 64, AP_TRIES = 1 << 14;  // polls between looks at the CTA's error flag, and looks
 constexpr float AP_LAZY = 8.0f;                  // log2 of the growth that scales O
 
 struct ApBars {
-    uint64_t full[AP_STAGES], empty[AP_STAGES], s_full[2], p_full[2], o_full[2];
+    uint64_t full[AP_STAGES], empty[AP_STAGES], s_full[2][2], p_full[2][2], o_done[2][2];  // [tile][step & 1]
     uint64_t drain;
     uint32_t tmem;
     int err, issued;  // a wait gave up; copies issued
@@ -48,8 +53,8 @@ struct ApBars {
 
 __device__ int g_ap_err;  // a wait of any launch gave up
 
-template <int NB> constexpr size_t ap_smem() {  // queries of two tiles, the ring, barriers, alignment
-    return (2 + AP_STAGES) * NB * AP_BLOCK + sizeof(ApBars) + 1024;
+template <int NB> constexpr size_t ap_smem() {  // queries of two tiles, the ring, barriers
+    return NB * (2 * AP_QBLOCK + AP_STAGES * AP_BLOCK) + sizeof(ApBars);
 }
 
 // 128-byte-swizzled tile, the summed dimension along the rows' 128 bytes
@@ -67,6 +72,15 @@ __device__ __forceinline__ uint64_t ap_desc_mn(uint32_t addr) {
 template <class T> __device__ __forceinline__ uint32_t ap_idesc(int n, bool b_rows) {
     const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)b_rows << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Products are issued by one lane: the warp runs the issuing loop and its waits as a
+// whole and branches on this only around the products, so that the descriptors stay
+// in uniform registers (a loop run by one lane alone moves them there before every
+// product, which took longer than the product).
+__device__ __forceinline__ bool ap_elect() {
+    uint32_t q;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(q));
+    return q != 0;
 }
 __device__ __forceinline__ void ap_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
     umma_bf16(d, a, b, idesc, acc);
@@ -106,38 +120,65 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
         AP_I8(r, 8), "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+#define AP_W8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+// the reads so far are done; the registers are named so that no use of them moves above the wait
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : AP_W8(r, 0), AP_W8(r, 8), AP_W8(r, 16), AP_W8(r, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : AP_W8(r, 0), AP_W8(r, 8)::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ap_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// columns from `left` on are no positions
+__device__ __forceinline__ void ap_mask(uint32_t (&s)[32], int left) {
+    if (left >= 32) return;
+#pragma unroll
+    for (int k = 0; k < 32; k++)
+        if (k >= left) s[k] = 0xFF800000u;  // -inf
+}
+
 // NB: blocks of 64 dimensions (head_dim <= 64 NB)
 template <class T, int NB>
-__global__ void __launch_bounds__(AP_THREADS, 1)
+__global__ void __maxnreg__(112)
     k_attn_prefix(AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
-    extern __shared__ uint8_t ap_raw[];
+    extern __shared__ __align__(1024) uint8_t smp[];  // the swizzle's atoms are 1 KB
     pdl_trigger_();
-    const uint32_t sm0 = (smem_u32(ap_raw) + 1023) & ~1023u;
-    uint8_t *smp = ap_raw + (sm0 - smem_u32(ap_raw));
-    const uint32_t ring = sm0 + 2 * NB * AP_BLOCK;
-    ApBars &B = *reinterpret_cast<ApBars *>(smp + (2 + AP_STAGES) * NB * AP_BLOCK);
+    const uint32_t sm0 = smem_u32(smp);
+    const uint32_t ring = sm0 + 2 * NB * AP_QBLOCK;
+    ApBars &B = *reinterpret_cast<ApBars *>(smp + NB * (2 * AP_QBLOCK + AP_STAGES * AP_BLOCK));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, hd = a.hd;
     const Item<T> it = item_of<T>(a, blockIdx.x, kvh);
     const int n = (it.p1 - it.p0 + AP_N - 1) / AP_N, rows = it.r1 - it.r0, tiles = rows > 128 ? 2 : 1;
     volatile int *err = &B.err;
-    auto wait = [&](uint64_t *bar, uint32_t parity) {
-        if (*err) return false;
-        if (mbar_wait_hint(bar, parity, AP_POLLS, 2000)) return true;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {  // false once any wait of the CTA has given up
+        for (int i = 0; i < AP_TRIES; i++) {
+            if (mbar_wait(bar, parity, AP_POLLS)) return true;
+            if (*err) return false;
+        }
         *err = 1;
         return false;
     };
-    auto fetch = [&](int i) {  // item i of the ring: keys (even) or values of 128 positions
+    // The ring's items in the order of their use: keys 0 and 1, then values j and keys
+    // j + 2 for every step j. Item i of the list, of which there are 2 n, is of
+    // keys or values of step `pos`.
+    auto item_pos = [&](int i, bool &values) {
+        const int lead = min(n, 2);
+        values = i >= lead && (i - lead < 2 * (n - lead) ? (i - lead) % 2 == 0 : true);
+        if (i < lead) return i;
+        return i - lead < 2 * (n - lead) ? (i - lead) / 2 + (values ? 0 : lead) : (n - lead) + (i - lead - 2 * (n - lead));
+    };
+    auto fetch = [&](int i) {
         const int s = i % AP_STAGES;
+        bool values;
+        const int pos = item_pos(i, values);
         mbar_expect_tx(&B.full[s], (uint32_t)(NB * AP_BLOCK));
         B.issued = i + 1;
         for (int b = 0; b < NB; b++)
-            ap_tma(ring + (uint32_t)((s * NB + b) * AP_BLOCK), i & 1 ? &mv : &mk, b * 64, it.p0 + (i >> 1) * AP_N, kvh, &B.full[s]);
+            ap_tma(ring + (uint32_t)((s * NB + b) * AP_BLOCK), values ? &mv : &mk, b * 64, it.p0 + pos * AP_N, kvh, &B.full[s]);
     };
     if (warp == 8 && lane == 0) {
         for (int s = 0; s < AP_STAGES; s++) {
@@ -145,9 +186,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             mbar_init_nf(&B.empty[s], 1);
         }
         for (int t = 0; t < 2; t++) {
-            mbar_init_nf(&B.s_full[t], 1);
-            mbar_init_nf(&B.p_full[t], 128);
-            mbar_init_nf(&B.o_full[t], 1);
+            for (int b = 0; b < 2; b++) {
+                mbar_init_nf(&B.s_full[t][b], 1);
+                mbar_init_nf(&B.p_full[t][b], 128);
+                mbar_init_nf(&B.o_done[t][b], 1);
+            }
         }
         mbar_init_nf(&B.drain, 1);
         B.err = 0;
@@ -173,7 +216,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
         }
         const int tl = j >> 7, r = j & 127;
-        *reinterpret_cast<uint4 *>(smp + (size_t)(tl * NB + c / 8) * AP_BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        *reinterpret_cast<uint4 *>(smp + (size_t)(tl * NB + c / 8) * AP_QBLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
     }
     fence_async_smem();
     tc_fence_before();
@@ -188,78 +231,106 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
         __syncwarp();
     } else if (warp == 9) {
-        if (lane == 0) {
-            const uint32_t id_s = ap_idesc<T>(AP_N, false), id_o = ap_idesc<T>((hd + 15) / 16 * 16, true);
-            const int ks = (hd + 15) / 16;
-            auto qk = [&](int t, int j) {  // S_t = Q_t K(j)^T
-                const uint32_t q = sm0 + (uint32_t)(t * NB * AP_BLOCK), k = ring + (uint32_t)((2 * j % AP_STAGES) * NB * AP_BLOCK);
-                for (int s = 0; s < ks; s++) {
-                    const uint32_t off = (uint32_t)((s >> 2) * AP_BLOCK + (s & 3) * 32);
-                    ap_mma_ss(tmem + t * 128, ap_desc_k(q + off), ap_desc_k(k + off), id_s, s > 0);
-                }
-                umma_commit(&B.s_full[t]);
-            };
-            auto item = [&](int i) { return wait(&B.full[i % AP_STAGES], (i / AP_STAGES) & 1); };
-            bool ok = item(0);
-            tc_fence_after();
-            for (int t = 0; t < tiles && ok; t++) qk(t, 0);
-            if (ok) umma_commit(&B.empty[0]);
-            for (int j = 0; j < n && ok; j++) {
-                ok = item(2 * j + 1) && (j + 1 >= n || item(2 * j + 2));
-                const uint32_t v = ring + (uint32_t)(((2 * j + 1) % AP_STAGES) * NB * AP_BLOCK);
-                for (int t = 0; t < tiles && ok; t++) {
-                    ok = wait(&B.p_full[t], j & 1);
-                    if (!ok) break;
-                    tc_fence_after();
+        // 24 products a step. A wait that gives up does not end the loop (its bound
+        // holds for all together: after one the others return at once).
+        const uint32_t id_s = ap_idesc<T>(AP_N, false), id_o = ap_idesc<T>((hd + 15) / 16 * 16, true);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int ks = (hd + 15) / 16;
+        const uint64_t dq = ap_desc_k(sm0), dk = ap_desc_k(ring), dv = ap_desc_mn(ring);
+        constexpr uint32_t STAGE = NB * AP_BLOCK >> 4;  // in the descriptors' 16 bytes
+        int st = 0;                                     // the ring's present stage
+        uint32_t ph = 0;                                // and its parity
+        auto step = [&]() {
+            if (++st == AP_STAGES) {
+                st = 0;
+                ph ^= 1;
+            }
+        };
+        // the tiles' products alternate: one that adds to the result of the one before
+        // it waits for that to leave the pipe
+        auto qk = [&](int b) {  // S = Q K^T of both tiles, keys in the present stage
+            const uint64_t k = dk + (uint32_t)st * STAGE;
+            const uint32_t d = tm + b * 64;
+            if (!ap_elect()) return;
 #pragma unroll
-                    for (int s = 0; s < AP_N / 16; s++)
-                        ap_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + s * 8, ap_desc_mn(v + s * 2048), id_o, j > 0 || s > 0);
-                    if (t == tiles - 1) umma_commit(&B.empty[(2 * j + 1) % AP_STAGES]);
-                    if (j + 1 < n)
-                        qk(t, j + 1);
-                    else
-                        umma_commit(&B.o_full[t]);
+            for (int s = 0; s < NB * 4; s++)
+                if (s < ks) {
+                    const uint64_t q = dq + ((s >> 2) * (AP_QBLOCK >> 4) + (s & 3) * 2), ks_ = k + ((s >> 2) * (AP_BLOCK >> 4) + (s & 3) * 2);
+                    ap_mma_ss(d, q, ks_, id_s, s > 0);
+                    if (tiles > 1) ap_mma_ss(d + 128, q + (NB * AP_QBLOCK >> 4), ks_, id_s, s > 0);
                 }
-                if (ok && j + 1 < n) umma_commit(&B.empty[(2 * j + 2) % AP_STAGES]);
+            umma_commit(&B.s_full[0][b]);
+            if (tiles > 1) umma_commit(&B.s_full[1][b]);
+            umma_commit(&B.empty[st]);
+        };
+        for (int j = 0; j < 2 && j < n; j++) {
+            wait(&B.full[st], ph);
+            tc_fence_after();
+            qk(j);
+            step();
+        }
+        for (int j = 0; j < n; j++) {
+            // values j in the present stage, keys j + 2 (if any) in the next
+            const int b = j & 1;
+            wait(&B.full[st], ph);
+            wait(&B.p_full[0][b], (j >> 1) & 1);
+            if (tiles > 1) wait(&B.p_full[1][b], (j >> 1) & 1);
+            tc_fence_after();
+            const uint64_t v = dv + (uint32_t)st * STAGE;
+            if (ap_elect()) {
+#pragma unroll
+                for (int s = 0; s < AP_N / 16; s++) {
+                    ap_mma_ts(tm + 256, tm + b * 64 + s * 8, v + s * (2048 >> 4), id_o, j > 0 || s > 0);
+                    if (tiles > 1) ap_mma_ts(tm + 384, tm + 128 + b * 64 + s * 8, v + s * (2048 >> 4), id_o, j > 0 || s > 0);
+                }
+                umma_commit(&B.o_done[0][b]);
+                if (tiles > 1) umma_commit(&B.o_done[1][b]);
+                umma_commit(&B.empty[st]);
+            }
+            __syncwarp();
+            step();
+            if (j + 2 < n) {
+                wait(&B.full[st], ph);
+                qk(b);
+                step();
             }
         }
-        __syncwarp();
     } else if (warp / 4 < tiles) {
         const int t = warp / 4, row = it.r0 + t * 128 + (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), ts = lanes + t * 128, to = lanes + 256 + t * 128;
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;
         for (int j = 0; j < n && ok; j++) {
-            ok = wait(&B.s_full[t], j & 1);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = __all_sync(0xffffffffu, wait(&B.s_full[t][j & 1], (j >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[128];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32(ts + c * 32, s + c * 32);
-            tmem_wait_ld();
+            const uint32_t tp = ts + (j & 1) * 64;
             const int left = it.p1 - (it.p0 + j * AP_N);
-            if (left < AP_N)
-#pragma unroll
-                for (int c = 0; c < 128; c++)
-                    if (c >= left) s[c] = 0xFF800000u;  // -inf
+            uint32_t s[2][32];
+            tmem_ld32(tp, s[0]);
+            tmem_ld32(tp + 32, s[1]);
+            tmem_wait_ld(s[0]);
+            tmem_wait_ld(s[1]);
+            ap_mask(s[0], left);
+            ap_mask(s[1], left - 32);
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 128; c += 4)
-#pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = fmaxf(x[k], __uint_as_float(s[c + k]));
+            for (int k = 0; k < 64; k++) x[k & 3] = fmaxf(x[k & 3], __uint_as_float(s[k / 32][k % 32]));
             const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;  // scale >= 0
             if (__any_sync(0xffffffffu, top > m + AP_LAZY || (m == -INFINITY && top > m))) {
                 const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : ex2(m - mn);
                 l0 *= f;
                 l1 *= f;
                 m = mn;
-                if (j) {
+                if (j) {  // the step before is in O, and this one is not: its P is not made
+                    ok = __all_sync(0xffffffffu, wait(&B.o_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1));
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < NB * 64; c += 16) {
                         uint32_t o[16];
                         tmem_ld16(to + c, o);
-                        tmem_wait_ld();
+                        tmem_wait_ld(o);
 #pragma unroll
                         for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
                         tmem_st16(to + c, o);
@@ -268,36 +339,36 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
+            for (int c = 0; c < 2; c++) {
                 uint32_t p[16];
 #pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    const float e0 = ex2(fmaf(__uint_as_float(s[h * 32 + 2 * c]), a.scale, -base));
-                    const float e1 = ex2(fmaf(__uint_as_float(s[h * 32 + 2 * c + 1]), a.scale, -base));
+                for (int k = 0; k < 16; k++) {
+                    const float e0 = ex2(fmaf(__uint_as_float(s[c][2 * k]), a.scale, -base));
+                    const float e1 = ex2(fmaf(__uint_as_float(s[c][2 * k + 1]), a.scale, -base));
                     l0 += e0;
                     l1 += e1;
-                    p[c] = pack2<T>(e0, e1);
+                    p[k] = pack2<T>(e0, e1);
                 }
-                tmem_st16(ts + h * 16, p);
+                tmem_st16(tp + c * 16, p);
             }
             tmem_wait_st();
             tc_fence_before();
-            ap_arrive(&B.p_full[t]);
+            ap_arrive(&B.p_full[t][j & 1]);
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait(&B.o_full[t], 0));
+        if (ok) ok = __all_sync(0xffffffffu, wait(&B.o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1));
         if (ok) {
             tc_fence_after();
             const bool in = row < it.r1;
             const size_t at = in ? part_at(a, it.slot, row, kvh) : 0;
             if (in) a.ml[at] = make_float2(m, l0 + l1);
             float *dst = a.acc + at * hd;
-            for (int c = 0; c < hd; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + c, o);
-                tmem_wait_ld();
+            for (int c = 0; c < hd; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(to + c, o);
+                tmem_wait_ld(o);
                 if (in)
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
+                    for (int k = 0; k < 16; k += 4)
                         if (c + k < hd)  // hd is a multiple of 8
                             *reinterpret_cast<uint4 *>(dst + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
             }

@@ -30,6 +30,14 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_HD = 256;
 
+// The end of a CTA. The chunk kernel may run beside the prefix's (attn_prefix.cu),
+// and the join waits for the chunk kernel alone: so one CTA of it, and with it the
+// kernel, ends after the prefix's. (Were it all of them, they would keep their
+// places on the SMs: the two kernels took 206 us, one after the other 223.)
+__device__ __forceinline__ void after_prefix() {
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait_();
+}
+
 // ---- any shape ---------------------------------------------------------------
 // One CTA per chunk of positions and KV head. 32 positions at a time go to
 // shared memory as f32; 16 query rows (row, head of the group) share them, a
@@ -47,7 +55,7 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
     const T *kb = it.k, *vb = it.v;
     const int64_t ps = it.pos_stride;
     if (p0 >= p1) {  // the join does not read this slot
-        pdl_wait_();
+        after_prefix();
         return;
     }
     for (int t0 = r0; t0 < r1; t0 += G_TR) {
@@ -118,7 +126,7 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
                 if (d * 32 + lane < hd) a.acc[at * hd + d * 32 + lane] = acc[j][d];
         }
     }
-    pdl_wait_();
+    after_prefix();
 }
 
 // ---- tensor cores, a few query rows per tile ------------------------------------
@@ -133,8 +141,8 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
 // are added to the running sums by f32 additions: the tensor core truncates its
 // own, which along a row of 128 dimensions cost 2.1e-6 of the result, not 1e-6.
 template <class T> constexpr int mma_tp() { return sizeof(T) == 4 ? 32 : 64; }
-template <class T, int HDP> constexpr int mma_kstride() { return sizeof(T) == 4 ? HDP + 8 : HDP + 8; }
-template <class T, int HDP> constexpr int mma_vstride() { return sizeof(T) == 4 ? HDP + 4 : HDP + 8; }
+template <class T, int HDP> constexpr int mma_kstride() { return sizeof(T) == 4 ? HDP + 8 : HDP; }
+template <class T, int HDP> constexpr int mma_vstride() { return sizeof(T) == 4 ? HDP + 4 : HDP; }
 template <class T, int HDP> constexpr size_t mma_stage() {
     return (size_t)mma_tp<T>() * (mma_kstride<T, HDP>() + mma_vstride<T, HDP>()) * sizeof(T);
 }
@@ -155,19 +163,25 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
     const int kvh = blockIdx.y;
     const Item<T> it = item_of<T>(a, a.first + blockIdx.x, kvh);
     if (it.p0 >= it.p1) {  // the join does not read this slot
-        pdl_wait_();
+        after_prefix();
         return;
     }
     auto stage_k = [&](int s) { return reinterpret_cast<T *>(smb + s * mma_stage<T, HDP>()); };
     auto stage_v = [&](int s) { return stage_k(s) + TP * KST; };
     float *sq = reinterpret_cast<float *>(smb + maxz(2 * mma_stage<T, HDP>(), (size_t)64 * HDP * 4));
     constexpr int QST = HDP + 8;
+    // 16-byte piece c of row j: 16-bit rows are unpadded (64 KB of tiles let the CTA fit
+    // beside one of the prefix's), their pieces permuted within groups of eight by the
+    // row, so that eight rows of a column of pieces touch all banks
+    auto piece = [](int j, int c) { return F ? c : c ^ (j & 7); };
     const int wide = (hd + SUB - 1) / SUB * SUB;  // the head dimension rounded up to a product's depth
     if (wide > hd)                                // its rest holds zeros, which the copies leave alone
         for (int i = tid; i < 2 * TP * (wide - hd); i += 128) {
+            constexpr int E = 16 / (int)sizeof(T);
             const int s = i / (TP * (wide - hd)), j = i / (wide - hd) % TP, d = hd + i % (wide - hd);
-            stage_k(s)[j * KST + d] = from_f32<T>(0.0f);
-            stage_v(s)[j * VST + d] = from_f32<T>(0.0f);
+            const int at = piece(j, d / E) * E + d % E;
+            stage_k(s)[j * KST + at] = from_f32<T>(0.0f);
+            stage_v(s)[j * VST + at] = from_f32<T>(0.0f);
         }
     const int cpr = hd * (int)sizeof(T) / 16;  // 16-byte pieces of a row
     const int drow = 128 / cpr, dcol = 128 % cpr;
@@ -177,8 +191,8 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
         while (j < TP) {
             const bool in = p + j < it.p1;
             const int64_t src = (int64_t)(in ? p + j : it.p0) * it.pos_stride + c * (16 / (int)sizeof(T));
-            cp_async16(k0 + j * (KST * (int)sizeof(T)) + c * 16, it.k + src, in);
-            cp_async16(v0 + j * (VST * (int)sizeof(T)) + c * 16, it.v + src, in);
+            cp_async16(k0 + j * (KST * (int)sizeof(T)) + piece(j, c) * 16, it.k + src, in);
+            cp_async16(v0 + j * (VST * (int)sizeof(T)) + piece(j, c) * 16, it.v + src, in);
             j += drow;
             c += dcol;
             if (c >= cpr) {
@@ -262,12 +276,12 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
 #pragma unroll
                     for (int j = 0; j < 4; j++) c[0][j] += small[j];
                 } else {
-                    const uint32_t at = smem_u32(sk + (sub + (lane >> 4) * 8 + (lane & 7)) * KST + ((lane >> 3) & 1) * 8);
+                    const uint32_t at = smem_u32(sk + (sub + (lane >> 4) * 8 + (lane & 7)) * KST);
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
                         if (k * 16 < wide) {
                             uint32_t b[4];
-                            ldmatrix_x4(b, at + k * 32);
+                            ldmatrix_x4(b, at + (((2 * k + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
                             mma_k16<T>(c[0], qf[k], b[0], b[1]);
                             mma_k16<T>(c[1], qf[k], b[2], b[3]);
                         }
@@ -344,12 +358,12 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
                     const float2 r0 = unpack2<T>(pf[0]), r1 = unpack2<T>(pf[1]), r2 = unpack2<T>(pf[2]), r3 = unpack2<T>(pf[3]);
                     l0 += (r0.x + r0.y) + (r2.x + r2.y);
                     l1 += (r1.x + r1.y) + (r3.x + r3.y);
-                    const uint32_t at = smem_u32(sv + (sub + ((lane >> 3) & 1) * 8 + (lane & 7)) * VST + (lane >> 4) * 8);
+                    const uint32_t at = smem_u32(sv + (sub + ((lane >> 3) & 1) * 8 + (lane & 7)) * VST);
 #pragma unroll
                     for (int i = 0; i < HDP / 16; i++) {
                         if (i * 16 < wide) {
                             uint32_t b[4];
-                            ldmatrix_x4_trans(b, at + i * 32);
+                            ldmatrix_x4_trans(b, at + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4));
                             mma_k16<T>(o[2 * i], pf, b[0], b[1]);
                             mma_k16<T>(o[2 * i + 1], pf, b[2], b[3]);
                         }
@@ -415,7 +429,7 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
             }
         }
     }
-    pdl_wait_();  // the join waits for this kernel, and through it for the prefix's
+    after_prefix();
 }
 
 // ---- join ----------------------------------------------------------------------

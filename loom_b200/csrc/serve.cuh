@@ -44,6 +44,9 @@ template <auto K> cudaError_t allow_smem(size_t smem) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || (dev < 16 && most[dev] >= smem)) return e;
     e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // kernels that are to share an SM need the same split of its memory: all of it shared
+    if (e == cudaSuccess && smem > 48 * 1024)
+        e = cudaFuncSetAttribute(K, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess && dev < 16) most[dev] = smem;
     return e;
 }
