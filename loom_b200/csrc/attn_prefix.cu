@@ -28,20 +28,16 @@
 // which is bound by memory where this one is not. P is rounded to the element type
 // as in attn_shared.cu. Every wait is bounded; one that gives up sets an error word
 // (bit 128 of loom_cuda_device_error), leaves NaN in the CTA's rows and ends.
-#include <cuda.h>  // CUtensorMap (the encoder is reached through the runtime's driver entry point)
-
 #include <type_traits>
 
 #include "attn_shared.cuh"
-#include "umma.cuh"
 
 namespace loom {
 namespace {
 
-constexpr int AP_THREADS = 320, AP_N = 64, AP_STAGES = 6;
+constexpr int AP_THREADS = 320, AP_N = ATTN_PREFIX_N, AP_STAGES = 6;
 constexpr size_t AP_QBLOCK = 128 * 128;          // 128 rows of 64 elements, swizzled in 128-byte rows
 constexpr size_t AP_BLOCK = AP_N * 128;          // the same of 64 positions
-constexpr uint32_t AP_POLLS = 64, AP_TRIES = 1 << 14;  // polls between looks at the CTA's error flag, and looks
 constexpr float AP_LAZY = 8.0f;                  // log2 of the growth that scales O
 
 struct ApBars {
@@ -92,12 +88,6 @@ __device__ __forceinline__ void ap_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
-__device__ __forceinline__ void ap_tma(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
 #define AP_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define AP_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
 // 32 columns of the warp's lanes, without the wait
@@ -129,10 +119,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : AP_W8(r, 0), AP_W8(r, 8)::"memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void ap_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // columns from `left` on are no positions
 __device__ __forceinline__ void ap_mask(uint32_t (&s)[32], int left) {
     if (left >= 32) return;
@@ -144,7 +130,7 @@ __device__ __forceinline__ void ap_mask(uint32_t (&s)[32], int left) {
 // NB: blocks of 64 dimensions (head_dim <= 64 NB)
 template <class T, int NB>
 __global__ void __maxnreg__(112)
-    k_attn_prefix(AttnArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+    k_attn_prefix(AttnArgs a, const __grid_constant__ AttnMaps maps) {
     extern __shared__ __align__(1024) uint8_t smp[];  // the swizzle's atoms are 1 KB
     pdl_trigger_();
     const uint32_t sm0 = smem_u32(smp);
@@ -155,8 +141,8 @@ __global__ void __maxnreg__(112)
     const int n = (it.p1 - it.p0 + AP_N - 1) / AP_N, rows = it.r1 - it.r0, tiles = rows > 128 ? 2 : 1;
     volatile int *err = &B.err;
     auto wait = [&](uint64_t *bar, uint32_t parity) {  // false once any wait of the CTA has given up
-        for (int i = 0; i < AP_TRIES; i++) {
-            if (mbar_wait(bar, parity, AP_POLLS)) return true;
+        for (int i = 0; i < ATTN_TRIES; i++) {
+            if (mbar_wait(bar, parity, ATTN_POLLS)) return true;
             if (*err) return false;
         }
         *err = 1;
@@ -178,7 +164,8 @@ __global__ void __maxnreg__(112)
         mbar_expect_tx(&B.full[s], (uint32_t)(NB * AP_BLOCK));
         B.issued = i + 1;
         for (int b = 0; b < NB; b++)
-            ap_tma(ring + (uint32_t)((s * NB + b) * AP_BLOCK), values ? &mv : &mk, b * 64, it.p0 + pos * AP_N, kvh, &B.full[s]);
+            attn_tma(ring + (uint32_t)((s * NB + b) * AP_BLOCK), values ? &maps.pv : &maps.pk, b * 64, it.p0 + pos * AP_N, kvh, 0,
+                     &B.full[s]);
     };
     if (warp == 8 && lane == 0) {
         for (int s = 0; s < AP_STAGES; s++) {
@@ -353,7 +340,7 @@ __global__ void __maxnreg__(112)
             }
             tmem_wait_st();
             tc_fence_before();
-            ap_arrive(&B.p_full[t][j & 1]);
+            attn_arrive(&B.p_full[t][j & 1]);
         }
         if (ok) ok = __all_sync(0xffffffffu, wait(&B.o_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1));
         if (ok) {
@@ -391,46 +378,11 @@ __global__ void __maxnreg__(112)
     if (warp == 9) tmem_free(tmem, 512);
 }
 
-typedef CUresult (*ApEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-ApEncodeFn ap_encoder() {
-    static ApEncodeFn f = nullptr;
-    if (!f) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            f = reinterpret_cast<ApEncodeFn>(p);
-    }
-    return f;
-}
-
-// [KV heads][positions][head_dim] of a cache in boxes of 128 positions x 64
-// dimensions; what lies outside reads as zero
-template <class T> bool ap_map(CUtensorMap &m, const AttnArgs &a, const void *base) {
-    ApEncodeFn enc = ap_encoder();
-    if (!enc) return false;
-    const cuuint64_t dims[3] = {(cuuint64_t)a.hd, (cuuint64_t)a.prefix, (cuuint64_t)a.nkv};
-    const cuuint64_t strides[2] = {(cuuint64_t)a.ppos * 2, (cuuint64_t)(a.nkv > 1 ? a.phead : a.ppos) * 2};
-    const cuuint32_t box[3] = {64, AP_N, 1}, es[3] = {1, 1, 1};
-    return enc(&m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-               const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <class T, int NB> cudaError_t ap_launch(const AttnArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
+template <class T, int NB> cudaError_t ap_launch(const AttnArgs &a, const AttnMaps &maps, cudaStream_t st) {
     if (const cudaError_t e = allow_smem<k_attn_prefix<T, NB>>(ap_smem<NB>()); e != cudaSuccess) return e;
-    k_attn_prefix<T, NB><<<dim3(a.n_pre * a.pre_tiles, a.nkv), AP_THREADS, ap_smem<NB>(), st>>>(a, mk, mv);
+    k_attn_prefix<T, NB><<<dim3(a.n_pre * a.pre_tiles, a.nkv), AP_THREADS, ap_smem<NB>(), st>>>(a, maps);
     count_launch();
     return cudaGetLastError();
-}
-
-template <class T> bool ap_run(const AttnArgs &a, cudaStream_t st, cudaError_t *e) {
-    CUtensorMap mk, mv;
-    if (!ap_map<T>(mk, a, a.pk) || !ap_map<T>(mv, a, a.pv)) return false;
-    *e = a.hd <= 64 ? ap_launch<T, 1>(a, mk, mv, st) : ap_launch<T, 2>(a, mk, mv, st);
-    return true;
 }
 
 }  // namespace
@@ -440,8 +392,9 @@ int attn_prefix_error() {
     return cudaMemcpyFromSymbol(&v, g_ap_err, sizeof v) == cudaSuccess ? v : -1;
 }
 
-bool attn_prefix_run(int type, const AttnArgs &a, cudaStream_t st, cudaError_t *e) {
-    return type == T_F16 ? ap_run<__half>(a, st, e) : ap_run<__nv_bfloat16>(a, st, e);
+cudaError_t attn_prefix_run(int type, const AttnArgs &a, const AttnMaps &maps, cudaStream_t st) {
+    if (type == T_F16) return a.hd <= 64 ? ap_launch<__half, 1>(a, maps, st) : ap_launch<__half, 2>(a, maps, st);
+    return a.hd <= 64 ? ap_launch<__nv_bfloat16, 1>(a, maps, st) : ap_launch<__nv_bfloat16, 2>(a, maps, st);
 }
 
 }  // namespace loom

@@ -30,6 +30,8 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_HD = 256;
 
+__device__ int g_err;  // a wait for a copy gave up
+
 // The end of a CTA. The chunk kernel may run beside the prefix's (attn_prefix.cu),
 // and the join waits for the chunk kernel alone: so one CTA of it, and with it the
 // kernel, ends after the prefix's. (Were it all of them, they would keep their
@@ -133,7 +135,9 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
 // Four warps over up to 64 query rows: a warp has 16 of them, and warps that are
 // left over when the rows are fewer share the rows and split the positions (a
 // decode step's 8 heads of a group: all four do), joining at the end. Positions
-// come in tiles through two shared-memory stages (16-byte asynchronous copies).
+// come in tiles of 64 (f32: 32) through two shared-memory stages, copied by TMA in
+// blocks of 128 bytes of dimensions, swizzled; one thread asks for them (the
+// addresses of 16-byte copies by all threads were half of their instructions).
 // Scores, maxima and sums are f32. The weights are rounded to the element type for
 // their product with the values (2^-9 or 2^-12 of each, the size of the output's
 // own rounding) and summed as rounded, so that they still add up to one; f32
@@ -141,23 +145,24 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
 // are added to the running sums by f32 additions: the tensor core truncates its
 // own, which along a row of 128 dimensions cost 2.1e-6 of the result, not 1e-6.
 template <class T> constexpr int mma_tp() { return sizeof(T) == 4 ? 32 : 64; }
-template <class T, int HDP> constexpr int mma_kstride() { return sizeof(T) == 4 ? HDP + 8 : HDP; }
-template <class T, int HDP> constexpr int mma_vstride() { return sizeof(T) == 4 ? HDP + 4 : HDP; }
-template <class T, int HDP> constexpr size_t mma_stage() {
-    return (size_t)mma_tp<T>() * (mma_kstride<T, HDP>() + mma_vstride<T, HDP>()) * sizeof(T);
-}
+template <class T> constexpr size_t mma_block() { return mma_tp<T>() * 128; }  // 128 bytes of a tile's rows
+template <class T, int HDP> constexpr size_t mma_tile() { return HDP * sizeof(T) / 128 * mma_block<T>(); }
 constexpr size_t maxz(size_t a, size_t b) { return a > b ? a : b; }
 template <class T, int HDP> constexpr size_t mma_smem() {  // stages (or the warps' sums), then f32 queries
-    return maxz(2 * mma_stage<T, HDP>(), (size_t)64 * HDP * 4) + (sizeof(T) == 4 ? (size_t)64 * (HDP + 8) * 4 : 0);
+    return maxz(4 * mma_tile<T, HDP>(), (size_t)64 * HDP * 4) + (sizeof(T) == 4 ? (size_t)64 * (HDP + 4) * 4 : 0);
 }
 
-template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a) {
-    constexpr int TP = mma_tp<T>(), KST = mma_kstride<T, HDP>(), VST = mma_vstride<T, HDP>();
+template <class T, int HDP>
+__global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __grid_constant__ AttnMaps maps) {
+    constexpr int TP = mma_tp<T>(), E = 128 / (int)sizeof(T);  // positions of a tile, dimensions of a block
+    constexpr uint32_t BLK = mma_block<T>(), TILE = mma_tile<T, HDP>();
     constexpr bool F = sizeof(T) == 4;
-    constexpr int SUB = F ? 8 : 16;            // positions of one step of a warp
-    constexpr int KS = F ? 1 : HDP / 16;       // query fragments held in registers (16-bit types)
-    extern __shared__ __align__(16) uint8_t smb[];
+    constexpr int SUB = F ? 8 : 16;       // positions of one step of a warp
+    constexpr int KS = F ? 1 : HDP / 16;  // query fragments held in registers (16-bit types)
+    extern __shared__ __align__(1024) uint8_t smb[];
     __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ uint64_t s_full[2], s_empty[2];
+    __shared__ int s_err;
     pdl_trigger_();
     const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kvh = blockIdx.y;
@@ -166,41 +171,37 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
         after_prefix();
         return;
     }
-    auto stage_k = [&](int s) { return reinterpret_cast<T *>(smb + s * mma_stage<T, HDP>()); };
-    auto stage_v = [&](int s) { return stage_k(s) + TP * KST; };
-    float *sq = reinterpret_cast<float *>(smb + maxz(2 * mma_stage<T, HDP>(), (size_t)64 * HDP * 4));
-    constexpr int QST = HDP + 8;
-    // 16-byte piece c of row j: 16-bit rows are unpadded (64 KB of tiles let the CTA fit
-    // beside one of the prefix's), their pieces permuted within groups of eight by the
-    // row, so that eight rows of a column of pieces touch all banks
-    auto piece = [](int j, int c) { return F ? c : c ^ (j & 7); };
-    const int wide = (hd + SUB - 1) / SUB * SUB;  // the head dimension rounded up to a product's depth
-    if (wide > hd)                                // its rest holds zeros, which the copies leave alone
-        for (int i = tid; i < 2 * TP * (wide - hd); i += 128) {
-            constexpr int E = 16 / (int)sizeof(T);
-            const int s = i / (TP * (wide - hd)), j = i / (wide - hd) % TP, d = hd + i % (wide - hd);
-            const int at = piece(j, d / E) * E + d % E;
-            stage_k(s)[j * KST + at] = from_f32<T>(0.0f);
-            stage_v(s)[j * VST + at] = from_f32<T>(0.0f);
+    const uint32_t sm0 = smem_u32(smb);
+    float *sq = reinterpret_cast<float *>(smb + maxz(4 * TILE, (size_t)64 * HDP * 4));
+    constexpr int QST = HDP + 4;
+    const int blocks = (hd + E - 1) / E, wide = F ? blocks * E : (hd + 15) / 16 * 16;
+    const int tiles = (it.p1 - it.p0 + TP - 1) / TP, left = it.p1 - it.p0 - (tiles - 1) * TP;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {  // false once any wait of the CTA has given up
+        for (int i = 0; i < ATTN_TRIES; i++) {
+            if (mbar_wait(bar, parity, ATTN_POLLS)) return true;
+            if (*reinterpret_cast<volatile int *>(&s_err)) return false;
         }
-    const int cpr = hd * (int)sizeof(T) / 16;  // 16-byte pieces of a row
-    const int drow = 128 / cpr, dcol = 128 % cpr;
-    auto fetch = [&](int s, int p) {
-        int j = tid / cpr, c = tid % cpr;
-        const uint32_t k0 = smem_u32(stage_k(s)), v0 = smem_u32(stage_v(s));
-        while (j < TP) {
-            const bool in = p + j < it.p1;
-            const int64_t src = (int64_t)(in ? p + j : it.p0) * it.pos_stride + c * (16 / (int)sizeof(T));
-            cp_async16(k0 + j * (KST * (int)sizeof(T)) + piece(j, c) * 16, it.k + src, in);
-            cp_async16(v0 + j * (VST * (int)sizeof(T)) + piece(j, c) * 16, it.v + src, in);
-            j += drow;
-            c += dcol;
-            if (c >= cpr) {
-                c -= cpr;
-                j++;
-            }
+        *reinterpret_cast<volatile int *>(&s_err) = 1;
+        return false;
+    };
+    auto fetch = [&](int s, int i) {  // tile i into stage s; what lies outside the cache reads as zero
+        const uint32_t dst = sm0 + s * 2 * TILE;
+        mbar_expect_tx(&s_full[s], 2 * blocks * BLK);
+        for (int b = 0; b < blocks; b++) {
+            attn_tma(dst + b * BLK, it.own ? &maps.ok : &maps.pk, b * E, it.p0 + i * TP, kvh, it.seq, &s_full[s]);
+            attn_tma(dst + TILE + b * BLK, it.own ? &maps.ov : &maps.pv, b * E, it.p0 + i * TP, kvh, it.seq, &s_full[s]);
         }
     };
+    if (tid == 0) {
+        for (int s = 0; s < 2; s++) {
+            mbar_init_nf(&s_full[s], 1);
+            mbar_init_nf(&s_empty[s], 4);
+        }
+        s_err = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    uint32_t seen = 0;  // tiles of the blocks of rows before
+    bool ok = true;
     for (int rb = it.r0; rb < it.r1; rb += 64) {
         const int rows = min(64, it.r1 - rb);
         const int nps = rows <= 16 ? 4 : rows <= 32 ? 2 : 1;  // warps that share 16 rows
@@ -211,92 +212,121 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
             return static_cast<const T *>(a.q) + (int64_t)(hr / a.group) * a.q_stride +
                    (int64_t)(kvh * a.group + hr % a.group) * hd;
         };
-        __syncthreads();  // the last block's joined sums have been read
-        fetch(0, it.p0);
-        cp_async_commit();
-        fetch(1, it.p0 + TP);
-        cp_async_commit();
+        fence_async_smem();  // zeros written below, before the copies that follow
+        __syncthreads();
+        if (tid == 0) {  // both stages are free: every tile before has been read
+            fetch(seen & 1, 0);
+            if (tiles > 1) fetch((seen + 1) & 1, 1);
+        }
         uint32_t qf[KS][4];
         if constexpr (F) {
             for (int j = warp; j < (rows + 15) / 16 * 16; j += 4) {
                 const float *src = reinterpret_cast<const float *>(q_row(min(rb + j, it.r1 - 1)));
                 for (int d = lane; d < wide; d += 32) sq[j * QST + d] = j < rows && d < hd ? src[d] : 0.0f;
             }
+            __syncthreads();
         } else {
+            // pairs of dimensions; whole words where rows lie on 4 bytes (hd is even)
+            const uint16_t *qa = reinterpret_cast<const uint16_t *>(q_row(in_a ? row_a : rb)) + 2 * t;
+            const uint16_t *qb = reinterpret_cast<const uint16_t *>(q_row(in_b ? row_b : rb)) + 2 * t;
+            const bool words = ((reinterpret_cast<uintptr_t>(qa) | reinterpret_cast<uintptr_t>(qb)) & 3) == 0;
+            auto two = [&](bool in, const uint16_t *p, int d) -> uint32_t {
+                if (!in || d + 2 * t >= hd) return 0u;
+                return words ? *reinterpret_cast<const uint32_t *>(p + d) : (uint32_t)p[d] | ((uint32_t)p[d + 1] << 16);
+            };
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const int d = k * 16 + 2 * t;
-                auto two = [&](bool in, int hr, int dd) -> uint32_t {
-                    if (!in || dd >= hd) return 0u;
-                    const uint16_t *p = reinterpret_cast<const uint16_t *>(q_row(hr) + dd);
-                    return (uint32_t)p[0] | ((uint32_t)p[1] << 16);  // hd is even
-                };
-                qf[k][0] = two(in_a, row_a, d);
-                qf[k][1] = two(in_b, row_b, d);
-                qf[k][2] = two(in_a, row_a, d + 8);
-                qf[k][3] = two(in_b, row_b, d + 8);
+                qf[k][0] = two(in_a, qa, k * 16);
+                qf[k][1] = two(in_b, qb, k * 16);
+                qf[k][2] = two(in_a, qa, k * 16 + 8);
+                qf[k][3] = two(in_b, qb, k * 16 + 8);
             }
         }
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         float o[HDP / 8][4];
 #pragma unroll
         for (int i = 0; i < HDP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        int s = 0;
-        for (int p = it.p0; p < it.p1; p += TP, s ^= 1) {
-            cp_async_wait<1>();
-            __syncthreads();
-            const T *sk = stage_k(s), *sv = stage_v(s);
-            for (int sub = ps * SUB; busy && sub < TP && p + sub < it.p1; sub += nps * SUB) {
+        for (int i = 0; i < tiles; i++, seen++) {
+            const int s = seen & 1, here = i == tiles - 1 ? left : TP;
+            ok = ok && wait(&s_full[s], (seen >> 1) & 1);
+            const uint32_t tk = sm0 + s * 2 * TILE, tv = tk + TILE;
+            if (here < TP) {  // what lies past the length may be anything, and 0 times it is not 0
+                __syncthreads();
+                for (int j = tid; j < (TP - here) * blocks * 8; j += 128)
+                    *reinterpret_cast<uint4 *>(smb + (tv - sm0) + (j >> 3) % blocks * BLK + (here + (j >> 3) / blocks) * 128 +
+                                               (j & 7) * 16) = make_uint4(0, 0, 0, 0);
+                __syncthreads();
+            }
+            for (int sub = ps * SUB; busy && sub < here; sub += nps * SUB) {
                 constexpr int NT = SUB / 8;
                 float c[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
                 if constexpr (F) {
+                    // lane t has dimensions 8t .. 8t + 7 of 32, in pieces 2t and 2t + 1, two
+                    // for each of four products: any order sums to the same scores
                     float small[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-                    for (int d = 0; d < wide; d += 8) {
-                        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const float2 qa = *reinterpret_cast<const float2 *>(sq + (rt * 16 + g) * QST + d + 2 * t);
-                        const float2 qb = *reinterpret_cast<const float2 *>(sq + (rt * 16 + g + 8) * QST + d + 2 * t);
-                        const float2 kk = *reinterpret_cast<const float2 *>(
-                            reinterpret_cast<const float *>(sk) + (sub + g) * KST + d + 2 * t);
-                        uint32_t ah[4], al[4], bh[2], bl[2];
-                        split_tf32(qa.x, ah[0], al[0]);
-                        split_tf32(qb.x, ah[1], al[1]);
-                        split_tf32(qa.y, ah[2], al[2]);
-                        split_tf32(qb.y, ah[3], al[3]);
-                        split_tf32(kk.x, bh[0], bl[0]);
-                        split_tf32(kk.y, bh[1], bl[1]);
-                        mma_tf32(small, al, bh[0], bh[1]);
-                        mma_tf32(small, ah, bl[0], bl[1]);
-                        mma_tf32(e, ah, bh[0], bh[1]);
+                    const float *qa = sq + (rt * 16 + g) * QST + 8 * t, *qb = qa + 8 * QST;
+                    const uint8_t *kr = smb + (tk - sm0) + (sub + g) * 128;
+#pragma unroll 2
+                    for (int d = 0; d < blocks; d++) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) c[0][j] += e[j];
+                        for (int h = 0; h < 2; h++) {
+                            const float4 ua = *reinterpret_cast<const float4 *>(qa + d * 32 + h * 4);
+                            const float4 ub = *reinterpret_cast<const float4 *>(qb + d * 32 + h * 4);
+                            const float4 kk = *reinterpret_cast<const float4 *>(kr + d * BLK + (((2 * t + h) ^ g) << 4));
+                            const float xa[4] = {ua.x, ua.y, ua.z, ua.w}, xb[4] = {ub.x, ub.y, ub.z, ub.w},
+                                        xk[4] = {kk.x, kk.y, kk.z, kk.w};
+#pragma unroll
+                            for (int u = 0; u < 4; u += 2) {
+                                uint32_t ah[4], al[4], bh[2], bl[2];
+                                float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                split_tf32(xa[u], ah[0], al[0]);
+                                split_tf32(xb[u], ah[1], al[1]);
+                                split_tf32(xa[u + 1], ah[2], al[2]);
+                                split_tf32(xb[u + 1], ah[3], al[3]);
+                                split_tf32(xk[u], bh[0], bl[0]);
+                                split_tf32(xk[u + 1], bh[1], bl[1]);
+                                mma_tf32(small, al, bh[0], bh[1]);
+                                mma_tf32(small, ah, bl[0], bl[1]);
+                                mma_tf32(e, ah, bh[0], bh[1]);
+#pragma unroll
+                                for (int j = 0; j < 4; j++) c[0][j] += e[j];
+                            }
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < 4; j++) c[0][j] += small[j];
                 } else {
-                    const uint32_t at = smem_u32(sk + (sub + (lane >> 4) * 8 + (lane & 7)) * KST);
+                    // 16-byte piece c of a row is at c ^ (row % 8) of its block
+                    const uint32_t row = tk + (sub + (lane >> 4) * 8 + (lane & 7)) * 128, x = ((lane >> 3) & 1) ^ (lane & 7);
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
                         if (k * 16 < wide) {
                             uint32_t b[4];
-                            ldmatrix_x4(b, at + (((2 * k + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+                            ldmatrix_x4(b, row + (k >> 2) * BLK + ((((2 * k) & 7) ^ x) << 4));
                             mma_k16<T>(c[0], qf[k], b[0], b[1]);
                             mma_k16<T>(c[1], qf[k], b[2], b[3]);
                         }
                     }
                 }
-                float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        c[n][j] *= a.scale;
-                        if (p + sub + n * 8 + 2 * t + (j & 1) >= it.p1) c[n][j] = -INFINITY;
-                        float &x = j < 2 ? x0 : x1;
-                        x = fmaxf(x, c[n][j]);
-                    }
+                    for (int j = 0; j < 4; j++) c[n][j] *= a.scale;
+                if (sub + SUB > here) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (sub + n * 8 + 2 * t + (j & 1) >= here) c[n][j] = -INFINITY;
+                }
+                float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    x0 = fmaxf(x0, fmaxf(c[n][0], c[n][1]));
+                    x1 = fmaxf(x1, fmaxf(c[n][2], c[n][3]));
+                }
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
                 x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
@@ -308,11 +338,11 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
                     l0 *= f0;
                     l1 *= f1;
 #pragma unroll
-                    for (int i = 0; i < HDP / 8; i++) {
-                        o[i][0] *= f0;
-                        o[i][1] *= f0;
-                        o[i][2] *= f1;
-                        o[i][3] *= f1;
+                    for (int i2 = 0; i2 < HDP / 8; i2++) {
+                        o[i2][0] *= f0;
+                        o[i2][1] *= f0;
+                        o[i2][2] *= f1;
+                        o[i2][3] *= f1;
                     }
                     m0 = n0;
                     m1 = n1;
@@ -332,21 +362,23 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
                     split_tf32(c[0][3], ah[3], al[3]);
                     l0 += c[0][0] + c[0][1];
                     l1 += c[0][2] + c[0][3];
-                    const float *v0 = reinterpret_cast<const float *>(sv) + (sub + 2 * t) * VST + g;
+                    const uint8_t *v0 = smb + (tv - sm0) + (sub + 2 * t) * 128 + (g & 3) * 4;
 #pragma unroll
-                    for (int i = 0; i < HDP / 8; i++) {
-                        if (i * 8 < wide) {
+                    for (int i2 = 0; i2 < HDP / 8; i2++) {
+                        if (i2 * 8 < hd) {
+                            const int piece = ((2 * i2) & 7) + (g >> 2);
+                            const uint8_t *v = v0 + (i2 >> 2) * BLK;
                             uint32_t bh[2], bl[2];
-                            split_tf32(v0[i * 8], bh[0], bl[0]);
-                            split_tf32(v0[VST + i * 8], bh[1], bl[1]);
+                            split_tf32(*reinterpret_cast<const float *>(v + ((piece ^ (2 * t)) << 4)), bh[0], bl[0]);
+                            split_tf32(*reinterpret_cast<const float *>(v + 128 + ((piece ^ (2 * t + 1)) << 4)), bh[1], bl[1]);
                             float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             mma_tf32(e, al, bh[0], bh[1]);
                             mma_tf32(e, ah, bl[0], bl[1]);
                             mma_tf32(e, ah, bh[0], bh[1]);
-                            o[i][0] += e[0];
-                            o[i][1] += e[1];
-                            o[i][2] += e[2];
-                            o[i][3] += e[3];
+                            o[i2][0] += e[0];
+                            o[i2][1] += e[1];
+                            o[i2][2] += e[2];
+                            o[i2][3] += e[3];
                         }
                     }
                 } else {
@@ -358,27 +390,30 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
                     const float2 r0 = unpack2<T>(pf[0]), r1 = unpack2<T>(pf[1]), r2 = unpack2<T>(pf[2]), r3 = unpack2<T>(pf[3]);
                     l0 += (r0.x + r0.y) + (r2.x + r2.y);
                     l1 += (r1.x + r1.y) + (r3.x + r3.y);
-                    const uint32_t at = smem_u32(sv + (sub + ((lane >> 3) & 1) * 8 + (lane & 7)) * VST);
+                    const uint32_t row = tv + (sub + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128, x = (lane >> 4) ^ (lane & 7);
 #pragma unroll
-                    for (int i = 0; i < HDP / 16; i++) {
-                        if (i * 16 < wide) {
+                    for (int i2 = 0; i2 < HDP / 16; i2++) {
+                        if (i2 * 16 < wide) {
                             uint32_t b[4];
-                            ldmatrix_x4_trans(b, at + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4));
-                            mma_k16<T>(o[2 * i], pf, b[0], b[1]);
-                            mma_k16<T>(o[2 * i + 1], pf, b[2], b[3]);
+                            ldmatrix_x4_trans(b, row + (i2 >> 2) * BLK + ((((2 * i2) & 7) ^ x) << 4));
+                            mma_k16<T>(o[2 * i2], pf, b[0], b[1]);
+                            mma_k16<T>(o[2 * i2 + 1], pf, b[2], b[3]);
                         }
                     }
                 }
             }
-            __syncthreads();
-            if (p + 2 * TP < it.p1) fetch(s, p + 2 * TP);
-            cp_async_commit();
+            __syncwarp();
+            if (lane == 0) attn_arrive(&s_empty[s]);
+            if (tid == 0 && i + 2 < tiles) {
+                ok = ok && wait(&s_empty[s], (seen >> 1) & 1);
+                if (ok) fetch(s, i + 2);
+            }
+            __syncwarp();
         }
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        cp_async_wait<0>();
         if (nps == 1) {
 #pragma unroll
             for (int half = 0; half < 2; half++) {
@@ -428,6 +463,10 @@ template <class T, int HDP> __global__ void __launch_bounds__(128) k_attn_shared
                 a.acc[at * hd + d] = v;
             }
         }
+    }
+    if (!ok || *reinterpret_cast<volatile int *>(&s_err)) {  // a copy that does not come: no result
+        for (int hr = it.r0 + tid; hr < it.r1; hr += 128) a.ml[part_at(a, it.slot, hr, kvh)] = make_float2(NAN, NAN);
+        if (tid == 0) atomicOr(&g_err, 128);
     }
     after_prefix();
 }
@@ -608,8 +647,8 @@ size_t ws_bytes_of(const AttnArgs &a) {
     return ml_bytes(a) + (size_t)(a.n_pre + a.n_own) * a.n_rows * a.nh * a.hd * sizeof(float);
 }
 
-// Whether the tensor-core kernels can take the call: whole 16-byte pieces in
-// every cache row, and rows of whole pieces apart.
+// Whether the copy engine can take the caches: whole 16-byte pieces in every row,
+// and rows of whole pieces apart.
 bool pieces(const AttnArgs &a, size_t size) {
     auto whole = [&](int64_t elems) { return elems * (int64_t)size % 16 == 0; };
     auto ptr = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -617,35 +656,79 @@ bool pieces(const AttnArgs &a, size_t size) {
            ptr(a.pk) && ptr(a.pv) && ptr(a.ok) && ptr(a.ov);
 }
 
-template <auto K> cudaError_t launch_items(size_t smem, int items, int threads, const AttnArgs &a, cudaStream_t st) {
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+    static EncodeFn f = nullptr;
+    if (!f) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            f = reinterpret_cast<EncodeFn>(p);
+    }
+    return f;
+}
+
+// [seqs][KV heads][positions][head_dim] of a cache in boxes of `box` positions x 128
+// bytes of dimensions; what lies outside reads as zero
+bool attn_map(CUtensorMap &m, int type, const void *base, const AttnArgs &a, int len, int64_t pos, int64_t head, int seqs,
+              int64_t seq, uint32_t box) {
+    EncodeFn enc = encoder();
+    if (!enc || !base) return false;
+    const cuuint64_t size = elem_bytes(type);
+    const cuuint64_t dims[4] = {(cuuint64_t)a.hd, (cuuint64_t)len, (cuuint64_t)a.nkv, (cuuint64_t)seqs};
+    auto stride = [&](int64_t s, int n) { return (cuuint64_t)(n > 1 ? s : pos) * size; };  // of one element: unused
+    const cuuint64_t strides[3] = {stride(pos, 2), stride(head, a.nkv), stride(seq, seqs)};
+    const cuuint32_t boxes[4] = {(cuuint32_t)(128 / size), box, 1, 1}, es[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType ty = type == T_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : type == T_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(&m, ty, 4, const_cast<void *>(base), dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <auto K, class... M>
+cudaError_t launch_items(size_t smem, int items, int threads, const AttnArgs &a, cudaStream_t st, const M &...maps) {
     cudaError_t e = allow_smem<K>(smem);
     if (e != cudaSuccess) return e;
     // beside the prefix's kernel where that came before (neither reads what the other writes)
-    if (a.first) return launch_pdl_(K, dim3(items, a.nkv), dim3(threads), smem, st, a);
-    K<<<dim3(items, a.nkv), threads, smem, st>>>(a);
+    if (a.first) return launch_pdl_(K, dim3(items, a.nkv), dim3(threads), smem, st, a, maps...);
+    K<<<dim3(items, a.nkv), threads, smem, st>>>(a, maps...);
     count_launch();
     return cudaGetLastError();
 }
 
 template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
     const int all = a.n_pre * a.pre_tiles + a.n_seqs * a.n_own;
-    const bool whole = pieces(a, sizeof(T));
+    constexpr int type = sizeof(T) == 4 ? (int)T_F32 : std::is_same<T, __half>::value ? (int)T_F16 : T_BF16;
     cudaError_t e = cudaSuccess;
-    if constexpr (sizeof(T) == 2)
-        if (tc && whole && attn_prefix_run(std::is_same<T, __half>::value ? T_F16 : T_BF16, a, st, &e)) {
-            if (e != cudaSuccess) return e;
-            a.first = a.n_pre * a.pre_tiles;
-        }
+    AttnMaps maps;
+    bool mapped = pieces(a, sizeof(T));
+    tc = tc && mapped;
+    const uint32_t pre_box = tc ? (uint32_t)ATTN_PREFIX_N : mma_tp<T>();
+    if (mapped && a.n_pre)
+        mapped = attn_map(maps.pk, type, a.pk, a, a.prefix, a.ppos, a.phead, 1, 0, pre_box) &&
+                 attn_map(maps.pv, type, a.pv, a, a.prefix, a.ppos, a.phead, 1, 0, pre_box);
+    if (mapped && a.n_own)
+        mapped = attn_map(maps.ok, type, a.ok, a, a.cap, a.opos, a.ohead, a.n_seqs, a.oseq, mma_tp<T>()) &&
+                 attn_map(maps.ov, type, a.ov, a, a.cap, a.opos, a.ohead, a.n_seqs, a.oseq, mma_tp<T>());
+    if (mapped && tc) {
+        e = attn_prefix_run(type, a, maps, st);
+        if (e != cudaSuccess) return e;
+        a.first = a.n_pre * a.pre_tiles;
+    }
     if (const int items = all - a.first) {
-        if (!whole)
+        if (!mapped)
             e = launch_items<k_attn_shared_any<T>>((size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * 4,
                                                    items, G_WARPS * 32, a, st);
         else if (a.hd <= 64)
-            e = launch_items<k_attn_shared_mma<T, 64>>(mma_smem<T, 64>(), items, 128, a, st);
+            e = launch_items<k_attn_shared_mma<T, 64>>(mma_smem<T, 64>(), items, 128, a, st, maps);
         else if (a.hd <= 128)
-            e = launch_items<k_attn_shared_mma<T, 128>>(mma_smem<T, 128>(), items, 128, a, st);
+            e = launch_items<k_attn_shared_mma<T, 128>>(mma_smem<T, 128>(), items, 128, a, st, maps);
         else
-            e = launch_items<k_attn_shared_mma<T, 256>>(mma_smem<T, 256>(), items, 128, a, st);
+            e = launch_items<k_attn_shared_mma<T, 256>>(mma_smem<T, 256>(), items, 128, a, st, maps);
         if (e != cudaSuccess) return e;
     }
     // Four warps share a (row, head) where one would read many parts in turn and the
@@ -662,6 +745,12 @@ template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
 }
 
 }  // namespace
+
+int attn_shared_error() {
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_err, sizeof v) == cudaSuccess ? v | attn_prefix_error() : -1;
+}
+
 }  // namespace loom
 
 using namespace loom;

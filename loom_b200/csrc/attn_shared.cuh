@@ -1,7 +1,10 @@
 // attn_shared.cuh -- arguments and work items of the shared-prefix attention's
 // kernels (attn_shared.cu, attn_prefix.cu).
 #pragma once
+#include <cuda.h>  // CUtensorMap (the encoder is reached through the runtime's driver entry point)
+
 #include "mma.cuh"
+#include "umma.cuh"
 
 namespace loom {
 
@@ -39,7 +42,8 @@ __device__ __forceinline__ SeqView seq_view(const AttnArgs &a, int b) {
 // A CTA's work: query rows r0 .. r1-1 (row * group + head of the group) of one KV
 // head against positions p0 .. p1-1 of a cache, and the slot for the parts.
 template <class T> struct Item {
-    int slot, r0, r1, p0, p1;
+    int slot, r0, r1, p0, p1, seq;
+    bool own;  // of the own cache of sequence `seq`, else of the prefix
     const T *k, *v;
     int64_t pos_stride;
 };
@@ -47,6 +51,8 @@ template <class T> __device__ __forceinline__ Item<T> item_of(const AttnArgs &a,
     Item<T> o;
     if (item < a.n_pre * a.pre_tiles) {
         o.slot = item / a.pre_tiles;
+        o.own = false;
+        o.seq = 0;
         o.r0 = (item % a.pre_tiles) * a.pre_rows;
         o.r1 = min(o.r0 + a.pre_rows, a.n_rows * a.group);
         o.p0 = o.slot * a.pre_chunk;
@@ -58,6 +64,8 @@ template <class T> __device__ __forceinline__ Item<T> item_of(const AttnArgs &a,
         item -= a.n_pre * a.pre_tiles;
         const int b = item / a.n_own, c = item % a.n_own;
         const SeqView s = seq_view(a, b);
+        o.own = true;
+        o.seq = b;
         o.slot = a.n_pre + c;
         o.r0 = s.row0 * a.group;
         o.r1 = o.r0 + s.rows * a.group;
@@ -73,10 +81,29 @@ __device__ __forceinline__ size_t part_at(const AttnArgs &a, int slot, int hr, i
     return ((size_t)slot * a.n_rows + hr / a.group) * a.nh + kvh * a.group + hr % a.group;
 }
 
+// The caches as the copy engine sees them; those without a position are not used.
+struct AttnMaps {
+    CUtensorMap pk, pv, ok, ov;
+};
+// one box of a cache (dimension x, position y, KV head z, sequence w) to shared memory
+__device__ __forceinline__ void attn_tma(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void attn_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+constexpr uint32_t ATTN_POLLS = 64;  // polls of a wait between looks at the CTA's error flag,
+constexpr int ATTN_TRIES = 1 << 14;  // and looks before it gives up
+
 // The prefix items of a 16-bit call (head_dim <= 128, scale >= 0, pre_rows <= 256,
-// pre_chunk a multiple of 128) on the tensor cores; false when the cache's layout
-// cannot be described to the copy engine (nothing was launched).
-bool attn_prefix_run(int type, const AttnArgs &a, cudaStream_t st, cudaError_t *e);
+// pre_chunk a multiple of the box of ATTN_PREFIX_N positions) on the 5th-generation
+// tensor cores.
+constexpr int ATTN_PREFIX_N = 64;
+cudaError_t attn_prefix_run(int type, const AttnArgs &a, const AttnMaps &maps, cudaStream_t st);
 int attn_prefix_error();  // 128 after a wait of it gave up; -1 when the device is in error
+int attn_shared_error();  // the same of all the operator's kernels
 
 }  // namespace loom

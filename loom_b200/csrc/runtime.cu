@@ -848,7 +848,7 @@ size_t loom_cuda_trace_read(uint64_t *out, size_t n_kernels) {
 int loom_cuda_device_error(void) {
     if (!g_inited) return 0;
     if (cudaStreamSynchronize(g_stream) != cudaSuccess) return -1;
-    int v = attn_prefix_error();
+    int v = attn_shared_error();
     if (v < 0 || !S.counters.p) return v;
     // the error word sits after the counters of the last layer shape reserved
     std::vector<int> all(S.counters.cap / 4);
