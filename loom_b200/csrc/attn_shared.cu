@@ -157,7 +157,6 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
     constexpr int TP = mma_tp<T>(), E = 128 / (int)sizeof(T);  // positions of a tile, dimensions of a block
     constexpr uint32_t BLK = mma_block<T>(), TILE = mma_tile<T, HDP>();
     constexpr bool F = sizeof(T) == 4;
-    constexpr int SUB = F ? 8 : 16;       // positions of one step of a warp
     constexpr int KS = F ? 1 : HDP / 16;  // query fragments held in registers (16-bit types)
     extern __shared__ __align__(1024) uint8_t smb[];
     __shared__ float s_m[4][16], s_l[4][16];
@@ -257,15 +256,18 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                                                (j & 7) * 16) = make_uint4(0, 0, 0, 0);
                 __syncthreads();
             }
-            for (int sub = ps * SUB; busy && sub < here; sub += nps * SUB) {
-                constexpr int NT = SUB / 8;
+            // 8 NT positions from `sub` on
+            auto step = [&](auto nt, const int sub) {
+                constexpr int NT = decltype(nt)::value;
                 float c[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
                 if constexpr (F) {
                     // lane t has dimensions 8t .. 8t + 7 of 32, in pieces 2t and 2t + 1, two
                     // for each of four products: any order sums to the same scores
-                    float small[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float small[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) small[n][0] = small[n][1] = small[n][2] = small[n][3] = 0.0f;
                     const float *qa = sq + (rt * 16 + g) * QST + 8 * t, *qb = qa + 8 * QST;
                     const uint8_t *kr = smb + (tk - sm0) + (sub + g) * 128;
 #pragma unroll 2
@@ -274,29 +276,39 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                         for (int h = 0; h < 2; h++) {
                             const float4 ua = *reinterpret_cast<const float4 *>(qa + d * 32 + h * 4);
                             const float4 ub = *reinterpret_cast<const float4 *>(qb + d * 32 + h * 4);
-                            const float4 kk = *reinterpret_cast<const float4 *>(kr + d * BLK + (((2 * t + h) ^ g) << 4));
-                            const float xa[4] = {ua.x, ua.y, ua.z, ua.w}, xb[4] = {ub.x, ub.y, ub.z, ub.w},
-                                        xk[4] = {kk.x, kk.y, kk.z, kk.w};
+                            uint32_t ah[2][4], al[2][4];
+                            split_tf32(ua.x, ah[0][0], al[0][0]);
+                            split_tf32(ub.x, ah[0][1], al[0][1]);
+                            split_tf32(ua.y, ah[0][2], al[0][2]);
+                            split_tf32(ub.y, ah[0][3], al[0][3]);
+                            split_tf32(ua.z, ah[1][0], al[1][0]);
+                            split_tf32(ub.z, ah[1][1], al[1][1]);
+                            split_tf32(ua.w, ah[1][2], al[1][2]);
+                            split_tf32(ub.w, ah[1][3], al[1][3]);
 #pragma unroll
-                            for (int u = 0; u < 4; u += 2) {
-                                uint32_t ah[4], al[4], bh[2], bl[2];
+                            for (int n = 0; n < NT; n++) {
+                                const float4 kk = *reinterpret_cast<const float4 *>(kr + d * BLK + n * 1024 + (((2 * t + h) ^ g) << 4));
+                                uint32_t bh[4], bl[4];
+                                split_tf32(kk.x, bh[0], bl[0]);
+                                split_tf32(kk.y, bh[1], bl[1]);
+                                split_tf32(kk.z, bh[2], bl[2]);
+                                split_tf32(kk.w, bh[3], bl[3]);
                                 float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                split_tf32(xa[u], ah[0], al[0]);
-                                split_tf32(xb[u], ah[1], al[1]);
-                                split_tf32(xa[u + 1], ah[2], al[2]);
-                                split_tf32(xb[u + 1], ah[3], al[3]);
-                                split_tf32(xk[u], bh[0], bl[0]);
-                                split_tf32(xk[u + 1], bh[1], bl[1]);
-                                mma_tf32(small, al, bh[0], bh[1]);
-                                mma_tf32(small, ah, bl[0], bl[1]);
-                                mma_tf32(e, ah, bh[0], bh[1]);
 #pragma unroll
-                                for (int j = 0; j < 4; j++) c[0][j] += e[j];
+                                for (int u = 0; u < 2; u++) {
+                                    mma_tf32(small[n], al[u], bh[2 * u], bh[2 * u + 1]);
+                                    mma_tf32(small[n], ah[u], bl[2 * u], bl[2 * u + 1]);
+                                    mma_tf32(e, ah[u], bh[2 * u], bh[2 * u + 1]);
+                                }
+#pragma unroll
+                                for (int j = 0; j < 4; j++) c[n][j] += e[j];
                             }
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) c[0][j] += small[j];
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) c[n][j] += small[n][j];
                 } else {
                     // 16-byte piece c of a row is at c ^ (row % 8) of its block
                     const uint32_t row = tk + (sub + (lane >> 4) * 8 + (lane & 7)) * 128, x = ((lane >> 3) & 1) ^ (lane & 7);
@@ -314,7 +326,7 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) c[n][j] *= a.scale;
-                if (sub + SUB > here) {
+                if (sub + 8 * NT > here) {
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -355,26 +367,32 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                     c[n][3] = ex2(c[n][3] - b1);
                 }
                 if constexpr (F) {
-                    uint32_t ah[4], al[4];
-                    split_tf32(c[0][0], ah[0], al[0]);  // depth t is position 2t, depth t + 4 is 2t + 1
-                    split_tf32(c[0][2], ah[1], al[1]);
-                    split_tf32(c[0][1], ah[2], al[2]);
-                    split_tf32(c[0][3], ah[3], al[3]);
-                    l0 += c[0][0] + c[0][1];
-                    l1 += c[0][2] + c[0][3];
+                    uint32_t ah[NT][4], al[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        split_tf32(c[n][0], ah[n][0], al[n][0]);  // depth t is position 2t, depth t + 4 is 2t + 1
+                        split_tf32(c[n][2], ah[n][1], al[n][1]);
+                        split_tf32(c[n][1], ah[n][2], al[n][2]);
+                        split_tf32(c[n][3], ah[n][3], al[n][3]);
+                        l0 += c[n][0] + c[n][1];
+                        l1 += c[n][2] + c[n][3];
+                    }
                     const uint8_t *v0 = smb + (tv - sm0) + (sub + 2 * t) * 128 + (g & 3) * 4;
 #pragma unroll
                     for (int i2 = 0; i2 < HDP / 8; i2++) {
                         if (i2 * 8 < hd) {
                             const int piece = ((2 * i2) & 7) + (g >> 2);
                             const uint8_t *v = v0 + (i2 >> 2) * BLK;
-                            uint32_t bh[2], bl[2];
-                            split_tf32(*reinterpret_cast<const float *>(v + ((piece ^ (2 * t)) << 4)), bh[0], bl[0]);
-                            split_tf32(*reinterpret_cast<const float *>(v + 128 + ((piece ^ (2 * t + 1)) << 4)), bh[1], bl[1]);
                             float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_tf32(e, al, bh[0], bh[1]);
-                            mma_tf32(e, ah, bl[0], bl[1]);
-                            mma_tf32(e, ah, bh[0], bh[1]);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                uint32_t bh[2], bl[2];
+                                split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + ((piece ^ (2 * t)) << 4)), bh[0], bl[0]);
+                                split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + 128 + ((piece ^ (2 * t + 1)) << 4)), bh[1], bl[1]);
+                                mma_tf32(e, al[n], bh[0], bh[1]);
+                                mma_tf32(e, ah[n], bl[0], bl[1]);
+                                mma_tf32(e, ah[n], bh[0], bh[1]);
+                            }
                             o[i2][0] += e[0];
                             o[i2][1] += e[1];
                             o[i2][2] += e[2];
@@ -400,6 +418,19 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                             mma_k16<T>(o[2 * i2 + 1], pf, b[2], b[3]);
                         }
                     }
+                }
+            };
+            // f32: the warp's share of a tile at once (splitting the queries takes as long as
+            // a product, and serves all of the share's positions)
+            if (busy) {
+                if constexpr (!F) {
+                    for (int sub = ps * 16; sub < here; sub += nps * 16) step(std::integral_constant<int, 2>{}, sub);
+                } else if (nps == 1) {
+                    step(std::integral_constant<int, 4>{}, 0);
+                } else if (nps == 2) {
+                    if (ps * 16 < here) step(std::integral_constant<int, 2>{}, ps * 16);
+                } else if (ps * 8 < here) {
+                    step(std::integral_constant<int, 1>{}, ps * 8);
                 }
             }
             __syncwarp();
@@ -474,13 +505,47 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
 // ---- join ----------------------------------------------------------------------
 // WPH warps per (row, head), one warp where the parts are few: their maxima and
 // sums a lane each, then the parts weighted by e^(m - M), eight in flight; then the
-// own rows that not every row of the sequence sees, and the division. A row that
-// sees nothing gives zeros. Bound by reading the parts.
-template <class T, int WPH> __global__ void __launch_bounds__(128) k_attn_shared_join(AttnArgs a) {
-    constexpr int ND = MAX_HD / 32;
-    __shared__ float s_acc[WPH > 1 ? 4 : 1][MAX_HD];
+// own rows that not every row of the sequence sees, four at a time, and the
+// division. A lane has four dimensions of each 128. A row that sees nothing gives
+// zeros. Bound by reading the parts.
+// elements d .. d + 3 of a row of n, zeros past it; one access where it is aligned
+template <class T> __device__ __forceinline__ float4 four(const T *p, int d, int n, bool whole) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (whole && d < n) {  // n is a multiple of 4
+        if constexpr (sizeof(T) == 4) {
+            v = *reinterpret_cast<const float4 *>(p + d);
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p + d);
+            const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y);
+            v = make_float4(a.x, a.y, b.x, b.y);
+        }
+    } else if (d < n) {
+        v.x = to_f32(p[d]);
+        if (d + 1 < n) v.y = to_f32(p[d + 1]);
+        if (d + 2 < n) v.z = to_f32(p[d + 2]);
+        if (d + 3 < n) v.w = to_f32(p[d + 3]);
+    }
+    return v;
+}
+__device__ __forceinline__ void mul_add(float4 &a, float f, const float4 &v) {
+    a.x = fmaf(v.x, f, a.x);
+    a.y = fmaf(v.y, f, a.y);
+    a.z = fmaf(v.z, f, a.z);
+    a.w = fmaf(v.w, f, a.w);
+}
+__device__ __forceinline__ void scale_by(float4 &a, float f) {
+    a.x *= f;
+    a.y *= f;
+    a.z *= f;
+    a.w *= f;
+}
+
+// ND: groups of 128 dimensions; whole: rows of parts, queries and own caches lie on
+// four elements
+template <class T, int WPH, int ND> __global__ void __launch_bounds__(128) k_attn_shared_join(AttnArgs a, bool whole) {
+    __shared__ float4 s_acc[WPH > 1 ? 4 : 1][ND * 32];
     __shared__ float2 s_ml[4];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPH;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPH, hd = a.hd;
     const int64_t rh = (int64_t)blockIdx.x * (4 / WPH) + warp / WPH;
     if (rh >= (int64_t)a.n_rows * a.nh) {
         pdl_wait_();
@@ -499,9 +564,13 @@ template <class T, int WPH> __global__ void __launch_bounds__(128) k_attn_shared
     const bool mine = r >= s.row0 && r < s.row0 + s.rows;
     const int n = a.n_pre + (mine ? (s.common + a.own_chunk - 1) / a.own_chunk : 0);
     const int see = mine ? max(s.len - (s.row0 + s.rows - 1 - r), 0) : 0;  // own positions this row sees
-    float acc[ND], m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    float4 acc[ND], q[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++) acc[d] = 0.0f;
+    for (int d = 0; d < ND; d++) {
+        acc[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        q[d] = four(static_cast<const T *>(a.q) + r * a.q_stride + (int64_t)h * hd, d * 128 + lane * 4, hd, whole);
+    }
     const int64_t step = (int64_t)a.n_rows * a.nh;  // (row, head) pairs from part to part
     pdl_wait_();
     for (int i0 = 0; i0 < n; i0 += 32 * WPH) {
@@ -514,23 +583,21 @@ template <class T, int WPH> __global__ void __launch_bounds__(128) k_attn_shared
         l = l * fix + warp_sum(p.y * f);
         m = top;
 #pragma unroll
-        for (int d = 0; d < ND; d++) acc[d] *= fix;
+        for (int d = 0; d < ND; d++) scale_by(acc[d], fix);
         const int here = min(32, (n - i0 - part + WPH - 1) / WPH);
-        const float *src = a.acc + ((i0 + part) * step + rh) * a.hd + lane;
+        const float *src = a.acc + ((i0 + part) * step + rh) * hd;
         for (int j0 = 0; j0 < here; j0 += 8) {
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                if (d * 32 >= a.hd) break;
-                float v[8];
+                float4 v[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool in = j0 + j < here && d * 32 + lane < a.hd;
-                    v[j] = in ? __ldcg(src + (int64_t)(j0 + j) * WPH * step * a.hd + d * 32) : 0.0f;
-                }
+                for (int j = 0; j < 8; j++)
+                    v[j] = j0 + j < here ? four(src + (int64_t)(j0 + j) * WPH * step * hd, d * 128 + lane * 4, hd, hd % 4 == 0)
+                                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float w = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
-                    if (j0 + j < here && w != 0.0f) acc[d] = fmaf(v[j], w, acc[d]);
+                    if (j0 + j < here && w != 0.0f) mul_add(acc[d], w, v[j]);
                 }
             }
         }
@@ -538,8 +605,7 @@ template <class T, int WPH> __global__ void __launch_bounds__(128) k_attn_shared
     if constexpr (WPH > 1) {
         if (lane == 0) s_ml[warp] = make_float2(m, l);
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-            if (d * 32 + lane < a.hd) s_acc[warp][d * 32 + lane] = acc[d];
+        for (int d = 0; d < ND; d++) s_acc[warp][d * 32 + lane] = acc[d];
         __syncthreads();
         if (part) return;
         float top = -INFINITY;
@@ -548,36 +614,53 @@ template <class T, int WPH> __global__ void __launch_bounds__(128) k_attn_shared
         m = top;
         l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; d++) acc[d] = 0.0f;
+        for (int d = 0; d < ND; d++) acc[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int w = 0; w < WPH; w++) {
             const float f = s_ml[w].y == 0.0f ? 0.0f : ex2(s_ml[w].x - base);
             l += s_ml[w].y * f;
 #pragma unroll
-            for (int d = 0; d < ND; d++)
-                if (d * 32 + lane < a.hd) acc[d] += s_acc[w][d * 32 + lane] * f;
+            for (int d = 0; d < ND; d++) mul_add(acc[d], f, s_acc[w][d * 32 + lane]);
         }
     }
-    const T *q = static_cast<const T *>(a.q) + r * a.q_stride + (int64_t)h * a.hd;
-    for (int p = s.common; p < see; p++) {
-        const T *k = static_cast<const T *>(a.ok) + b * a.oseq + p * a.opos + kvh * a.ohead;
-        const T *v = static_cast<const T *>(a.ov) + b * a.oseq + p * a.opos + kvh * a.ohead;
-        float x = 0.0f;
+    const T *k0 = static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead, *v0 = static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead;
+    for (int p0 = s.common; p0 < see; p0 += 4) {
+        float x[4];
+        float4 v[4][ND];
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-            if (d * 32 + lane < a.hd) x = fmaf(to_f32(q[d * 32 + lane]) * a.scale, to_f32(k[d * 32 + lane]), x);
-        x = warp_sum(x);
-        if (x == -INFINITY) continue;
-        const float mn = fmaxf(m, x), fa = ex2(m - mn), fb = ex2(x - mn);
-        l = l * fa + fb;
-        m = mn;
+        for (int j = 0; j < 4; j++) {
+            x[j] = 0.0f;
+            const int64_t at = (int64_t)min(p0 + j, see - 1) * a.opos;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-            if (d * 32 + lane < a.hd) acc[d] = acc[d] * fa + to_f32(v[d * 32 + lane]) * fb;
+            for (int d = 0; d < ND; d++) {
+                const float4 k = four(k0 + at, d * 128 + lane * 4, hd, whole);
+                v[j][d] = four(v0 + at, d * 128 + lane * 4, hd, whole);
+                x[j] = fmaf(q[d].x, k.x, fmaf(q[d].y, k.y, fmaf(q[d].z, k.z, fmaf(q[d].w, k.w, x[j]))));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[j] = warp_sum(x[j]) * a.scale;
+            if (p0 + j >= see || x[j] == -INFINITY) continue;
+            const float mn = fmaxf(m, x[j]), fa = ex2(m - mn), fb = ex2(x[j] - mn);
+            l = l * fa + fb;
+            m = mn;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                scale_by(acc[d], fa);
+                mul_add(acc[d], fb, v[j][d]);
+            }
+        }
     }
-    T *out = static_cast<T *>(a.out) + r * a.out_stride + (int64_t)h * a.hd;
+    T *out = static_cast<T *>(a.out) + r * a.out_stride + (int64_t)h * hd;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-        if (d * 32 + lane < a.hd) out[d * 32 + lane] = from_f32<T>(l != 0.0f ? acc[d] / l : 0.0f);
+    for (int d = 0; d < ND; d++) {
+        const int at = d * 128 + lane * 4;
+        const float e[4] = {acc[d].x, acc[d].y, acc[d].z, acc[d].w};
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (at + k < hd) out[at + k] = from_f32<T>(l != 0.0f ? e[k] * inv : 0.0f);
+    }
 }
 
 const char *check(const loom_attn_shared_desc *d) {
@@ -621,7 +704,7 @@ void plan(const loom_attn_shared_desc *d, AttnArgs &a) {
     a.ohead = (int64_t)d->own_head_stride;
     a.oseq = (int64_t)d->own_seq_stride;
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int want = 6 * 148;
+    const int want = 6 * 148;  // 3 to 12 per SM measured alike
     const int64_t rows = std::max<int64_t>((int64_t)a.n_rows * a.group, 1);
     if (prefix_tc(d)) {  // one CTA per SM, one round of them
         a.pre_tiles = (int)up(rows, 256);
@@ -700,6 +783,23 @@ cudaError_t launch_items(size_t smem, int items, int threads, const AttnArgs &a,
     return cudaGetLastError();
 }
 
+template <class T, int ND> cudaError_t launch_join(const AttnArgs &a, int items, cudaStream_t st) {
+    // Four warps share a (row, head) where one would read many parts in turn and the
+    // rows alone leave SMs idle.
+    const int64_t pairs = (int64_t)a.n_rows * a.nh;
+    const bool few = a.n_pre + a.n_own > 16 && pairs < 4 * 4 * 148;
+    const auto on = [&](int64_t elems) { return elems % 4 == 0; };
+    const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0; };
+    const bool whole = on(a.hd) && on(a.q_stride) && on(a.opos) && on(a.ohead) && on(a.oseq) && at(a.q) && at(a.ok) && at(a.ov);
+    const dim3 grid((unsigned)(few ? pairs : (pairs + 3) / 4));
+    if (items)
+        return few ? launch_pdl_(k_attn_shared_join<T, 4, ND>, grid, dim3(128), 0, st, a, whole)
+                   : launch_pdl_(k_attn_shared_join<T, 1, ND>, grid, dim3(128), 0, st, a, whole);
+    k_attn_shared_join<T, 1, ND><<<grid, 128, 0, st>>>(a, whole);  // reads seq_rows before its wait: only behind its own kernel
+    count_launch();
+    return cudaGetLastError();
+}
+
 template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
     const int all = a.n_pre * a.pre_tiles + a.n_seqs * a.n_own;
     constexpr int type = sizeof(T) == 4 ? (int)T_F32 : std::is_same<T, __half>::value ? (int)T_F16 : T_BF16;
@@ -731,17 +831,7 @@ template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
             e = launch_items<k_attn_shared_mma<T, 256>>(mma_smem<T, 256>(), items, 128, a, st, maps);
         if (e != cudaSuccess) return e;
     }
-    // Four warps share a (row, head) where one would read many parts in turn and the
-    // rows alone leave SMs idle.
-    const int64_t pairs = (int64_t)a.n_rows * a.nh;
-    const bool four = a.n_pre + a.n_own > 16 && pairs < 4 * 4 * 148;
-    const dim3 grid((unsigned)(four ? pairs : (pairs + 3) / 4));
-    if (all)
-        return four ? launch_pdl_(k_attn_shared_join<T, 4>, grid, dim3(128), 0, st, a)
-                    : launch_pdl_(k_attn_shared_join<T, 1>, grid, dim3(128), 0, st, a);
-    k_attn_shared_join<T, 1><<<grid, 128, 0, st>>>(a);  // reads seq_rows before its wait: only behind its own kernel
-    count_launch();
-    return cudaGetLastError();
+    return a.hd <= 128 ? launch_join<T, 1>(a, all, st) : launch_join<T, 2>(a, all, st);
 }
 
 }  // namespace
