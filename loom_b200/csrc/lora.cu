@@ -14,10 +14,11 @@
 // weights as two tf32 terms (mma.cuh; 16-bit weights are exact in one), since
 // they would otherwise be bound by their multiply-adds as soon as some rows share
 // an adapter; few rows leave most of a fragment idle, but those are bound by
-// reading the weights. Operands come straight from global memory in 16-byte
-// pieces: the order of the summed dimension is free, so lane t of a row takes
-// its elements 8t .. 8t + 7 of 32, the four products of which use two each.
+// reading the weights. The order of the summed dimension is free, so lane t of a
+// row takes its elements 8t .. 8t + 7 of 32, the four products of which use two
+// each: operands are read from shared memory 16 bytes at a time.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/loom_cuda.h"
 #include "mma.cuh"
@@ -28,7 +29,7 @@ namespace {
 
 constexpr int L_RB = 64;   // rows of a block
 constexpr int L_NB = 8;    // column tiles (of 8) of a warp's step
-constexpr int L_OUT = 256; // output columns of a CTA
+constexpr int L_OUT = 128; // output columns of a CTA
 
 struct LoraArgs {
     const float *x, *scales, *base;
@@ -45,75 +46,84 @@ __device__ __forceinline__ int lora_rank(const LoraArgs &a, int id) {
     return id < 0 ? 0 : min(max(a.ranks[id], 0), a.max_rank);
 }
 
-// The rows of the j-th adapter (in order of appearance) among the block's rows:
-// their count (0: there are fewer adapters), in s_rows[]; id -1 stands for none.
+// The rows of the j-th adapter (in order of appearance) among a block's rows: their
+// count (0: there are fewer adapters), the adapter (-1: none) and the rows in
+// s_rows[]. Every warp looks for itself, two rows to a lane, without a barrier;
+// the rows are the same in all, and s_rows may be read after the next one.
 struct Group {
     int rows, id;
 };
-__device__ __forceinline__ Group group_of(const LoraArgs &a, int r0, int j, int *s_ids, int *s_rows) {
-    __shared__ int s_id, s_n;
-    __shared__ uint32_t s_mask[2];
-    const int tid = threadIdx.x, lane = tid & 31;
-    if (tid < L_RB) {
-        int id = r0 + tid < a.n_rows ? a.ids[r0 + tid] : -2;
-        if (id != -2 && (id < 0 || id >= a.n_adapters)) id = -1;
-        if (r0 + tid >= a.n_rows) id = -2;
-        s_ids[tid] = id;
+__device__ __forceinline__ Group group_of(const LoraArgs &a, int r0, int j, int *s_rows) {
+    const int lane = threadIdx.x & 31;
+    auto id_of = [&](int r) {
+        if (r >= a.n_rows) return -2;
+        const int id = a.ids[r];
+        return id < 0 || id >= a.n_adapters ? -1 : id;
+    };
+    const int ia = id_of(r0 + lane), ib = id_of(r0 + 32 + lane);
+    const uint32_t ma = __match_any_sync(0xffffffffu, ia), mb = __match_any_sync(0xffffffffu, ib);
+    bool second = ib != -2;  // b's first row of its adapter, none among a's
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        const int other = __shfl_sync(0xffffffffu, ia, i);  // by all lanes, whatever they have found
+        second = second && other != ib;
     }
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    bool first = false;
-    if (tid < L_RB) {
-        first = s_ids[tid] != -2;
-        for (int i = 0; i < tid && first; i++) first = s_ids[i] != s_ids[tid];
-        const uint32_t m = __ballot_sync(0xffffffffu, first);
-        if (lane == 0) s_mask[tid >> 5] = m;
+    const uint32_t below = (1u << lane) - 1;
+    const uint32_t fa = __ballot_sync(0xffffffffu, ia != -2 && !(ma & below));
+    const uint32_t fb = __ballot_sync(0xffffffffu, second && !(mb & below));
+    const int na = __popc(fa);
+    if (j >= na + __popc(fb)) return {0, 0};
+    // the lane whose row is the j-th first one
+    const uint32_t here = __ballot_sync(0xffffffffu, j < na ? ((fa >> lane) & 1) && __popc(fa & below) == j
+                                                              : ((fb >> lane) & 1) && __popc(fb & below) == j - na);
+    const int id = __shfl_sync(0xffffffffu, j < na ? ia : ib, __ffs(here) - 1);
+    const uint32_t ra = __ballot_sync(0xffffffffu, ia == id), rb = __ballot_sync(0xffffffffu, ib == id);
+    if (threadIdx.x < 32) {
+        if (ia == id) s_rows[__popc(ra & below)] = r0 + lane;
+        if (ib == id) s_rows[__popc(ra) + __popc(rb & below)] = r0 + 32 + lane;
     }
-    __syncthreads();
-    if (first && (tid < 32 ? 0 : __popc(s_mask[0])) + __popc(s_mask[tid >> 5] & ((1u << lane) - 1)) == j) {
-        s_id = s_ids[tid];
-        s_n = 1;
-    }
-    __syncthreads();
-    if (!s_n) return {0, 0};
-    const int id = s_id;
-    bool mine = false;
-    if (tid < L_RB) {
-        mine = s_ids[tid] == id;
-        const uint32_t m = __ballot_sync(0xffffffffu, mine);
-        if (lane == 0) s_mask[tid >> 5] = m;
-    }
-    __syncthreads();
-    if (mine) s_rows[(tid < 32 ? 0 : __popc(s_mask[0])) + __popc(s_mask[tid >> 5] & ((1u << lane) - 1))] = r0 + tid;
-    const int n = __popc(s_mask[0]) + __popc(s_mask[1]);
-    __syncthreads();
-    return {n, id};
+    return {__popc(ra) + __popc(rb), id};
 }
 
-// elements i .. i + 7 of p as f32, zeros from n on; two 16-byte reads (one for
-// 16-bit types) where that is aligned
-__device__ __forceinline__ void load8(float (&v)[8], const float *p, int i, int n, bool wide) {
-    if (wide && i + 8 <= n) {
-        const float4 u = __ldg(reinterpret_cast<const float4 *>(p + i)), w = __ldg(reinterpret_cast<const float4 *>(p + i + 4));
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
-    } else {
+// A tile of `rows` x `cols` elements in shared memory, rows `stride` bytes apart, from
+// rows at row_of(j) (null: zeros) of which `n` columns exist; 16 bytes at a time,
+// asynchronously where `wide` says that rows lie on 16 bytes.
+template <class E, class F>
+__device__ __forceinline__ void load_tile(uint8_t *dst, int stride, int rows, int cols, int n, bool wide, F row_of) {
+    constexpr int N = 16 / (int)sizeof(E);
+    const int per = cols / N;
+    for (int i = threadIdx.x; i < rows * per; i += 128) {
+        const int j = i / per, c = (i % per) * N;
+        const E *src = row_of(j);
+        uint8_t *d = dst + j * stride + c * (int)sizeof(E);
+        if (wide && (c + N <= n || c >= n || !src)) {
+            const bool in = src && c < n;
+            cp_async16(smem_u32(d), in ? src + c : row_of(0), in);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = i + k < n ? p[i + k] : 0.0f;
+            for (int k = 0; k < N; k++) reinterpret_cast<E *>(d)[k] = src && c + k < n ? src[c + k] : from_f32<E>(0.0f);
+        }
     }
 }
-template <class T> __device__ __forceinline__ void load8(float (&v)[8], const T *p, int i, int n, bool wide) {
-    if (wide && i + 8 <= n) {
-        const uint4 u = ld_v4(p + i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+
+// eight elements of a tile's row as f32
+__device__ __forceinline__ void read8(float (&v)[8], const float *p) {
+    const float4 u = *reinterpret_cast<const float4 *>(p), w = *reinterpret_cast<const float4 *>(p + 4);
+    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
+}
+template <class T> __device__ __forceinline__ void read8(float (&v)[8], const T *p) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float2 f = unpack2<T>(w[k]);
-            v[2 * k] = f.x, v[2 * k + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = i + k < n ? to_f32(p[i + k]) : 0.0f;
+    for (int k = 0; k < 4; k++) {
+        const float2 f = unpack2<T>(w[k]);
+        v[2 * k] = f.x, v[2 * k + 1] = f.y;
     }
+}
+// bytes between rows of a tile of `cols` weights: the quarter warps that read 8 rows'
+// worth of 16 bytes at once touch every bank
+template <class T> __host__ __device__ constexpr int w_stride(int cols) {
+    return sizeof(T) == 4 ? cols * 4 + 16 : cols * 2 + (cols == 32 ? 0 : 64);
 }
 
 // c += (16 rows x 32) . (32 x 8) for the lane's eight elements of each operand:
@@ -151,43 +161,72 @@ __device__ __forceinline__ void split_rows(uint32_t (&ah)[4][4], uint32_t (&al)[
 }
 
 // Parts of t: CTA (block of rows, adapter of the block, slice of n_in). A warp has
-// 16 rows; warps left over split the slice and join in shared memory.
+// 16 rows; warps left over split the depth of a tile and join in shared memory. x
+// and the weights come in tiles of 32 deep for each of the nk warps that split it,
+// through stages of asynchronous copies.
+template <class T> constexpr int l_stages() { return sizeof(T) == 4 ? 2 : 3; }
+constexpr int L_XTILE = 64 * (32 * 4 + 16);                                       // the largest of 64 x 32, 32 x 64, 16 x 128
+template <class T> constexpr int l_stage() { return L_XTILE + 64 * w_stride<T>(128); }  // and of the weights' 64 rows
+
 template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs a) {
-    __shared__ int s_ids[L_RB], s_rows[L_RB];
-    __shared__ float s_t[4][16][L_NB * 8 + 1];
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int s_rows[L_RB];
     pdl_trigger_();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const Group gr = group_of(a, blockIdx.x * L_RB, blockIdx.y, s_ids, s_rows);
+    const Group gr = group_of(a, blockIdx.x * L_RB, blockIdx.y, s_rows);
     const int rank = gr.rows ? lora_rank(a, gr.id) : 0;
     if (!rank) return;
+    __syncthreads();
     const int nk = gr.rows <= 16 ? 4 : gr.rows <= 32 ? 2 : 1, mt = warp / nk, kp = warp % nk;
-    const int i0 = blockIdx.z * a.slice, i1 = min(i0 + a.slice, a.n_in);
-    const bool ina = mt * 16 + g < gr.rows, inb = mt * 16 + g + 8 < gr.rows;
-    const float *xa = a.x + (ina ? s_rows[mt * 16 + g] : 0) * a.x_stride;
-    const float *xb = a.x + (inb ? s_rows[mt * 16 + g + 8] : 0) * a.x_stride;
+    const int i0 = blockIdx.z * a.slice, i1 = min(i0 + a.slice, a.n_in), deep = 32 * nk;
+    const int xst = deep * 4 + 16, wst = w_stride<T>(deep), tiles = (i1 - i0 + deep - 1) / deep;
     const T *w = static_cast<const T *>(a.a) + gr.id * a.a_adapter;
     float *part = a.t + (size_t)blockIdx.z * a.n_rows * a.max_rank;
+    const bool busy = mt * 16 < gr.rows;
     for (int k0 = 0; k0 < rank; k0 += L_NB * 8) {
+        const int cols = min(rank - k0, L_NB * 8);
+        auto fetch = [&](int i) {
+            if (i < tiles) {
+                uint8_t *st = smem + i % l_stages<T>() * l_stage<T>();
+                const int at = i0 + i * deep;
+                load_tile<float>(st, xst, (gr.rows + 15) / 16 * 16, deep, i1 - at, a.wide_x, [&](int j) {
+                    return j < gr.rows ? a.x + s_rows[j] * a.x_stride + at : (const float *)nullptr;
+                });
+                load_tile<T>(st + L_XTILE, wst, (cols + 7) / 8 * 8, deep, i1 - at, a.wide_a,
+                             [&](int j) { return j < cols ? w + (k0 + j) * a.a_row + at : (const T *)nullptr; });
+            }
+            cp_async_commit();
+        };
         float c[L_NB][4];
 #pragma unroll
         for (int n = 0; n < L_NB; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
-        if (mt * 16 < gr.rows) {
-            for (int i = i0 + kp * 32; i < i1; i += nk * 32) {
+        __syncthreads();  // the sums of the ranks before have been read
+        for (int i = 0; i < l_stages<T>() - 1; i++) fetch(i);
+        for (int i = 0; i < tiles; i++) {
+            cp_async_wait<l_stages<T>() - 2>();
+            __syncthreads();
+            fetch(i + l_stages<T>() - 1);  // into the stage that was read in the step before
+            const uint8_t *st = smem + i % l_stages<T>() * l_stage<T>();
+            if (busy) {
                 float ua[8], ub[8];
-                load8(ua, xa, i + 8 * t, ina ? i1 : 0, a.wide_x);
-                load8(ub, xb, i + 8 * t, inb ? i1 : 0, a.wide_x);
-                float v[L_NB][8];
-#pragma unroll
-                for (int n = 0; n < L_NB; n++)
-                    load8(v[n], w + (k0 + n * 8 + g) * a.a_row, i + 8 * t, k0 + n * 8 + g < rank ? i1 : 0, a.wide_a);
                 uint32_t ah[4][4], al[4][4];
+                const float *x = reinterpret_cast<const float *>(st + (mt * 16 + g) * xst) + kp * 32 + 8 * t;
+                read8(ua, x);
+                read8(ub, x + 8 * (xst / 4));
                 split_rows(ah, al, ua, ub);
+                const uint8_t *ws = st + L_XTILE + g * wst + (kp * 32 + 8 * t) * (int)sizeof(T);
 #pragma unroll
                 for (int n = 0; n < L_NB; n++)
-                    if (k0 + n * 8 < rank) mma_32<T>(c[n], ah, al, v[n]);
+                    if (n * 8 < cols) {
+                        float v[8];
+                        read8(v, reinterpret_cast<const T *>(ws + n * 8 * wst));
+                        mma_32<T>(c[n], ah, al, v);
+                    }
             }
         }
+        cp_async_wait<0>();
         __syncthreads();
+        float(*s_t)[16][L_NB * 8 + 1] = reinterpret_cast<float(*)[16][L_NB * 8 + 1]>(smem);
 #pragma unroll
         for (int n = 0; n < L_NB; n++) {
             s_t[warp][g][n * 8 + 2 * t] = c[n][0];
@@ -196,7 +235,6 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
             s_t[warp][g + 8][n * 8 + 2 * t + 1] = c[n][3];
         }
         __syncthreads();
-        const int cols = min(rank - k0, L_NB * 8);
         for (int j = tid; j < gr.rows * cols; j += 128) {
             const int m = j / cols, k = j % cols;
             float s = 0.0f;
@@ -206,82 +244,115 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
     }
 }
 
-// out: CTA (block of rows, adapter of the block, L_OUT columns); a warp has a
-// quarter of the columns, for all the rows.
+// out: CTA (block of rows, adapter of the block, L_OUT columns). A warp has 16 rows;
+// warps left over split the columns. The weights and the base, which do not wait for
+// t, are asked for before it. Bound by reading the base and writing out.
+constexpr int L_DEEP = 64;  // ranks at a time
+template <class T> constexpr size_t l_expand_smem() { return (size_t)L_OUT * w_stride<T>(L_DEEP) + 64 * (L_DEEP * 4 + 16); }
+
 template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs a) {
-    extern __shared__ float s_x[];  // t of the group's rows [64][stride]
-    __shared__ int s_ids[L_RB], s_rows[L_RB];
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int s_rows[L_RB];
+    constexpr int WST = w_stride<T>(L_DEEP), TST = L_DEEP + 4;
+    float *s_x = reinterpret_cast<float *>(smem + L_OUT * WST);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const Group gr = group_of(a, blockIdx.x * L_RB, blockIdx.y, s_ids, s_rows);
-    pdl_wait_();
-    if (!gr.rows) return;
-    const int rank = lora_rank(a, gr.id), deep = (rank + 31) / 32 * 32, stride = a.max_rank + 36;
-    const float scale = rank ? a.scales[gr.id] : 0.0f;
-    for (int j = tid; j < (gr.rows + 15) / 16 * 16 * deep; j += 128) {
-        const int m = j / deep, k = j % deep;
-        float s = 0.0f;
-        if (m < gr.rows && k < rank)
-            for (int z = 0; z < a.n_slices; z++) s += a.t[((size_t)z * a.n_rows + s_rows[m]) * a.max_rank + k];
-        s_x[m * stride + k] = s * scale;
+    const Group gr = group_of(a, blockIdx.x * L_RB, blockIdx.y, s_rows);
+    if (!gr.rows) {
+        pdl_wait_();
+        return;
     }
     __syncthreads();
-    const int o0 = blockIdx.z * L_OUT + warp * (L_OUT / 4);
-    const T *w = static_cast<const T *>(a.b) + (rank ? gr.id : 0) * a.b_adapter;
-    for (int m0 = 0; m0 < gr.rows; m0 += 16) {
-        float c[L_NB][4];
-        const bool in[2] = {m0 + g < gr.rows, m0 + g + 8 < gr.rows};
-        const int64_t row[2] = {in[0] ? s_rows[m0 + g] : 0, in[1] ? s_rows[m0 + g + 8] : 0};
+    const int rank = lora_rank(a, gr.id);
+    const float scale = rank ? a.scales[gr.id] : 0.0f;
+    const int o0 = blockIdx.z * L_OUT, outs = min(L_OUT, a.n_out - o0);
+    const T *w = static_cast<const T *>(a.b) + (rank ? gr.id : 0) * a.b_adapter + o0 * a.b_row;
+    auto weights = [&](int k) {
+        const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
+        load_tile<T>(smem, WST, (outs + 7) / 8 * 8, deep, rank - k, a.wide_b,
+                     [&](int j) { return j < outs ? w + j * a.b_row + k : (const T *)nullptr; });
+        cp_async_commit();
+    };
+    if (rank) weights(0);
+    const int nc = gr.rows <= 16 ? 4 : gr.rows <= 32 ? 2 : 1, mt = warp / nc, cp = warp % nc;
+    const bool in[2] = {mt * 16 + g < gr.rows, mt * 16 + g + 8 < gr.rows};
+    const int64_t row[2] = {in[0] ? s_rows[mt * 16 + g] : 0, in[1] ? s_rows[mt * 16 + g + 8] : 0};
+    auto go = [&](auto tiles) {
+        constexpr int NT = decltype(tiles)::value;  // column tiles of 8
+        const int c0 = cp * NT * 8;
+        float c[NT][4];
 #pragma unroll
-        for (int n = 0; n < L_NB; n++) {
-            const int o = o0 + n * 8 + 2 * t;
+        for (int n = 0; n < NT; n++) {
+            const int o = c0 + n * 8 + 2 * t;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 float2 b = make_float2(0.0f, 0.0f);
                 if (in[h] && a.base) {
-                    const float *p = a.base + row[h] * a.base_stride + o;
-                    if (a.wide_out && o + 1 < a.n_out)
+                    const float *p = a.base + row[h] * a.base_stride + o0 + o;
+                    if (a.wide_out && o + 1 < outs) {
                         b = *reinterpret_cast<const float2 *>(p);
-                    else {
-                        if (o < a.n_out) b.x = p[0];
-                        if (o + 1 < a.n_out) b.y = p[1];
+                    } else {
+                        if (o < outs) b.x = p[0];
+                        if (o + 1 < outs) b.y = p[1];
                     }
                 }
                 c[n][2 * h] = b.x;
                 c[n][2 * h + 1] = b.y;
             }
         }
-        for (int k = 0; k < rank; k += 32) {
-            uint32_t ah[4][4], al[4][4];
-            float ua[8], ub[8];
-#pragma unroll
-            for (int q = 0; q < 8; q++) {
-                ua[q] = s_x[(m0 + g) * stride + k + 8 * t + q];
-                ub[q] = s_x[(m0 + g + 8) * stride + k + 8 * t + q];
+        pdl_wait_();  // t is there
+        for (int k = 0; k < rank; k += L_DEEP) {
+            const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
+            if (k) {
+                __syncthreads();
+                weights(k);
             }
-            split_rows(ah, al, ua, ub);
-            float v[L_NB][8];
+            for (int j = tid; j < (gr.rows + 15) / 16 * 16 * deep; j += 128) {
+                const int m = j / deep, q = k + j % deep;
+                float s = 0.0f;
+                if (m < gr.rows && q < rank) {
+                    const float *p = a.t + (size_t)s_rows[m] * a.max_rank + q;
+#pragma unroll 4
+                    for (int z = 0; z < a.n_slices; z++) s += __ldcg(p + (size_t)z * a.n_rows * a.max_rank);
+                }
+                s_x[m * TST + j % deep] = s * scale;
+            }
+            cp_async_wait<0>();
+            __syncthreads();
+            if (mt * 16 < gr.rows)
+                for (int q = 0; q < deep; q += 32) {
+                    float ua[8], ub[8];
+                    uint32_t ah[4][4], al[4][4];
+                    read8(ua, s_x + (mt * 16 + g) * TST + q + 8 * t);
+                    read8(ub, s_x + (mt * 16 + g + 8) * TST + q + 8 * t);
+                    split_rows(ah, al, ua, ub);
 #pragma unroll
-            for (int n = 0; n < L_NB; n++)
-                load8(v[n], w + (int64_t)(o0 + n * 8 + g) * a.b_row, k + 8 * t, o0 + n * 8 + g < a.n_out ? rank : 0, a.wide_b);
-#pragma unroll
-            for (int n = 0; n < L_NB; n++) mma_32<T>(c[n], ah, al, v[n]);
+                    for (int n = 0; n < NT; n++)
+                        if (c0 + n * 8 < outs) {
+                            float v[8];
+                            read8(v, reinterpret_cast<const T *>(smem + (c0 + n * 8 + g) * WST) + q + 8 * t);
+                            mma_32<T>(c[n], ah, al, v);
+                        }
+                }
         }
 #pragma unroll
-        for (int n = 0; n < L_NB; n++) {
-            const int o = o0 + n * 8 + 2 * t;
+        for (int n = 0; n < NT; n++) {
+            const int o = c0 + n * 8 + 2 * t;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 if (!in[h]) continue;
-                float *p = a.out + row[h] * a.out_stride + o;
-                if (a.wide_out && o + 1 < a.n_out)
+                float *p = a.out + row[h] * a.out_stride + o0 + o;
+                if (a.wide_out && o + 1 < outs) {
                     *reinterpret_cast<float2 *>(p) = make_float2(c[n][2 * h], c[n][2 * h + 1]);
-                else {
-                    if (o < a.n_out) p[0] = c[n][2 * h];
-                    if (o + 1 < a.n_out) p[1] = c[n][2 * h + 1];
+                } else {
+                    if (o < outs) p[0] = c[n][2 * h];
+                    if (o + 1 < outs) p[1] = c[n][2 * h + 1];
                 }
             }
         }
-    }
+    };
+    if (nc == 4) go(std::integral_constant<int, L_OUT / 32>{});
+    else if (nc == 2) go(std::integral_constant<int, L_OUT / 16>{});
+    else go(std::integral_constant<int, L_OUT / 8>{});
 }
 
 const char *check(const loom_lora_desc *d) {
@@ -308,17 +379,18 @@ size_t ws_bytes_of(const loom_lora_desc *d) { return slices_of(d) * d->n_rows * 
 
 template <class T> cudaError_t launch(const LoraArgs &a, cudaStream_t st) {
     const unsigned blocks = (a.n_rows + L_RB - 1) / L_RB, groups = std::min(std::min(L_RB, a.n_rows), a.n_adapters + 1);
-    if (a.n_adapters) {
-        k_lora_shrink<T><<<dim3(blocks, groups, a.n_slices), 128, 0, st>>>(a);
-        count_launch();
-        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-    }
-    const size_t smem = (size_t)L_RB * (a.max_rank + 36) * sizeof(float);
-    cudaError_t e = allow_smem<k_lora_expand<T>>(smem);
+    cudaError_t e = allow_smem<k_lora_expand<T>>(l_expand_smem<T>());
     if (e != cudaSuccess) return e;
+    if (a.n_adapters) {
+        constexpr size_t smem = (size_t)l_stages<T>() * l_stage<T>();
+        if ((e = allow_smem<k_lora_shrink<T>>(smem)) != cudaSuccess) return e;
+        k_lora_shrink<T><<<dim3(blocks, groups, a.n_slices), 128, smem, st>>>(a);
+        count_launch();
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
     const dim3 grid(blocks, groups, (a.n_out + L_OUT - 1) / L_OUT);
-    if (a.n_adapters) return launch_pdl_(k_lora_expand<T>, grid, dim3(128), smem, st, a);
-    k_lora_expand<T><<<grid, 128, smem, st>>>(a);  // reads ids before its wait: only behind this call's own kernel
+    if (a.n_adapters) return launch_pdl_(k_lora_expand<T>, grid, dim3(128), l_expand_smem<T>(), st, a);
+    k_lora_expand<T><<<grid, 128, l_expand_smem<T>(), st>>>(a);  // reads ids before its wait: only behind this call's own kernel
     count_launch();
     return cudaGetLastError();
 }

@@ -70,6 +70,15 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
 }
 
+// 16 bytes global -> shared without registers; zeros when !in (nothing is read)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // 2^x to 2^-22 of it; results below the normal range are zero
 __device__ __forceinline__ float ex2(float x) {
     float y;
