@@ -85,23 +85,24 @@ __device__ __forceinline__ Group group_of(const LoraArgs &a, int r0, int j, int 
     return {__popc(ra) + __popc(rb), id};
 }
 
-// A tile of `rows` x `cols` elements in shared memory, rows `stride` bytes apart, from
-// rows at row_of(j) (null: zeros) of which `n` columns exist; 16 bytes at a time,
-// asynchronously where `wide` says that rows lie on 16 bytes.
+// A tile of `rows` x `cols` elements (cols a power of two) in shared memory, rows
+// `stride` bytes apart, from rows at row_of(j) (null: zeros) of which `n` columns
+// exist; 16 bytes at a time, asynchronously where `wide` says that rows lie on 16 bytes
+// (`any`: an address there). row_of is asked for a thread's rows in their order.
 template <class E, class F>
-__device__ __forceinline__ void load_tile(uint8_t *dst, int stride, int rows, int cols, int n, bool wide, F row_of) {
+__device__ __forceinline__ void load_tile(uint8_t *dst, int stride, int rows, int cols, int n, bool wide, F row_of, const E *any) {
     constexpr int N = 16 / (int)sizeof(E);
-    const int per = cols / N;
-    for (int i = threadIdx.x; i < rows * per; i += 128) {
-        const int j = i / per, c = (i % per) * N;
+    const int shift = 31 - __clz(cols / N), c = (threadIdx.x & ((1 << shift) - 1)) * N;  // a thread keeps its columns:
+    uint8_t *d = dst + c * (int)sizeof(E);                                               // there are at most 128 pieces a row
+    const bool fast = wide && (c + N <= n || c >= n);
+    for (int j = threadIdx.x >> shift; j < rows; j += 128 >> shift) {
         const E *src = row_of(j);
-        uint8_t *d = dst + j * stride + c * (int)sizeof(E);
-        if (wide && (c + N <= n || c >= n || !src)) {
+        if (fast) {
             const bool in = src && c < n;
-            cp_async16(smem_u32(d), in ? src + c : row_of(0), in);
+            cp_async16(smem_u32(d + j * stride), in ? src + c : any, in);
         } else {
 #pragma unroll
-            for (int k = 0; k < N; k++) reinterpret_cast<E *>(d)[k] = src && c + k < n ? src[c + k] : from_f32<E>(0.0f);
+            for (int k = 0; k < N; k++) reinterpret_cast<E *>(d + j * stride)[k] = src && c + k < n ? src[c + k] : from_f32<E>(0.0f);
         }
     }
 }
@@ -164,82 +165,99 @@ __device__ __forceinline__ void split_rows(uint32_t (&ah)[4][4], uint32_t (&al)[
 // 16 rows; warps left over split the depth of a tile and join in shared memory. x
 // and the weights come in tiles of 32 deep for each of the nk warps that split it,
 // through stages of asynchronous copies.
-template <class T> constexpr int l_stages() { return sizeof(T) == 4 ? 2 : 3; }
-constexpr int L_XTILE = 64 * (32 * 4 + 16);                                       // the largest of 64 x 32, 32 x 64, 16 x 128
-template <class T> constexpr int l_stage() { return L_XTILE + 64 * w_stride<T>(128); }  // and of the weights' 64 rows
+// bytes of a stage: 64 / nk rows of x and 64 of weights, 32 nk deep; as many stages,
+// up to four, as fit what three CTAs of an SM (f32 weights: two) can have
+template <class T> __host__ __device__ constexpr int l_xtile(int nk) { return 64 / nk * (128 * nk + 16); }
+template <class T> __host__ __device__ constexpr int l_stage(int nk) { return l_xtile<T>(nk) + 64 * w_stride<T>(32 * nk); }
+template <class T> __host__ __device__ constexpr int l_smem() { return 2 * l_stage<T>(4); }
 
 template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_rows[L_RB];
     pdl_trigger_();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const Group gr = group_of(a, blockIdx.x * L_RB, blockIdx.y, s_rows);
-    const int rank = gr.rows ? lora_rank(a, gr.id) : 0;
-    if (!rank) return;
-    __syncthreads();
-    const int nk = gr.rows <= 16 ? 4 : gr.rows <= 32 ? 2 : 1, mt = warp / nk, kp = warp % nk;
-    const int i0 = blockIdx.z * a.slice, i1 = min(i0 + a.slice, a.n_in), deep = 32 * nk;
-    const int xst = deep * 4 + 16, wst = w_stride<T>(deep), tiles = (i1 - i0 + deep - 1) / deep;
-    const T *w = static_cast<const T *>(a.a) + gr.id * a.a_adapter;
+    const int i0 = blockIdx.z * a.slice, i1 = min(i0 + a.slice, a.n_in);
     float *part = a.t + (size_t)blockIdx.z * a.n_rows * a.max_rank;
-    const bool busy = mt * 16 < gr.rows;
-    for (int k0 = 0; k0 < rank; k0 += L_NB * 8) {
-        const int cols = min(rank - k0, L_NB * 8);
-        auto fetch = [&](int i) {
-            if (i < tiles) {
-                uint8_t *st = smem + i % l_stages<T>() * l_stage<T>();
-                const int at = i0 + i * deep;
-                load_tile<float>(st, xst, (gr.rows + 15) / 16 * 16, deep, i1 - at, a.wide_x, [&](int j) {
-                    return j < gr.rows ? a.x + s_rows[j] * a.x_stride + at : (const float *)nullptr;
-                });
-                load_tile<T>(st + L_XTILE, wst, (cols + 7) / 8 * 8, deep, i1 - at, a.wide_a,
-                             [&](int j) { return j < cols ? w + (k0 + j) * a.a_row + at : (const T *)nullptr; });
-            }
-            cp_async_commit();
-        };
-        float c[L_NB][4];
+    for (int j = blockIdx.y;; j += gridDim.y) {
+        __syncthreads();  // the rows of the group before have been read
+        const Group gr = group_of(a, blockIdx.x * L_RB, j, s_rows);
+        if (!gr.rows) return;
+        const int rank = lora_rank(a, gr.id);
+        if (!rank) continue;
+        __syncthreads();
+        const int nk = gr.rows <= 16 ? 4 : gr.rows <= 32 ? 2 : 1, mt = warp / nk, kp = warp % nk, deep = 32 * nk;
+        const int xst = deep * 4 + 16, wst = w_stride<T>(deep), tiles = (i1 - i0 + deep - 1) / deep;
+        const int size = l_stage<T>(nk), stages = min(l_smem<T>() / size, 4), padded = (gr.rows + 15) / 16 * 16;
+        const T *w = static_cast<const T *>(a.a) + gr.id * a.a_adapter;
+        const bool busy = mt * 16 < gr.rows;
+        // the rows of x that this thread copies: the same in every tile
+        const int per = 8 * nk, first = tid / per, every = 128 / per;
+        const float *xr[4];
 #pragma unroll
-        for (int n = 0; n < L_NB; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
-        __syncthreads();  // the sums of the ranks before have been read
-        for (int i = 0; i < l_stages<T>() - 1; i++) fetch(i);
-        for (int i = 0; i < tiles; i++) {
-            cp_async_wait<l_stages<T>() - 2>();
+        for (int q = 0; q < 4; q++) xr[q] = first + q * every < gr.rows ? a.x + s_rows[first + q * every] * a.x_stride : nullptr;
+        for (int k0 = 0; k0 < rank; k0 += L_NB * 8) {
+            const int cols = min(rank - k0, L_NB * 8);
+            auto fetch = [&](int i) {
+                if (i < tiles) {
+                    uint8_t *st = smem + i % stages * size;
+                    const int at = i0 + i * deep;
+                    int q = 0;
+                    load_tile<float>(st, xst, padded, deep, i1 - at, a.wide_x, [&](int r) {
+                        const float *x = q == 0 ? xr[0] : q == 1 ? xr[1] : q == 2 ? xr[2] : xr[3];
+                        q++;
+                        return r < gr.rows ? x + at : (const float *)nullptr;
+                    }, a.x);
+                    load_tile<T>(st + l_xtile<T>(nk), wst, (cols + 7) / 8 * 8, deep, i1 - at, a.wide_a,
+                                 [&](int r) { return r < cols ? w + (k0 + r) * a.a_row + at : (const T *)nullptr; }, w);
+                }
+                cp_async_commit();
+            };
+            float c[L_NB][4];
+#pragma unroll
+            for (int n = 0; n < L_NB; n++) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.0f;
+            __syncthreads();  // the sums of the ranks before have been read
+            for (int i = 0; i < stages - 1; i++) fetch(i);
+            for (int i = 0; i < tiles; i++) {
+                if (stages == 4) cp_async_wait<2>();
+                else if (stages == 3) cp_async_wait<1>();
+                else cp_async_wait<0>();
+                __syncthreads();
+                fetch(i + stages - 1);  // into the stage that was read in the step before
+                const uint8_t *st = smem + i % stages * size;
+                if (busy) {
+                    float ua[8], ub[8];
+                    uint32_t ah[4][4], al[4][4];
+                    const float *x = reinterpret_cast<const float *>(st + (mt * 16 + g) * xst) + kp * 32 + 8 * t;
+                    read8(ua, x);
+                    read8(ub, x + 8 * (xst / 4));
+                    split_rows(ah, al, ua, ub);
+                    const uint8_t *ws = st + l_xtile<T>(nk) + g * wst + (kp * 32 + 8 * t) * (int)sizeof(T);
+#pragma unroll
+                    for (int n = 0; n < L_NB; n++)
+                        if (n * 8 < cols) {
+                            float v[8];
+                            read8(v, reinterpret_cast<const T *>(ws + n * 8 * wst));
+                            mma_32<T>(c[n], ah, al, v);
+                        }
+                }
+            }
+            cp_async_wait<0>();
             __syncthreads();
-            fetch(i + l_stages<T>() - 1);  // into the stage that was read in the step before
-            const uint8_t *st = smem + i % l_stages<T>() * l_stage<T>();
-            if (busy) {
-                float ua[8], ub[8];
-                uint32_t ah[4][4], al[4][4];
-                const float *x = reinterpret_cast<const float *>(st + (mt * 16 + g) * xst) + kp * 32 + 8 * t;
-                read8(ua, x);
-                read8(ub, x + 8 * (xst / 4));
-                split_rows(ah, al, ua, ub);
-                const uint8_t *ws = st + L_XTILE + g * wst + (kp * 32 + 8 * t) * (int)sizeof(T);
+            float(*s_t)[16][L_NB * 8 + 1] = reinterpret_cast<float(*)[16][L_NB * 8 + 1]>(smem);
 #pragma unroll
-                for (int n = 0; n < L_NB; n++)
-                    if (n * 8 < cols) {
-                        float v[8];
-                        read8(v, reinterpret_cast<const T *>(ws + n * 8 * wst));
-                        mma_32<T>(c[n], ah, al, v);
-                    }
+            for (int n = 0; n < L_NB; n++) {
+                s_t[warp][g][n * 8 + 2 * t] = c[n][0];
+                s_t[warp][g][n * 8 + 2 * t + 1] = c[n][1];
+                s_t[warp][g + 8][n * 8 + 2 * t] = c[n][2];
+                s_t[warp][g + 8][n * 8 + 2 * t + 1] = c[n][3];
             }
-        }
-        cp_async_wait<0>();
-        __syncthreads();
-        float(*s_t)[16][L_NB * 8 + 1] = reinterpret_cast<float(*)[16][L_NB * 8 + 1]>(smem);
-#pragma unroll
-        for (int n = 0; n < L_NB; n++) {
-            s_t[warp][g][n * 8 + 2 * t] = c[n][0];
-            s_t[warp][g][n * 8 + 2 * t + 1] = c[n][1];
-            s_t[warp][g + 8][n * 8 + 2 * t] = c[n][2];
-            s_t[warp][g + 8][n * 8 + 2 * t + 1] = c[n][3];
-        }
-        __syncthreads();
-        for (int j = tid; j < gr.rows * cols; j += 128) {
-            const int m = j / cols, k = j % cols;
-            float s = 0.0f;
-            for (int q = 0; q < nk; q++) s += s_t[(m / 16) * nk + q][m % 16][k];
-            part[(size_t)s_rows[m] * a.max_rank + k0 + k] = s;
+            __syncthreads();
+            for (int m = warp; m < gr.rows; m += 4)
+                for (int k = lane; k < cols; k += 32) {
+                    float s = 0.0f;
+                    for (int q = 0; q < nk; q++) s += s_t[(m / 16) * nk + q][m % 16][k];
+                    part[(size_t)s_rows[m] * a.max_rank + k0 + k] = s;
+                }
         }
     }
 }
@@ -256,103 +274,122 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs
     constexpr int WST = w_stride<T>(L_DEEP), TST = L_DEEP + 4;
     float *s_x = reinterpret_cast<float *>(smem + L_OUT * WST);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const Group gr = group_of(a, blockIdx.x * L_RB, blockIdx.y, s_rows);
-    if (!gr.rows) {
-        pdl_wait_();
-        return;
-    }
-    __syncthreads();
-    const int rank = lora_rank(a, gr.id);
-    const float scale = rank ? a.scales[gr.id] : 0.0f;
-    const int o0 = blockIdx.z * L_OUT, outs = min(L_OUT, a.n_out - o0);
-    const T *w = static_cast<const T *>(a.b) + (rank ? gr.id : 0) * a.b_adapter + o0 * a.b_row;
-    auto weights = [&](int k) {
-        const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
-        load_tile<T>(smem, WST, (outs + 7) / 8 * 8, deep, rank - k, a.wide_b,
-                     [&](int j) { return j < outs ? w + j * a.b_row + k : (const T *)nullptr; });
-        cp_async_commit();
-    };
-    if (rank) weights(0);
-    const int nc = gr.rows <= 16 ? 4 : gr.rows <= 32 ? 2 : 1, mt = warp / nc, cp = warp % nc;
-    const bool in[2] = {mt * 16 + g < gr.rows, mt * 16 + g + 8 < gr.rows};
-    const int64_t row[2] = {in[0] ? s_rows[mt * 16 + g] : 0, in[1] ? s_rows[mt * 16 + g + 8] : 0};
-    auto go = [&](auto tiles) {
-        constexpr int NT = decltype(tiles)::value;  // column tiles of 8
-        const int c0 = cp * NT * 8;
-        float c[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int o = c0 + n * 8 + 2 * t;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float2 b = make_float2(0.0f, 0.0f);
-                if (in[h] && a.base) {
-                    const float *p = a.base + row[h] * a.base_stride + o0 + o;
-                    if (a.wide_out && o + 1 < outs) {
-                        b = *reinterpret_cast<const float2 *>(p);
-                    } else {
-                        if (o < outs) b.x = p[0];
-                        if (o + 1 < outs) b.y = p[1];
-                    }
-                }
-                c[n][2 * h] = b.x;
-                c[n][2 * h + 1] = b.y;
-            }
-        }
-        pdl_wait_();  // t is there
-        for (int k = 0; k < rank; k += L_DEEP) {
+    for (int grp = blockIdx.y;; grp += gridDim.y) {
+        __syncthreads();  // the rows and tiles of the group before have been read
+        const Group gr = group_of(a, blockIdx.x * L_RB, grp, s_rows);
+        if (!gr.rows) break;
+        __syncthreads();
+        const int rank = lora_rank(a, gr.id);
+        const float scale = rank ? a.scales[gr.id] : 0.0f;
+        const int o0 = blockIdx.z * L_OUT, outs = min(L_OUT, a.n_out - o0);
+        const T *w = static_cast<const T *>(a.b) + (rank ? gr.id : 0) * a.b_adapter + o0 * a.b_row;
+        auto weights = [&](int k) {
             const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
-            if (k) {
-                __syncthreads();
-                weights(k);
-            }
-            for (int j = tid; j < (gr.rows + 15) / 16 * 16 * deep; j += 128) {
-                const int m = j / deep, q = k + j % deep;
-                float s = 0.0f;
-                if (m < gr.rows && q < rank) {
-                    const float *p = a.t + (size_t)s_rows[m] * a.max_rank + q;
-#pragma unroll 4
-                    for (int z = 0; z < a.n_slices; z++) s += __ldcg(p + (size_t)z * a.n_rows * a.max_rank);
-                }
-                s_x[m * TST + j % deep] = s * scale;
-            }
-            cp_async_wait<0>();
-            __syncthreads();
-            if (mt * 16 < gr.rows)
-                for (int q = 0; q < deep; q += 32) {
-                    float ua[8], ub[8];
-                    uint32_t ah[4][4], al[4][4];
-                    read8(ua, s_x + (mt * 16 + g) * TST + q + 8 * t);
-                    read8(ub, s_x + (mt * 16 + g + 8) * TST + q + 8 * t);
-                    split_rows(ah, al, ua, ub);
+            load_tile<T>(smem, WST, (outs + 7) / 8 * 8, deep, rank - k, a.wide_b,
+                         [&](int j) { return j < outs ? w + j * a.b_row + k : (const T *)nullptr; }, w);
+            cp_async_commit();
+        };
+        if (rank) weights(0);
+        const int nc = gr.rows <= 16 ? 4 : gr.rows <= 32 ? 2 : 1, mt = warp / nc, cp = warp % nc;
+        const bool in[2] = {mt * 16 + g < gr.rows, mt * 16 + g + 8 < gr.rows};
+        const int64_t row[2] = {in[0] ? s_rows[mt * 16 + g] : 0, in[1] ? s_rows[mt * 16 + g + 8] : 0};
+        auto go = [&](auto tiles) {
+            constexpr int NT = decltype(tiles)::value;  // column tiles of 8
+            const int c0 = cp * NT * 8;
+            float c[NT][4];
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        if (c0 + n * 8 < outs) {
-                            float v[8];
-                            read8(v, reinterpret_cast<const T *>(smem + (c0 + n * 8 + g) * WST) + q + 8 * t);
-                            mma_32<T>(c[n], ah, al, v);
+            for (int n = 0; n < NT; n++) {
+                const int o = c0 + n * 8 + 2 * t;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float2 b = make_float2(0.0f, 0.0f);
+                    if (in[h] && a.base) {
+                        const float *p = a.base + row[h] * a.base_stride + o0 + o;
+                        if (a.wide_out && o + 1 < outs) {
+                            b = *reinterpret_cast<const float2 *>(p);
+                        } else {
+                            if (o < outs) b.x = p[0];
+                            if (o + 1 < outs) b.y = p[1];
+                        }
+                    }
+                    c[n][2 * h] = b.x;
+                    c[n][2 * h + 1] = b.y;
+                }
+            }
+            pdl_wait_();  // t is there
+            for (int k = 0; k < rank; k += L_DEEP) {
+                const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
+                if (k) {
+                    __syncthreads();
+                    weights(k);
+                }
+                const size_t next = (size_t)a.n_rows * a.max_rank;  // from part to part
+                if (a.max_rank % 4 == 0) {  // 16 ranks a row's quarter warp, four at a time
+                    for (int m = tid >> 4; m < (gr.rows + 15) / 16 * 16; m += 8) {
+                        const int q = (tid & 15) * 4;
+                        if (q >= deep) continue;
+                        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (m < gr.rows && k + q < rank) {
+                            const float *p = a.t + (size_t)s_rows[m] * a.max_rank + k + q;
+#pragma unroll 8
+                            for (int z = 0; z < a.n_slices; z++) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + z * next));
+                                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+                            }
+                        }
+                        const int left = rank - k - q;  // what lies past the rank was not written
+                        *reinterpret_cast<float4 *>(s_x + m * TST + q) =
+                            make_float4(left > 0 ? s.x * scale : 0.0f, left > 1 ? s.y * scale : 0.0f, left > 2 ? s.z * scale : 0.0f,
+                                        left > 3 ? s.w * scale : 0.0f);
+                    }
+                } else {
+                    for (int m = warp; m < (gr.rows + 15) / 16 * 16; m += 4)
+                        for (int q = lane; q < deep; q += 32) {
+                            float s = 0.0f;
+                            if (m < gr.rows && k + q < rank)
+                                for (int z = 0; z < a.n_slices; z++) s += __ldcg(a.t + z * next + (size_t)s_rows[m] * a.max_rank + k + q);
+                            s_x[m * TST + q] = s * scale;
                         }
                 }
-        }
+                cp_async_wait<0>();
+                __syncthreads();
+                if (mt * 16 < gr.rows)
+                    for (int q = 0; q < deep; q += 32) {
+                        float ua[8], ub[8];
+                        uint32_t ah[4][4], al[4][4];
+                        read8(ua, s_x + (mt * 16 + g) * TST + q + 8 * t);
+                        read8(ub, s_x + (mt * 16 + g + 8) * TST + q + 8 * t);
+                        split_rows(ah, al, ua, ub);
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int o = c0 + n * 8 + 2 * t;
+                        for (int n = 0; n < NT; n++)
+                            if (c0 + n * 8 < outs) {
+                                float v[8];
+                                read8(v, reinterpret_cast<const T *>(smem + (c0 + n * 8 + g) * WST) + q + 8 * t);
+                                mma_32<T>(c[n], ah, al, v);
+                            }
+                    }
+            }
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (!in[h]) continue;
-                float *p = a.out + row[h] * a.out_stride + o0 + o;
-                if (a.wide_out && o + 1 < outs) {
-                    *reinterpret_cast<float2 *>(p) = make_float2(c[n][2 * h], c[n][2 * h + 1]);
-                } else {
-                    if (o < outs) p[0] = c[n][2 * h];
-                    if (o + 1 < outs) p[1] = c[n][2 * h + 1];
+            for (int n = 0; n < NT; n++) {
+                const int o = c0 + n * 8 + 2 * t;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (!in[h]) continue;
+                    float *p = a.out + row[h] * a.out_stride + o0 + o;
+                    if (a.wide_out && o + 1 < outs) {
+                        *reinterpret_cast<float2 *>(p) = make_float2(c[n][2 * h], c[n][2 * h + 1]);
+                    } else {
+                        if (o < outs) p[0] = c[n][2 * h];
+                        if (o + 1 < outs) p[1] = c[n][2 * h + 1];
+                    }
                 }
             }
-        }
-    };
-    if (nc == 4) go(std::integral_constant<int, L_OUT / 32>{});
-    else if (nc == 2) go(std::integral_constant<int, L_OUT / 16>{});
-    else go(std::integral_constant<int, L_OUT / 8>{});
+        };
+        if (nc == 4) go(std::integral_constant<int, L_OUT / 32>{});
+        else if (nc == 2) go(std::integral_constant<int, L_OUT / 16>{});
+        else go(std::integral_constant<int, L_OUT / 8>{});
+    }
+    pdl_wait_();  // also where there was nothing to do
 }
 
 const char *check(const loom_lora_desc *d) {
@@ -378,17 +415,22 @@ size_t slices_of(const loom_lora_desc *d) { return (d->n_in + slice_of(d) - 1) /
 size_t ws_bytes_of(const loom_lora_desc *d) { return slices_of(d) * d->n_rows * d->max_rank * sizeof(float); }
 
 template <class T> cudaError_t launch(const LoraArgs &a, cudaStream_t st) {
-    const unsigned blocks = (a.n_rows + L_RB - 1) / L_RB, groups = std::min(std::min(L_RB, a.n_rows), a.n_adapters + 1);
+    const unsigned blocks = (a.n_rows + L_RB - 1) / L_RB, most = std::min(std::min(L_RB, a.n_rows), a.n_adapters + 1);
+    // A CTA per adapter of a decode batch's one block; of a prompt's blocks, whose rows
+    // come in runs, as many as fill the GPU, each taking several adapters in turn where
+    // there are more.
+    auto groups = [&](unsigned others) { return blocks == 1 ? most : std::min(most, std::max(2u, 6 * 148 / (blocks * others))); };
     cudaError_t e = allow_smem<k_lora_expand<T>>(l_expand_smem<T>());
     if (e != cudaSuccess) return e;
     if (a.n_adapters) {
-        constexpr size_t smem = (size_t)l_stages<T>() * l_stage<T>();
+        constexpr size_t smem = l_smem<T>();
         if ((e = allow_smem<k_lora_shrink<T>>(smem)) != cudaSuccess) return e;
-        k_lora_shrink<T><<<dim3(blocks, groups, a.n_slices), 128, smem, st>>>(a);
+        k_lora_shrink<T><<<dim3(blocks, groups(a.n_slices), a.n_slices), 128, smem, st>>>(a);
         count_launch();
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
-    const dim3 grid(blocks, groups, (a.n_out + L_OUT - 1) / L_OUT);
+    const unsigned outs = (a.n_out + L_OUT - 1) / L_OUT;
+    const dim3 grid(blocks, groups(outs), outs);
     if (a.n_adapters) return launch_pdl_(k_lora_expand<T>, grid, dim3(128), l_expand_smem<T>(), st, a);
     k_lora_expand<T><<<grid, 128, l_expand_smem<T>(), st>>>(a);  // reads ids before its wait: only behind this call's own kernel
     count_launch();
