@@ -112,44 +112,61 @@ __device__ __forceinline__ void read8(float (&v)[8], const float *p) {
     const float4 u = *reinterpret_cast<const float4 *>(p), w = *reinterpret_cast<const float4 *>(p + 4);
     v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
 }
-template <class T> __device__ __forceinline__ void read8(float (&v)[8], const T *p) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const float2 f = unpack2<T>(w[k]);
-        v[2 * k] = f.x, v[2 * k + 1] = f.y;
-    }
-}
 // bytes between rows of a tile of `cols` weights: the quarter warps that read 8 rows'
 // worth of 16 bytes at once touch every bank
 template <class T> __host__ __device__ constexpr int w_stride(int cols) {
     return sizeof(T) == 4 ? cols * 4 + 16 : cols * 2 + (cols == 32 ? 0 : 64);
 }
 
-// c += (16 rows x 32) . (32 x 8) for the lane's eight elements of each operand:
-// ua, ub of rows g and g + 8, w of column g. The 32 are summed from zero by the
-// tensor core and added to c by f32 additions, which round where it truncates.
-template <class T>
-__device__ __forceinline__ void mma_32(float (&c)[4], const uint32_t (&ah)[4][4], const uint32_t (&al)[4][4], const float (&w)[8]) {
-    float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+// c[n] += (16 rows x 32) . (32 x 8) for NT column tiles, the lane's eight elements of
+// each: rows g and g + 8 split in ah, al, weights of column g of tile n at w + n * 8
+// rows of `stride` bytes. The 32 are summed from zero by the tensor core and added to
+// c by f32 additions, which round where it truncates; the tiles take turns, since a
+// product that adds to the one before it waits for it.
+template <class T, int NT>
+__device__ __forceinline__ void mma_tiles(float (*c)[4], const uint32_t (&ah)[4][4], const uint32_t (&al)[4][4], const uint8_t *w,
+                                          int stride) {
+    constexpr int P = sizeof(T) == 4 ? 2 : 1;
+    uint4 raw[NT][P];
+    float e[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int p = 0; p < P; p++) raw[n][p] = *reinterpret_cast<const uint4 *>(w + n * 8 * stride + p * 16);
+        e[n][0] = e[n][1] = e[n][2] = e[n][3] = 0.0f;
+    }
 #pragma unroll
     for (int s = 0; s < 4; s++) {
         if constexpr (sizeof(T) == 4) {
-            uint32_t bh[2], bl[2];
-            split_tf32(w[2 * s], bh[0], bl[0]);
-            split_tf32(w[2 * s + 1], bh[1], bl[1]);
-            mma_tf32(e, al[s], bh[0], bh[1]);
-            mma_tf32(e, ah[s], bl[0], bl[1]);
-            mma_tf32(e, ah[s], bh[0], bh[1]);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const uint4 &r = raw[n][s / 2];
+                uint32_t bh[2], bl[2];
+                split_tf32(__uint_as_float(s % 2 ? r.z : r.x), bh[0], bl[0]);
+                split_tf32(__uint_as_float(s % 2 ? r.w : r.y), bh[1], bl[1]);
+                mma_tf32(e[n], al[s], bh[0], bh[1]);
+                mma_tf32(e[n], ah[s], bl[0], bl[1]);
+                mma_tf32(e[n], ah[s], bh[0], bh[1]);
+            }
         } else {  // 8 or 11 significant bits: whole in tf32
-            const uint32_t b0 = __float_as_uint(w[2 * s]), b1 = __float_as_uint(w[2 * s + 1]);
-            mma_tf32(e, al[s], b0, b1);
-            mma_tf32(e, ah[s], b0, b1);
+            uint32_t b[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const uint4 &r = raw[n][0];
+                const float2 f = unpack2<T>(s == 0 ? r.x : s == 1 ? r.y : s == 2 ? r.z : r.w);
+                b[n][0] = __float_as_uint(f.x);
+                b[n][1] = __float_as_uint(f.y);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma_tf32(e[n], al[s], b[n][0], b[n][1]);
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma_tf32(e[n], ah[s], b[n][0], b[n][1]);
         }
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) c[j] += e[j];
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) c[n][j] += e[n][j];
 }
 __device__ __forceinline__ void split_rows(uint32_t (&ah)[4][4], uint32_t (&al)[4][4], const float (&ua)[8], const float (&ub)[8]) {
 #pragma unroll
@@ -207,7 +224,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
                         q++;
                         return r < gr.rows ? x + at : (const float *)nullptr;
                     }, a.x);
-                    load_tile<T>(st + l_xtile<T>(nk), wst, (cols + 7) / 8 * 8, deep, i1 - at, a.wide_a,
+                    load_tile<T>(st + l_xtile<T>(nk), wst, cols > 32 ? 64 : (cols + 15) / 16 * 16, deep, i1 - at, a.wide_a,
                                  [&](int r) { return r < cols ? w + (k0 + r) * a.a_row + at : (const T *)nullptr; }, w);
                 }
                 cp_async_commit();
@@ -232,13 +249,9 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
                     read8(ub, x + 8 * (xst / 4));
                     split_rows(ah, al, ua, ub);
                     const uint8_t *ws = st + l_xtile<T>(nk) + g * wst + (kp * 32 + 8 * t) * (int)sizeof(T);
-#pragma unroll
-                    for (int n = 0; n < L_NB; n++)
-                        if (n * 8 < cols) {
-                            float v[8];
-                            read8(v, reinterpret_cast<const T *>(ws + n * 8 * wst));
-                            mma_32<T>(c[n], ah, al, v);
-                        }
+                    mma_tiles<T, 2>(c, ah, al, ws, wst);
+                    if (cols > 16) mma_tiles<T, 2>(c + 2, ah, al, ws + 16 * wst, wst);
+                    if (cols > 32) mma_tiles<T, 4>(c + 4, ah, al, ws + 32 * wst, wst);
                 }
             }
             cp_async_wait<0>();
@@ -285,7 +298,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs
         const T *w = static_cast<const T *>(a.b) + (rank ? gr.id : 0) * a.b_adapter + o0 * a.b_row;
         auto weights = [&](int k) {
             const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
-            load_tile<T>(smem, WST, (outs + 7) / 8 * 8, deep, rank - k, a.wide_b,
+            load_tile<T>(smem, WST, L_OUT, deep, rank - k, a.wide_b,
                          [&](int j) { return j < outs ? w + j * a.b_row + k : (const T *)nullptr; }, w);
             cp_async_commit();
         };
@@ -361,12 +374,8 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs
                         read8(ub, s_x + (mt * 16 + g + 8) * TST + q + 8 * t);
                         split_rows(ah, al, ua, ub);
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
-                            if (c0 + n * 8 < outs) {
-                                float v[8];
-                                read8(v, reinterpret_cast<const T *>(smem + (c0 + n * 8 + g) * WST) + q + 8 * t);
-                                mma_32<T>(c[n], ah, al, v);
-                            }
+                        for (int n = 0; n < NT; n += 4)
+                            mma_tiles<T, 4>(c + n, ah, al, smem + (c0 + n * 8 + g) * WST + (q + 8 * t) * (int)sizeof(T), WST);
                     }
             }
 #pragma unroll
