@@ -58,16 +58,29 @@ def _laid(t, strides) -> bool:
     return t.numel() == 0 or all(w is None or s == w or n == 1 for s, w, n in zip(t.stride(), strides, t.shape))
 
 
-def _workspace(n: int, dev: int, stream: Optional[int]):
-    """Scratch from torch's allocator (kept from reuse until a stream other than the current one is done with it), and
-    the stream of the call."""
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    cur = torch.cuda.current_stream(dev).cuda_stream
-    if stream is None or stream == cur:
-        return ws, cur
-    if n:
-        ws.record_stream(torch.cuda.ExternalStream(stream, device=dev))
-    return ws, stream
+_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(dev).cuda_stream gives, 1.2 us sooner
+_capturing = torch.cuda.is_current_stream_capturing
+_kept = {}          # (device, stream) -> scratch of calls on that stream, in their order
+_KEEP = 4 << 20     # bytes of it; calls that need more take theirs from torch's allocator
+
+
+def _run(op: str, entry, size, desc, args, dev: int, stream: Optional[int]) -> None:
+    """One call: its stream (the current one unless given) and scratch, the refusal as LoomCudaError. Small calls on one
+    stream share a buffer, as they run one after the other; one that is being captured gets its own, which the graph
+    keeps."""
+    cur = _stream(dev)
+    st = cur if stream is None else stream
+    if st == cur and not _capturing():
+        ws = _kept.get((dev, cur))
+        if ws is None:
+            ws = _kept[dev, cur] = torch.empty(_KEEP, dtype=torch.uint8, device=dev)
+        if entry(desc, *args, ws.data_ptr(), _KEEP, cur) == _lib.OK:
+            return
+    need = size(desc)  # larger, captured, on a stream of the caller's, or refused: then for the reason it names
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    if st != cur and need:
+        ws.record_stream(torch.cuda.ExternalStream(st, device=dev))
+    _lib.must(entry(desc, *args, ws.data_ptr(), need, st), op)
 
 
 def attn_shared(q, prefix_k, prefix_v, own_k, own_v, seq_rows, seq_len, scale: float, out=None,
@@ -114,13 +127,9 @@ def attn_shared(q, prefix_k, prefix_v, own_k, own_v, seq_rows, seq_len, scale: f
     ref = C.byref(_lib.AttnSharedDesc(TYPES[ty], scale, seqs, n, h, kv, hd, qst[0], dst[0], pre, pst[0], pst[1], cap,
                                       ost[1], ost[2], ost[0]))
     L = _lib.lib()
-    need = L.loom_cuda_attn_shared_workspace(ref)
-    ws, st = _workspace(need, dev, stream)
-    rc = L.loom_cuda_attn_shared(ref, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), own_k.data_ptr(),
-                                 own_v.data_ptr(), seq_rows.data_ptr(), seq_len.data_ptr(), out.data_ptr(),
-                                 ws.data_ptr(), need, st)
-    if rc:
-        _lib.must(rc, "attn_shared")
+    _run("attn_shared", L.loom_cuda_attn_shared, L.loom_cuda_attn_shared_workspace, ref,
+         (q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), own_k.data_ptr(), own_v.data_ptr(),
+          seq_rows.data_ptr(), seq_len.data_ptr(), out.data_ptr()), dev, stream)
     return out
 
 
@@ -159,13 +168,9 @@ def lora(x, a, b, ranks, scales, ids, base=None, out=None, stream: Optional[int]
     ref = C.byref(_lib.LoraDesc(TYPES[ty], n, nin, nout, na, rank, xst[0], cst[0], dst[0], ast[1], ast[0], bst[1],
                                 bst[0]))
     L = _lib.lib()
-    need = L.loom_cuda_lora_workspace(ref)
-    ws, st = _workspace(need, dev, stream)
-    rc = L.loom_cuda_lora(ref, x.data_ptr(), a.data_ptr(), b.data_ptr(), ranks.data_ptr(), scales.data_ptr(),
-                          ids.data_ptr(), None if base is None else base.data_ptr(), out.data_ptr(), ws.data_ptr(),
-                          need, st)
-    if rc:
-        _lib.must(rc, "lora")
+    _run("lora", L.loom_cuda_lora, L.loom_cuda_lora_workspace, ref,
+         (x.data_ptr(), a.data_ptr(), b.data_ptr(), ranks.data_ptr(), scales.data_ptr(), ids.data_ptr(),
+          None if base is None else base.data_ptr(), out.data_ptr()), dev, stream)
     return out
 
 
@@ -212,12 +217,8 @@ def verify(logits, tokens, seq_rows, u, temperature=None, draft_probs=None, out=
             _refuse("verify", dev, want)
     ref = C.byref(_lib.VerifyDesc(TYPES[ty], seqs, n, v, lst[0], pst[0]))
     L = _lib.lib()
-    need = L.loom_cuda_verify_workspace(ref)
-    ws, st = _workspace(need, dev, stream)
-    rc = L.loom_cuda_verify(ref, logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
-                            tokens.data_ptr(), seq_rows.data_ptr(), u.data_ptr(),
-                            None if temperature is None else temperature.data_ptr(), tok.data_ptr(), cnt.data_ptr(),
-                            lp.data_ptr(), ws.data_ptr(), need, st)
-    if rc:
-        _lib.must(rc, "verify")
+    _run("verify", L.loom_cuda_verify, L.loom_cuda_verify_workspace, ref,
+         (logits.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(),
+          seq_rows.data_ptr(), u.data_ptr(), None if temperature is None else temperature.data_ptr(), tok.data_ptr(),
+          cnt.data_ptr(), lp.data_ptr()), dev, stream)
     return out
