@@ -70,6 +70,15 @@ __device__ __forceinline__ float weight(float l, float top, float inv) {
     return e == e ? e : 0.0f;
 }
 
+__device__ __forceinline__ double running(double v) {  // sum over the lanes up to this one
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -225,7 +234,7 @@ template <class T> struct RowPieces {
 // parts meet in row_stat, so the cluster meets once, for the maximum). Reading the
 // logits once would take 14 us for 366 rows of 129,281 bf16; what bounds it is
 // issuing about 20 instructions per logit, half of them e^x.
-template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_rows(VerifyArgs a) {
+template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, sizeof(T) == 4 ? 2 : 3) k_verify_rows(VerifyArgs a) {
     __shared__ float s_best[V_W], s_cta;
     __shared__ double s_sum[V_W];
     __shared__ int s_arg;
@@ -311,8 +320,9 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
 }
 
 // One cluster per sequence: the accepted drafts, then one token. The sums of the
-// weights over the runs of all the cluster's warps say in whose run the chosen
-// index lies; that warp alone goes through its run again, and finds it.
+// weights over the runs of all the cluster's warps say in whose run the chosen index
+// lies, that warp's sums over its steps in which of them; it weighs that step again
+// and finds the index. Bound by the chain of such meetings and by reading the row.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_pick(VerifyArgs a) {
     __shared__ double s_sum[V_W], s_all[V_C * V_W];
     __shared__ int s_stop;
@@ -383,37 +393,65 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     const RowPieces<T> row(row_at(stop), a.vocab);
     const float *q = !full && a.probs ? a.probs + stop * a.probs_stride : nullptr;
     const int d = full ? -1 : a.tokens[stop + 1];
-    const int steps = row.steps();
+    const int steps = row.steps(), span = (steps + 31) / 32;
+    // The weights of the N elements from i on: max(p - q, 0), or without probabilities
+    // those of every token but the draft; after the last draft, and when that rest is
+    // empty, the target's own.
     bool rest = !full;
-    // weight of element i with logit l: max(p - q, 0), or without probabilities every
-    // token but the draft; after the last draft, and when that rest is empty, the
-    // target's own
-    auto w_of = [&](float l, int i) {
-        const float e = weight(l, s.top, inv);
-        if (!rest || i < 0 || i >= a.vocab) return e;
-        if (!q) return i == d ? 0.0f : e;
-        const float left = fsub(__fdiv_rn(e, s.z), __ldg(q + i));
-        return left > 0.0f ? left : 0.0f;
+    const bool wide = q && (reinterpret_cast<uintptr_t>(q - row.head) & 15) == 0;  // a piece's q in 16 bytes too
+    auto load_q = [&](float (&v)[N], int i) {
+        if (!rest || !q) return;
+        if (wide && i >= 0 && i + N <= a.vocab) {
+#pragma unroll
+            for (int k = 0; k < N; k += 4) {
+                const float4 f = __ldg(reinterpret_cast<const float4 *>(q + i + k));
+                v[k] = f.x, v[k + 1] = f.y, v[k + 2] = f.z, v[k + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) v[k] = i + k >= 0 && i + k < a.vocab ? __ldg(q + i + k) : 0.0f;
+        }
     };
+    auto weigh = [&](float (&w)[N], const Piece<T> &p, const float (&v)[N], int i) {
+#pragma unroll
+        for (int k = 0; k < N; k++) w[k] = weight(p.get(k), s.top, inv);
+        if (!rest) return;
+        if (!q) {
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (i + k == d) w[k] = 0.0f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) w[k] = fmaxf(fsub(__fdiv_rn(w[k], s.z), v[k]), 0.0f);  // of a NaN, 0
+        }
+    };
+    double slot = 0.0;               // sum of this warp's steps span lane .. span (lane + 1) - 1
     double upto = 0.0, total = 0.0;  // of the sums of warps 4 lane .. 4 lane + 3, and of all
+    constexpr int BATCH = sizeof(T) == 4 ? 4 : 2;
     for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
         double mine = 0.0;
-        for (int j0 = 0; j0 < steps; j0 += 4) {
-            Piece<T> p[4];
+        slot = 0.0;
+        for (int j0 = 0; j0 < steps; j0 += BATCH) {
+            Piece<T> p[BATCH];
+            float v[BATCH][N];
 #pragma unroll
-            for (int j = 0; j < 4; j++) p[j] = row.load(j0 + j);  // past the run: past the row, or unused
-            Sum01 s;
+            for (int j = 0; j < BATCH; j++) {  // past the run: past the row, or unused
+                p[j] = row.load(j0 + j);
+                load_q(v[j], row.base(j0 + j));
+            }
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j0 + j < steps)
+            for (int j = 0; j < BATCH; j++) {
+                if (j0 + j >= steps) break;
+                float w[N];
+                weigh(w, p[j], v[j], row.base(j0 + j));
+                Sum01 sum;
 #pragma unroll
-                    for (int k = 0; k < N; k += 2) {
-                        const int i = row.base(j0 + j) + k;
-                        s.add(f2(w_of(p[j].get(k), i), w_of(p[j].get(k + 1), i + 1)));
-                    }
-            mine += s.get();
+                for (int k = 0; k < N; k += 2) sum.add(f2(w[k], w[k + 1]));
+                const double all = warp_sum_d(sum.get());
+                mine += all;
+                if ((j0 + j) / span == lane) slot += all;
+            }
         }
-        mine = warp_sum_d(mine);
         if (lane == 0) s_sum[warp] = mine;
         cluster_sync();
         if (tid < V_C * V_W) s_all[tid] = peer_ldd(peer(&s_sum[tid % V_W], tid / V_W));
@@ -421,12 +459,7 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         double four = 0.0;
 #pragma unroll
         for (int k = 0; k < 4; k++) four += s_all[4 * lane + k];
-        upto = four;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
+        upto = running(four);
         total = __shfl_sync(0xffffffffu, upto, 31);
         if (total > 0.0 || !rest) break;
         rest = false;
@@ -448,7 +481,7 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         }
         c += v;
     }
-    const uint32_t m = __ballot_sync(0xffffffffu, pick >= 0);
+    uint32_t m = __ballot_sync(0xffffffffu, pick >= 0);
     if (m) {
         pick = __shfl_sync(0xffffffffu, pick, __ffs(m) - 1);
         before = __shfl_sync(0xffffffffu, start, __ffs(m) - 1);
@@ -461,37 +494,35 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         return;
     }
     if (pick != (int)rank * V_W + warp) return;
+    // the same among the run's slots of steps, then step by step within the slot
+    const double ends = before + running(slot);
+    m = __ballot_sync(0xffffffffu, slot > 0.0 && ends > want);
+    const uint32_t some = __ballot_sync(0xffffffffu, slot > 0.0);
+    const int at = m ? __ffs(m) - 1 : 31 - __clz(some);
+    before = __shfl_sync(0xffffffffu, ends - slot, at);
     int first = -1, last = -1;
-    auto look = [&](const float (&e)[N], int j) {
+    for (int j = at * span; j < min((at + 1) * span, steps) && first < 0; j++) {
+        const Piece<T> p = row.load(j);
+        float v[N], e[N];
+        load_q(v, row.base(j));
+        weigh(e, p, v, row.base(j));
         double sum = 0.0;
 #pragma unroll
         for (int k = 0; k < N; k++) sum += e[k];
-        double run = sum;  // over the lanes
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double v = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += v;
-        }
-        double at = before + (run - sum);
+        const double run = running(sum);
+        double here = before + (run - sum);
         before += __shfl_sync(0xffffffffu, run, 31);
         int mine = 0x7FFFFFFF;
 #pragma unroll
         for (int k = 0; k < N; k++) {
-            at += e[k];
+            here += e[k];
             if (e[k] > 0.0f) {
                 last = max(last, row.base(j) + k);
-                if (at > want) mine = min(mine, row.base(j) + k);
+                if (here > want) mine = min(mine, row.base(j) + k);
             }
         }
         mine = __reduce_min_sync(0xffffffffu, mine);
         if (mine != 0x7FFFFFFF) first = mine;
-    };
-    for (int j = 0; j < steps && first < 0; j++) {
-        const Piece<T> p = row.load(j);
-        float e[N];
-#pragma unroll
-        for (int k = 0; k < N; k++) e[k] = w_of(p.get(k), row.base(j) + k);
-        look(e, j);
     }
     last = __reduce_max_sync(0xffffffffu, last);
     if (lane == 0) emit(first >= 0 ? first : max(last, 0));
