@@ -416,6 +416,41 @@ int loom_cuda_model_prefill(uint64_t handle, const uint32_t *tokens, size_t n, s
  * [B], or NULL). Synchronous. Declines MLA models. */
 int loom_cuda_model_decode_batch(uint64_t handle, const uint32_t *tokens, const uint32_t *positions, size_t B,
                                  float *logits, uint32_t *next);
+/* One step of many sequences that share a prompt, bring adapters and draft tokens
+ * (no counterpart in the reference; loom_cuda_attn_shared, loom_cuda_lora and
+ * loom_cuda_verify below, run through every layer): the prompt is positions
+ * 0 .. prefix_len - 1 of the single-sequence cache (loom_cuda_model_prefill), which
+ * all sequences read; sequence b's rows seq_rows[b] .. seq_rows[b + 1] - 1 (at least
+ * one: its last token, then its drafts) are the last of its seq_len[b] own
+ * positions, which follow the prompt, in the caches of loom_cuda_model_decode_batch.
+ * The drafts are judged and one more token chosen as loom_cuda_verify says, at
+ * temperature[b] (NULL: greedy) with the random numbers u (by row; NULL: zeros) and
+ * the drafter's probabilities d_draft_probs (device f32 [rows][vocab], NULL: a
+ * drafter without chance). out, n_out and logprobs (may be NULL) are those of
+ * loom_cuda_verify, logits (may be NULL) [rows][vocab]; host memory, like all but
+ * d_draft_probs and the adapters. After it a sequence has n_out[b] tokens more than
+ * before its rows: the accepted drafts, whose cache rows stand, and the chosen one,
+ * the first row of its next step, which starts n_out[b] positions after this one's.
+ * Synchronous. Declines MLA models and what the operators decline. */
+typedef struct {
+    int type; /* of the matrices: LOOM_F32, LOOM_F16 or LOOM_BF16 */
+    size_t n_adapters, max_rank;
+    const int32_t *d_ranks; /* device [n_adapters] */
+    const float *d_scales;
+    /* host arrays [n_layers] of device pointers, A [n_adapters][max_rank][dim] and
+     * B [n_adapters][rows of the projection][max_rank]; NULL (array or entry): none */
+    const void *const *q_a, *const *q_b, *const *v_a, *const *v_b;
+} loom_model_adapters;
+typedef struct {
+    size_t n_seqs, prefix_len;
+    const uint32_t *seq_rows, *seq_len, *tokens;
+    const float *u, *temperature, *d_draft_probs;
+    const loom_model_adapters *adapters; /* NULL: none */
+    const int32_t *adapter_ids;          /* [n_seqs]; outside 0 .. n_adapters - 1: none */
+    int32_t *out, *n_out;
+    float *logprobs, *logits;
+} loom_shared_step;
+int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *step);
 /* Copy one cache row (layer, pos) of keys and values (n_kv*hd f32 each; with
  * MLA the compressed row, kv_lora f32, and the rope row, rope_dim f32) to the
  * host -- the read-back that keeps a host copy authoritative (mlaReadCache,

@@ -100,6 +100,17 @@ class VerifyDesc(C.Structure):  # loom_verify_desc
         "n_seqs", "n_rows", "vocab", "logits_stride", "probs_stride")]
 
 
+class ModelAdapters(C.Structure):  # loom_model_adapters
+    _fields_ = [("type", C.c_int), ("n_adapters", C.c_size_t), ("max_rank", C.c_size_t)] + [(n, C.c_void_p) for n in (
+        "d_ranks", "d_scales", "q_a", "q_b", "v_a", "v_b")]
+
+
+class SharedStep(C.Structure):  # loom_shared_step
+    _fields_ = [("n_seqs", C.c_size_t), ("prefix_len", C.c_size_t)] + [(n, C.c_void_p) for n in (
+        "seq_rows", "seq_len", "tokens", "u", "temperature", "d_draft_probs", "adapters", "adapter_ids", "out", "n_out",
+        "logprobs", "logits")]
+
+
 def header_symbols() -> list[str]:
     """Every function the public header declares."""
     src = open(HEADER).read()
@@ -180,6 +191,7 @@ def lib() -> C.CDLL:
         "loom_cuda_model_read_kv": (i, [u64, sz, sz, vp, vp]),
         "loom_cuda_model_prefill": (i, [u64, vp, sz, sz, vp, C.POINTER(C.c_uint32)]),
         "loom_cuda_model_decode_batch": (i, [u64, vp, vp, sz, vp, vp]),
+        "loom_cuda_model_shared_step": (i, [u64, C.POINTER(SharedStep)]),
         "loom_cuda_model_free": (i, [u64]),
         "loom_cuda_model_error": (i, [u64]),
         "loom_cuda_model_trace": (i, [u64, i, vp, sz]),

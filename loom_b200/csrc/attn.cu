@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(QR_WARPS * 32) k_qk_rope(float *q, float *k, c
                                                           const float *kn, int n_heads, int n_kv, int hd,
                                                           int rope_dim, int neox, const float *rope, float eps,
                                                           const uint32_t *pos_p, int ctx, float *kc, float *vc,
-                                                          int pos_rows, size_t cache_stride) {
+                                                          int pos_rows, size_t cache_stride, const uint32_t *row_seq) {
     __shared__ float hv_all[QR_WARPS][MAX_HD];
     __shared__ float inv_all[QR_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -153,12 +153,14 @@ __global__ void __launch_bounds__(QR_WARPS * 32) k_qk_rope(float *q, float *k, c
     q += (size_t)blockIdx.y * n_heads * hd;
     k += (size_t)blockIdx.y * n_kv * hd;
     v += (size_t)blockIdx.y * n_kv * hd;
-    kc += blockIdx.y * cache_stride;
-    vc += blockIdx.y * cache_stride;
     pdl_wait_();
     pdl_trigger_();
     if (head >= n_heads + n_kv) return;
-    // row blockIdx.y: position pos_p[y] of its own cache (a batch of sequences, pos_rows) or *pos_p + y
+    // row blockIdx.y: position pos_p[y] of its own cache (a batch of sequences, pos_rows; row_seq: of that
+    // sequence's) or *pos_p + y
+    const size_t owner = row_seq ? row_seq[blockIdx.y] : blockIdx.y;
+    kc += owner * cache_stride;
+    vc += owner * cache_stride;
     const int pos = pos_rows ? (int)pos_p[blockIdx.y] : (int)*pos_p + (int)blockIdx.y;
     if (pos >= ctx) return;
     const bool isk = head >= n_heads;
@@ -887,9 +889,10 @@ void launch_rmsnorm_q(float *x, const float *add, const float *w, int dim, float
 
 void launch_qk_rope(float *q, float *k, const float *v, const float *qn, const float *kn, int n_heads, int n_kv,
                     int hd, int rope_dim, int neox, const float *rope, float eps, const uint32_t *pos, int ctx,
-                    float *kc, float *vc, cudaStream_t st, int ntok, int pos_rows, size_t cache_stride) {
+                    float *kc, float *vc, cudaStream_t st, int ntok, int pos_rows, size_t cache_stride,
+                    const uint32_t *row_seq) {
     launch_pdl_(k_qk_rope, dim3(cdiv_u(n_heads + n_kv, QR_WARPS), ntok), dim3(QR_WARPS * 32), 0, st, q, k, v, qn, kn,
-                n_heads, n_kv, hd, rope_dim, neox, rope, eps, pos, ctx, kc, vc, pos_rows, cache_stride);
+                n_heads, n_kv, hd, rope_dim, neox, rope, eps, pos, ctx, kc, vc, pos_rows, cache_stride, row_seq);
 }
 
 bool launch_attention_prefill_rows(const float *q, const float *kc, const float *vc, int n_heads, int n_kv, int hd,

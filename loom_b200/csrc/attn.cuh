@@ -28,10 +28,12 @@ void launch_rmsnorm_q(float *x, const float *add, const float *w, int dim, float
 // ntok > 1: token i of a batch (q, k, v advance by one token's heads) at
 // position *pos + i; with pos_rows, token i is sequence i at position pos[i]
 // with its own cache rows at kc / vc + i * cache_stride (the same for the
-// attention launchers below).
+// attention launchers below); with row_seq, of sequence row_seq[i], which may
+// have several tokens.
 void launch_qk_rope(float *q, float *k, const float *v, const float *qn, const float *kn, int n_heads, int n_kv,
                     int hd, int rope_dim, int neox, const float *rope, float eps, const uint32_t *pos, int ctx,
-                    float *kc, float *vc, cudaStream_t st, int ntok = 1, int pos_rows = 0, size_t cache_stride = 0);
+                    float *kc, float *vc, cudaStream_t st, int ntok = 1, int pos_rows = 0, size_t cache_stride = 0,
+                    const uint32_t *row_seq = nullptr);
 // The ordered attention for a batch of ntok tokens at positions *pos + i
 // (llama.zig:1749-1774 stepBatch: token i sees cache rows 0..*pos + i only),
 // q and out [ntok][n_heads * hd]; one CTA per (query head, token).

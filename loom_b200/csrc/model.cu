@@ -118,6 +118,19 @@ struct Model {
     size_t bd_cap = 0;
     float *bkc = nullptr, *bvc = nullptr, *bd_logits = nullptr, *bd_part = nullptr;
     uint32_t *bd_pos = nullptr, *bd_next = nullptr;
+    // drafted steps of sequences that share a prompt (loom_cuda_model_shared_step)
+    size_t sh_rows = 0, sh_seqs = 0, sh_ws = 0;
+    float *sh_logits = nullptr;
+    uint32_t *sh_in = nullptr, *sh_out = nullptr, *sh_host = nullptr;  // one upload, one download, their pinned mirror
+    uint8_t *sh_scratch = nullptr;
+};
+
+// The parts of loom_cuda_model_shared_step that the layers need, on the device
+struct SharedRows {
+    size_t n_seqs, n_rows, prefix;
+    const uint32_t *pos, *row_seq, *seq_rows, *seq_len;
+    const int32_t *ids;
+    const loom_model_adapters *ad;
 };
 
 std::unordered_map<uint64_t, Model *> g_models;
@@ -139,6 +152,7 @@ void free_model(Model *m) {
     for (void *p : m->allocs) cudaFree(p);
     if (m->io_host) cudaFreeHost(m->io_host);
     if (m->h_logits) cudaFreeHost(m->h_logits);
+    if (m->sh_host) cudaFreeHost(m->sh_host);
     delete m;
 }
 
@@ -430,11 +444,65 @@ int run_prefill(Model &m, int n, int pos_base, cudaStream_t st) {
     return cur;  // the buffer holding the final rows
 }
 
+// The attention of a drafted step: queries as the projections leave them, the prefix
+// in the single-sequence cache, every sequence's rows in its own from position `prefix`.
+loom_attn_shared_desc shared_desc(const Model &m, size_t n_seqs, size_t n_rows, size_t prefix) {
+    const size_t kvd = m.nkv * m.hd;
+    loom_attn_shared_desc d{};
+    d.type = LOOM_F32;
+    d.scale = m.scale;
+    d.n_seqs = n_seqs;
+    d.n_rows = n_rows;
+    d.n_heads = m.nh;
+    d.n_kv_heads = m.nkv;
+    d.head_dim = m.hd;
+    d.q_stride = d.out_stride = m.nh * m.hd;
+    d.prefix_len = prefix;
+    d.prefix_pos_stride = d.own_pos_stride = kvd;
+    d.prefix_head_stride = d.own_head_stride = m.hd;
+    d.own_cap = m.ctx - prefix;
+    d.own_seq_stride = m.n_layers * m.ctx * kvd;
+    return d;
+}
+loom_lora_desc lora_desc(const Model &m, size_t n_rows, const loom_model_adapters &ad, size_t n_out) {
+    loom_lora_desc d{};
+    d.type = ad.type;
+    d.n_rows = n_rows;
+    d.n_in = d.x_stride = m.dim;
+    d.n_out = d.base_stride = d.out_stride = n_out;
+    d.n_adapters = ad.n_adapters;
+    d.max_rank = d.b_row_stride = ad.max_rank;
+    d.a_row_stride = m.dim;
+    d.a_adapter_stride = ad.max_rank * m.dim;
+    d.b_adapter_stride = n_out * ad.max_rank;
+    return d;
+}
+int adapt(Model &m, const SharedRows &sh, const void *a, const void *b, size_t n_out, float *y, cudaStream_t st) {
+    const loom_lora_desc d = lora_desc(m, sh.n_rows, *sh.ad, n_out);
+    return loom_cuda_lora(&d, m.pf_normed, a, b, sh.ad->d_ranks, sh.ad->d_scales, sh.ids, y, y, m.sh_scratch, m.sh_ws, st);
+}
+
+// the batch's caches (zeroed), logits and next tokens, sized by the first call
+int alloc_batch(Model &m, size_t B) {
+    if (m.bd_cap) return 0;
+    const size_t cache = B * m.n_layers * m.ctx * m.nkv * m.hd;
+    int rc = 0;
+    if ((rc = dalloc(m, m.bkc, cache, true)) || (rc = dalloc(m, m.bvc, cache, true)) ||
+        (rc = dalloc(m, m.bd_logits, B * m.vocab)) || (rc = dalloc(m, m.bd_pos, B)) || (rc = dalloc(m, m.bd_next, B)) ||
+        (rc = dalloc(m, m.bd_part, B * attn_part_floats((int)m.nh, (int)m.nkv, (int)m.hd, (int)m.ctx))))
+        return rc;
+    m.bd_cap = B;
+    return 0;
+}
+
 // llama.zig:1939 decodeBatch: B sequences one token each, sequence b at position pos[b] with its
 // own KV cache (m.bkc / m.bvc: [B][layers][ctx][kv dim]); the prefill's row-batched kernels with
 // per-row positions and cache bases, the attention per (head or KV head, sequence), the FFN of
-// all B rows on the expert-major batch path, then every row's final norm, head and argmax.
-int run_decode_batch(Model &m, int B, cudaStream_t st) {
+// all B rows on the expert-major path, then every row's final norm, head and argmax.
+// With `sh`, the B rows are those of its sequences, several to a sequence, behind a
+// prefix in the single-sequence cache: adapters on q and v, the attention over the
+// prefix and the own caches, and logits of every row without the argmax.
+int run_decode_batch(Model &m, int B, cudaStream_t st, const SharedRows *sh = nullptr) {
     const int dim = (int)m.dim, nh = (int)m.nh, nkv = (int)m.nkv, hd = (int)m.hd, qd = nh * hd;
     const size_t layer_stride = m.ctx * m.nkv * m.hd, seq_stride = m.n_layers * layer_stride;
     const XQW none{};
@@ -448,10 +516,23 @@ int run_decode_batch(Model &m, int B, cudaStream_t st) {
         matmul_rows(l.wq, m.pf_normed, m.pf_n256, m.pf_n32, B, m.pf_q, st);
         matmul_rows(l.wk, m.pf_normed, m.pf_n256, m.pf_n32, B, m.pf_k, st);
         matmul_rows(l.wv, m.pf_normed, m.pf_n256, m.pf_n32, B, m.pf_v, st);
+        if (sh && sh->ad) {
+            const loom_model_adapters &ad = *sh->ad;
+            if (ad.q_a && ad.q_a[li])
+                if (int rc = adapt(m, *sh, ad.q_a[li], ad.q_b[li], qd, m.pf_q, st)) return rc;
+            if (ad.v_a && ad.v_a[li])
+                if (int rc = adapt(m, *sh, ad.v_a[li], ad.v_b[li], nkv * hd, m.pf_v, st)) return rc;
+        }
         float *kc = m.bkc + li * layer_stride, *vc = m.bvc + li * layer_stride;
         launch_qk_rope(m.pf_q, m.pf_k, m.pf_v, l.qn, l.kn, nh, nkv, hd, (int)m.rope_dim, m.neox, m.rope, m.eps,
-                       m.bd_pos, (int)m.ctx, kc, vc, st, B, 1, seq_stride);
-        if (m.ordered_attn)
+                       sh ? sh->pos : m.bd_pos, (int)m.ctx, kc, vc, st, B, 1, seq_stride, sh ? sh->row_seq : nullptr);
+        if (sh) {
+            const loom_attn_shared_desc d = shared_desc(m, sh->n_seqs, sh->n_rows, sh->prefix);
+            const size_t at = li * layer_stride, skip = sh->prefix * nkv * hd;  // own rows lie at their positions
+            if (int rc = loom_cuda_attn_shared(&d, m.pf_q, m.kc + at, m.vc + at, kc + skip, vc + skip, sh->seq_rows, sh->seq_len,
+                                               m.pf_att, m.sh_scratch, m.sh_ws, st))
+                return rc;
+        } else if (m.ordered_attn)
             launch_attention_ordered_rows(m.pf_q, kc, vc, nh, nkv, hd, m.scale, m.bd_pos, (int)m.ctx, m.pf_att, B, st, 1,
                                           seq_stride);
         else  // the single-sequence step's split form, one grid over every sequence's chunks
@@ -479,8 +560,8 @@ int run_decode_batch(Model &m, int B, cudaStream_t st) {
             o32 = m.pf_n32;
     }
     launch_rmsnorm_q(m.pf_x[cur], nullptr, m.out_norm, dim, m.eps, m.pf_normed, o256, o32, m.serial_norm, st, B);
-    matmul_rows(m.out, m.pf_normed, m.pf_n256, m.pf_n32, B, m.bd_logits, st);
-    for (int b = 0; b < B; b++)
+    matmul_rows(m.out, m.pf_normed, m.pf_n256, m.pf_n32, B, sh ? m.sh_logits : m.bd_logits, st);
+    for (int b = 0; b < B && !sh; b++)
         if (int rc = loom_cuda_argmax(m.bd_logits + (size_t)b * m.vocab, m.vocab, m.bd_next + b, st)) return rc;
     MCK(cudaGetLastError());
     return LOOM_CUDA_OK;
@@ -952,15 +1033,7 @@ int loom_cuda_model_decode_batch(uint64_t handle, const uint32_t *tokens, const 
         if (tokens[i] >= m.vocab || positions[i] >= m.ctx) return rt_decline("decode_batch: token or position out of range");
     if ((size_t)ATT_ORDERED_LIMIT < m.ctx) return rt_decline("decode_batch: context beyond the ordered attention's limit");
     if (int rc = alloc_prefill(m, B)) return rc;
-    if (!m.bd_cap) {  // the sequences' caches (zeroed), logits and next tokens, sized by the first call
-        const size_t cache = B * m.n_layers * m.ctx * m.nkv * m.hd;
-        int rc = 0;
-        if ((rc = dalloc(m, m.bkc, cache, true)) || (rc = dalloc(m, m.bvc, cache, true)) ||
-            (rc = dalloc(m, m.bd_logits, B * m.vocab)) || (rc = dalloc(m, m.bd_pos, B)) || (rc = dalloc(m, m.bd_next, B)) ||
-            (rc = dalloc(m, m.bd_part, B * attn_part_floats((int)m.nh, (int)m.nkv, (int)m.hd, (int)m.ctx))))
-            return rc;
-        m.bd_cap = B;
-    }
+    if (int rc = alloc_batch(m, B)) return rc;
     if (int rc = loom_cuda_reserve(B, m.dim, std::max<size_t>(m.max_ffn, 1), m.max_ne, m.max_nu)) return rc;
     cudaStream_t st = rt_stream(nullptr);
     MCK(cudaMemcpyAsync(m.pf_tok, tokens, B * 4, cudaMemcpyHostToDevice, st));
@@ -969,6 +1042,104 @@ int loom_cuda_model_decode_batch(uint64_t handle, const uint32_t *tokens, const 
     if (logits) MCK(cudaMemcpyAsync(logits, m.bd_logits, B * m.vocab * 4, cudaMemcpyDeviceToHost, st));
     if (next) MCK(cudaMemcpyAsync(next, m.bd_next, B * 4, cudaMemcpyDeviceToHost, st));
     MCK(cudaStreamSynchronize(st));
+    return LOOM_CUDA_OK;
+}
+
+int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
+    if (int rc = rt_need_init()) return rc;
+    Model *mp = find(handle);
+    if (!mp) return rt_decline("unknown model handle");
+    Model &m = *mp;
+    if (m.mla) return rt_decline("shared_step: multi-head latent attention models decode one sequence");
+    if (m.persistent) return rt_decline("shared_step: not with the persistent whole-token kernel");
+    if (!s || !s->tokens || !s->seq_rows || !s->seq_len || !s->out || !s->n_out || s->n_seqs == 0)
+        return rt_decline("shared_step: no sequences");
+    const size_t n = s->n_seqs, rows = s->seq_rows[n];
+    if (m.bd_cap && n > m.bd_cap) return rt_decline("shared_step: more sequences than the first call's batch");
+    if (s->prefix_len >= m.ctx) return rt_decline("shared_step: the prefix fills the context");
+    if (s->seq_rows[0] != 0 || rows > (1u << 16)) return rt_decline("shared_step: rows must start at 0 and be at most 65536");
+    for (size_t b = 0; b < n; b++) {
+        if (s->seq_rows[b + 1] <= s->seq_rows[b]) return rt_decline("shared_step: every sequence needs a row");
+        const size_t own = s->seq_rows[b + 1] - s->seq_rows[b];
+        if (s->seq_len[b] < own || s->seq_len[b] > m.ctx - s->prefix_len)
+            return rt_decline("shared_step: a sequence's length must hold its rows and fit the context");
+    }
+    for (size_t r = 0; r < rows; r++)
+        if (s->tokens[r] >= m.vocab) return rt_decline("shared_step: token id out of range");
+    const loom_model_adapters *ad = s->adapters;
+    if (ad && (!s->adapter_ids || !ad->n_adapters || !ad->max_rank || !ad->d_ranks || !ad->d_scales ||
+               (ad->q_a && !ad->q_b) || (ad->v_a && !ad->v_b)))
+        return rt_decline("shared_step: adapters need ids, ranks, scales and both of their matrices");
+    const loom_verify_desc vd{LOOM_F32, n, rows, m.vocab, m.vocab, m.vocab};
+    const loom_attn_shared_desc adesc = shared_desc(m, n, rows, s->prefix_len);
+    size_t ws = std::max(loom_cuda_attn_shared_workspace(&adesc), loom_cuda_verify_workspace(&vd));
+    if (!ws) return rt_decline("shared_step: the attention does not take this model");
+    if (ad) {
+        for (size_t out : {m.nh * m.hd, m.nkv * m.hd}) {
+            const loom_lora_desc d = lora_desc(m, rows, *ad, out);
+            const size_t need = loom_cuda_lora_workspace(&d);
+            if (!need) return rt_decline("shared_step: adapters of a type, rank or number that loom_cuda_lora declines");
+            ws = std::max(ws, need);
+        }
+    }
+    if (int rc = alloc_prefill(m, rows)) return rc;
+    if (int rc = alloc_batch(m, n)) return rc;
+    int rc = 0;
+    const size_t words_in = 5 * rows + 3 * n + 1, words_out = 2 * rows + n;
+    if (rows > m.sh_rows || n > m.sh_seqs) {
+        const size_t r = std::max(rows, m.sh_rows), q = std::max(n, m.sh_seqs);
+        if ((rc = dalloc(m, m.sh_logits, r * m.vocab)) || (rc = dalloc(m, m.sh_in, 5 * r + 3 * q + 1)) ||
+            (rc = dalloc(m, m.sh_out, 2 * r + q)))
+            return rc;
+        if (m.sh_host) cudaFreeHost(m.sh_host);
+        m.sh_host = nullptr;
+        m.sh_rows = m.sh_seqs = 0;
+        MCK(cudaHostAlloc(&m.sh_host, (5 * r + 3 * q + 1) * 4, cudaHostAllocDefault));
+        m.sh_rows = r;
+        m.sh_seqs = q;
+    }
+    if (ws > m.sh_ws) {
+        m.sh_ws = 0;
+        if ((rc = dalloc(m, m.sh_scratch, ws))) return rc;
+        m.sh_ws = ws;
+    }
+    if ((rc = loom_cuda_reserve(rows, m.dim, std::max<size_t>(m.max_ffn, 1), m.max_ne, m.max_nu))) return rc;
+    // [tokens][positions][sequence of the row][adapter of the row][random numbers] by row, [first rows][lengths][temperatures]
+    cudaStream_t st = rt_stream(nullptr);
+    uint32_t *h = m.sh_host;
+    const float zero = 0.0f;
+    std::memcpy(h, s->tokens, rows * 4);
+    for (size_t b = 0; b < n; b++)
+        for (size_t r = s->seq_rows[b]; r < s->seq_rows[b + 1]; r++) {
+            h[rows + r] = (uint32_t)(s->prefix_len + s->seq_len[b] - (s->seq_rows[b + 1] - r));
+            h[2 * rows + r] = (uint32_t)b;
+            const int32_t id = ad ? s->adapter_ids[b] : -1;
+            std::memcpy(h + 3 * rows + r, &id, 4);
+            std::memcpy(h + 4 * rows + r, s->u ? s->u + r : &zero, 4);
+        }
+    std::memcpy(h + 5 * rows, s->seq_rows, (n + 1) * 4);
+    std::memcpy(h + 5 * rows + n + 1, s->seq_len, n * 4);
+    if (s->temperature)
+        std::memcpy(h + 5 * rows + 2 * n + 1, s->temperature, n * 4);
+    else
+        std::memset(h + 5 * rows + 2 * n + 1, 0, n * 4);
+    MCK(cudaMemcpyAsync(m.sh_in, h, words_in * 4, cudaMemcpyHostToDevice, st));
+    MCK(cudaMemcpyAsync(m.pf_tok, m.sh_in, rows * 4, cudaMemcpyDeviceToDevice, st));
+    const uint32_t *in = m.sh_in, *d_rows = in + 5 * rows;
+    const SharedRows sh{n,      rows,        s->prefix_len, in + rows, in + 2 * rows, d_rows, d_rows + n + 1,
+                        reinterpret_cast<const int32_t *>(in + 3 * rows), ad};
+    if ((rc = run_decode_batch(m, (int)rows, st, &sh))) return rc;
+    int32_t *out = reinterpret_cast<int32_t *>(m.sh_out);
+    if ((rc = loom_cuda_verify(&vd, m.sh_logits, s->d_draft_probs, reinterpret_cast<const int32_t *>(in), d_rows,
+                               reinterpret_cast<const float *>(in + 4 * rows), reinterpret_cast<const float *>(d_rows + 2 * n + 1),
+                               out, out + rows, reinterpret_cast<float *>(out + rows + n), m.sh_scratch, m.sh_ws, st)))
+        return rc;
+    MCK(cudaMemcpyAsync(h, m.sh_out, words_out * 4, cudaMemcpyDeviceToHost, st));
+    if (s->logits) MCK(cudaMemcpyAsync(s->logits, m.sh_logits, rows * m.vocab * 4, cudaMemcpyDeviceToHost, st));
+    MCK(cudaStreamSynchronize(st));
+    std::memcpy(s->out, h, rows * 4);
+    std::memcpy(s->n_out, h + rows, n * 4);
+    if (s->logprobs) std::memcpy(s->logprobs, h + rows + n, rows * 4);
     return LOOM_CUDA_OK;
 }
 

@@ -218,6 +218,49 @@ def deepseek_v3(n_layers: int = 61, ctx_len: int = 4096, n_expert: int = 256, vo
                                 ffn_down_dense=Q4_K, ffn_down_shexp=Q4_K), seed=seed)
 
 
+class Adapters:
+    """Low-rank adapters of a model's query and value projections, one set of matrices per layer.
+
+    q, v: per layer (a [n, max_rank, dim], b [n, rows of the projection, max_rank]) contiguous torch cuda tensors of one
+    type (float32, float16, bfloat16), or None; ranks, scales: per adapter."""
+
+    def __init__(self, q, v, ranks, scales):
+        import torch
+        from .serve import TYPES
+        pairs = [p for p in list(q or []) + list(v or []) if p is not None]
+        if not pairs:
+            raise _lib.LoomCudaError("adapters: no matrices")
+        n, rank, _ = pairs[0][0].shape
+        ty, dev = pairs[0][0].dtype, pairs[0][0].device
+        for a, b in pairs:
+            if (ty not in TYPES or a.dtype is not ty or b.dtype is not ty or tuple(a.shape[:2]) != (n, rank) or
+                    (b.shape[0], b.shape[2]) != (n, rank) or not a.is_contiguous() or not b.is_contiguous() or
+                    not a.is_cuda or a.device != dev or b.device != dev):
+                raise _lib.LoomCudaError("adapters: a [n, max_rank, dim] and b [n, rows, max_rank] must be contiguous cuda "
+                                         "tensors of one type")
+        self.q, self.v, self.n = q, v, n  # kept alive
+        self.ranks = torch.as_tensor(ranks, dtype=torch.int32, device=dev).contiguous()
+        self.scales = torch.as_tensor(scales, dtype=torch.float32, device=dev).contiguous()
+        if self.ranks.shape != (n,) or self.scales.shape != (n,):
+            raise _lib.LoomCudaError("adapters: ranks and scales must be [n]")
+
+        def table(layers, k):
+            if layers is None:
+                return None
+            return (C.c_void_p * len(layers))(*[None if p is None else p[k].data_ptr() for p in layers])
+
+        self._tables = [table(q, 0), table(q, 1), table(v, 0), table(v, 1)]
+        torch.cuda.current_stream(dev).synchronize()  # made on torch's stream, read on the backend's
+        self.c = _lib.ModelAdapters(TYPES[ty], n, rank, self.ranks.data_ptr(), self.scales.data_ptr(),
+                                    *[None if t is None else C.cast(t, C.c_void_p) for t in self._tables])
+
+    def fits(self, spec: "ModelSpec") -> bool:
+        rows = {"q": spec.n_heads * spec.head_dim, "v": spec.n_kv_heads * spec.head_dim}
+        return all(layers is None or (len(layers) == spec.n_layers and all(
+            p is None or (p[0].shape[2] == spec.dim and p[1].shape[1] == rows[k]) for p in layers))
+            for k, layers in (("q", self.q), ("v", self.v)))
+
+
 class DeviceModel:
     """A ModelSpec's tensors on the GPU plus the backend's model handle."""
 
@@ -312,6 +355,41 @@ class DeviceModel:
                                                           lg.ctypes.data_as(C.c_void_p) if logits else None,
                                                           nxt.ctypes.data_as(C.c_void_p)), "model_decode_batch")
         return nxt, lg
+
+    def shared_step(self, prefix_len: int, rows, seq_len, u=None, temperature=None, draft_probs=None, adapters=None,
+                    adapter_ids=None, logits: bool = False):
+        """One step of sequences that share the prompt of the last prefill (positions 0 .. prefix_len - 1).
+
+        rows: per sequence its last token, then its drafted tokens; seq_len: per sequence its own positions after the
+        prompt, these rows included; u: per row in [0, 1); temperature: per sequence (None: greedy); draft_probs: torch
+        cuda float32 [rows, vocab] or None; adapters: Adapters with adapter_ids per sequence (-1: none). Returns
+        (tokens per sequence: the accepted drafts and the chosen one, their log-probabilities, logits or None)."""
+        n = len(rows)
+        first = np.concatenate([[0], np.cumsum([len(r) for r in rows])]).astype(np.uint32)
+        total, v = int(first[-1]), self.spec.vocab
+        if len(seq_len) != n or (u is not None and len(u) != total) or (temperature is not None and len(temperature) != n):
+            raise _lib.LoomCudaError("shared_step: one length and temperature per sequence, one random number per row")
+        if adapters is not None and (adapter_ids is None or len(adapter_ids) != n or not adapters.fits(self.spec)):
+            raise _lib.LoomCudaError("shared_step: the adapters do not fit the model, or not one id per sequence")
+        if draft_probs is not None:
+            import torch
+            if not (draft_probs.is_cuda and draft_probs.dtype is torch.float32 and draft_probs.is_contiguous() and
+                    tuple(draft_probs.shape) == (total, v)):
+                raise _lib.LoomCudaError("shared_step: draft_probs must be contiguous cuda float32 [rows, vocab]")
+        arr = lambda x, ty: None if x is None else np.ascontiguousarray(np.asarray(x, dtype=ty))  # noqa: E731
+        tok, ln, uu = arr([t for r in rows for t in r], np.uint32), arr(seq_len, np.uint32), arr(u, np.float32)
+        tt, ids = arr(temperature, np.float32), arr(adapter_ids, np.int32)
+        out, cnt, lp = np.zeros(total, np.int32), np.zeros(n, np.int32), np.zeros(total, np.float32)
+        lg = np.empty((total, v), np.float32) if logits else None
+        p = lambda x: None if x is None else x.ctypes.data  # noqa: E731
+        if draft_probs is not None:  # made on torch's stream, read on the backend's
+            torch.cuda.current_stream(draft_probs.device).synchronize()
+        s = _lib.SharedStep(n, prefix_len, p(first), p(ln), p(tok), p(uu), p(tt),
+                            None if draft_probs is None else draft_probs.data_ptr(),
+                            None if adapters is None else C.addressof(adapters.c), p(ids), p(out), p(cnt), p(lp), p(lg))
+        _lib.must(_lib.lib().loom_cuda_model_shared_step(self.handle, C.byref(s)), "model_shared_step")
+        cut = [slice(int(first[b]), int(first[b]) + int(cnt[b])) for b in range(n)]
+        return [out[c].tolist() for c in cut], [lp[c].tolist() for c in cut], lg
 
     def step(self, d_token, d_pos, d_logits=None, d_next=None, stream=None) -> None:
         """The step on device buffers (torch cuda tensors: int32 [1])."""
