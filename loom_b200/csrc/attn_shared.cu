@@ -265,9 +265,13 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                 if constexpr (F) {
                     // lane t has dimensions 8t .. 8t + 7 of 32, in pieces 2t and 2t + 1, two
                     // for each of four products: any order sums to the same scores
-                    float small[NT][4];
+                    // (products that add to one result wait for one another: the tiles and the
+                    // two small terms take turns)
+                    float small[2][NT][4];
 #pragma unroll
-                    for (int n = 0; n < NT; n++) small[n][0] = small[n][1] = small[n][2] = small[n][3] = 0.0f;
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) small[0][n][j] = small[1][n][j] = 0.0f;
                     const float *qa = sq + (rt * 16 + g) * QST + 8 * t, *qb = qa + 8 * QST;
                     const uint8_t *kr = smb + (tk - sm0) + (sub + g) * 128;
 #pragma unroll 2
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                         for (int h = 0; h < 2; h++) {
                             const float4 ua = *reinterpret_cast<const float4 *>(qa + d * 32 + h * 4);
                             const float4 ub = *reinterpret_cast<const float4 *>(qb + d * 32 + h * 4);
-                            uint32_t ah[2][4], al[2][4];
+                            uint32_t ah[2][4], al[2][4], bh[NT][4], bl[NT][4];
                             split_tf32(ua.x, ah[0][0], al[0][0]);
                             split_tf32(ub.x, ah[0][1], al[0][1]);
                             split_tf32(ua.y, ah[0][2], al[0][2]);
@@ -285,30 +289,35 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                             split_tf32(ub.z, ah[1][1], al[1][1]);
                             split_tf32(ua.w, ah[1][2], al[1][2]);
                             split_tf32(ub.w, ah[1][3], al[1][3]);
+                            float e[NT][4];
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
                                 const float4 kk = *reinterpret_cast<const float4 *>(kr + d * BLK + n * 1024 + (((2 * t + h) ^ g) << 4));
-                                uint32_t bh[4], bl[4];
-                                split_tf32(kk.x, bh[0], bl[0]);
-                                split_tf32(kk.y, bh[1], bl[1]);
-                                split_tf32(kk.z, bh[2], bl[2]);
-                                split_tf32(kk.w, bh[3], bl[3]);
-                                float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                                for (int u = 0; u < 2; u++) {
-                                    mma_tf32(small[n], al[u], bh[2 * u], bh[2 * u + 1]);
-                                    mma_tf32(small[n], ah[u], bl[2 * u], bl[2 * u + 1]);
-                                    mma_tf32(e, ah[u], bh[2 * u], bh[2 * u + 1]);
-                                }
-#pragma unroll
-                                for (int j = 0; j < 4; j++) c[n][j] += e[j];
+                                split_tf32(kk.x, bh[n][0], bl[n][0]);
+                                split_tf32(kk.y, bh[n][1], bl[n][1]);
+                                split_tf32(kk.z, bh[n][2], bl[n][2]);
+                                split_tf32(kk.w, bh[n][3], bl[n][3]);
+                                e[n][0] = e[n][1] = e[n][2] = e[n][3] = 0.0f;
                             }
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                                for (int n = 0; n < NT; n++) mma_tf32(e[n], ah[u], bh[n][2 * u], bh[n][2 * u + 1]);
+#pragma unroll
+                                for (int n = 0; n < NT; n++) mma_tf32(small[0][n], al[u], bh[n][2 * u], bh[n][2 * u + 1]);
+#pragma unroll
+                                for (int n = 0; n < NT; n++) mma_tf32(small[1][n], ah[u], bl[n][2 * u], bl[n][2 * u + 1]);
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; n++)
+#pragma unroll
+                                for (int j = 0; j < 4; j++) c[n][j] += e[n][j];
                         }
                     }
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) c[n][j] += small[n][j];
+                        for (int j = 0; j < 4; j++) c[n][j] += small[0][n][j] + small[1][n][j];
                 } else {
                     // 16-byte piece c of a row is at c ^ (row % 8) of its block
                     const uint32_t row = tk + (sub + (lane >> 4) * 8 + (lane & 7)) * 128, x = ((lane >> 3) & 1) ^ (lane & 7);
@@ -379,24 +388,33 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                     }
                     const uint8_t *v0 = smb + (tv - sm0) + (sub + 2 * t) * 128 + (g & 3) * 4;
 #pragma unroll
-                    for (int i2 = 0; i2 < HDP / 8; i2++) {
-                        if (i2 * 8 < hd) {
-                            const int piece = ((2 * i2) & 7) + (g >> 2);
-                            const uint8_t *v = v0 + (i2 >> 2) * BLK;
-                            float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int i4 = 0; i4 < HDP / 8; i4 += 4) {  // a block of 32 dimensions, zeros past hd
+                        if (i4 * 8 < hd) {
+                            const uint8_t *v = v0 + (i4 >> 2) * BLK;
+                            float e[4][4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) e[i][0] = e[i][1] = e[i][2] = e[i][3] = 0.0f;
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
-                                uint32_t bh[2], bl[2];
-                                split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + ((piece ^ (2 * t)) << 4)), bh[0], bl[0]);
-                                split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + 128 + ((piece ^ (2 * t + 1)) << 4)), bh[1], bl[1]);
-                                mma_tf32(e, al[n], bh[0], bh[1]);
-                                mma_tf32(e, ah[n], bl[0], bl[1]);
-                                mma_tf32(e, ah[n], bh[0], bh[1]);
+                                uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    const int piece = 2 * i + (g >> 2);
+                                    split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + ((piece ^ (2 * t)) << 4)), bh[i][0], bl[i][0]);
+                                    split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + 128 + ((piece ^ (2 * t + 1)) << 4)),
+                                               bh[i][1], bl[i][1]);
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; i++) mma_tf32(e[i], al[n], bh[i][0], bh[i][1]);
+#pragma unroll
+                                for (int i = 0; i < 4; i++) mma_tf32(e[i], ah[n], bl[i][0], bl[i][1]);
+#pragma unroll
+                                for (int i = 0; i < 4; i++) mma_tf32(e[i], ah[n], bh[i][0], bh[i][1]);
                             }
-                            o[i2][0] += e[0];
-                            o[i2][1] += e[1];
-                            o[i2][2] += e[2];
-                            o[i2][3] += e[3];
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+#pragma unroll
+                                for (int j = 0; j < 4; j++) o[i4 + i][j] += e[i][j];
                         }
                     }
                 } else {

@@ -61,7 +61,7 @@ def _laid(t, strides) -> bool:
 _stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(dev).cuda_stream gives, 1.2 us sooner
 _capturing = torch.cuda.is_current_stream_capturing
 _kept = {}          # (device, stream) -> scratch of calls on that stream, in their order
-_KEEP = 4 << 20     # bytes of it; calls that need more take theirs from torch's allocator
+_KEEP = 32 << 20    # bytes of it; calls that need more take theirs from torch's allocator
 
 
 def _run(op: str, entry, size, desc, args, dev: int, stream: Optional[int]) -> None:
