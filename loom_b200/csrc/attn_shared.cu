@@ -153,7 +153,7 @@ template <class T, int HDP> constexpr size_t mma_smem() {  // stages (or the war
 }
 
 template <class T, int HDP>
-__global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __grid_constant__ AttnMaps maps) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_attn_shared_mma(AttnArgs a, const __grid_constant__ AttnMaps maps) {
     constexpr int TP = mma_tp<T>(), E = 128 / (int)sizeof(T);  // positions of a tile, dimensions of a block
     constexpr uint32_t BLK = mma_block<T>(), TILE = mma_tile<T, HDP>();
     constexpr bool F = sizeof(T) == 4;
@@ -324,10 +324,13 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
                         if (k * 16 < wide) {
-                            uint32_t b[4];
-                            ldmatrix_x4(b, row + (k >> 2) * BLK + ((((2 * k) & 7) ^ x) << 4));
-                            mma_k16<T>(c[0], qf[k], b[0], b[1]);
-                            mma_k16<T>(c[1], qf[k], b[2], b[3]);
+#pragma unroll
+                            for (int n = 0; n < NT; n += 2) {
+                                uint32_t b[4];
+                                ldmatrix_x4(b, row + n * 1024 + (k >> 2) * BLK + ((((2 * k) & 7) ^ x) << 4));
+                                mma_k16<T>(c[n], qf[k], b[0], b[1]);
+                                mma_k16<T>(c[n + 1], qf[k], b[2], b[3]);
+                            }
                         }
                     }
                 }
@@ -418,31 +421,39 @@ __global__ void __launch_bounds__(128) k_attn_shared_mma(AttnArgs a, const __gri
                         }
                     }
                 } else {
-                    uint32_t pf[4];
-                    pf[0] = pack2<T>(c[0][0], c[0][1]);
-                    pf[1] = pack2<T>(c[0][2], c[0][3]);
-                    pf[2] = pack2<T>(c[1][0], c[1][1]);
-                    pf[3] = pack2<T>(c[1][2], c[1][3]);
-                    const float2 r0 = unpack2<T>(pf[0]), r1 = unpack2<T>(pf[1]), r2 = unpack2<T>(pf[2]), r3 = unpack2<T>(pf[3]);
-                    l0 += (r0.x + r0.y) + (r2.x + r2.y);
-                    l1 += (r1.x + r1.y) + (r3.x + r3.y);
+                    uint32_t pf[NT / 2][4];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint32_t pa = pack2<T>(c[n][0], c[n][1]), pb = pack2<T>(c[n][2], c[n][3]);
+                        pf[n / 2][n % 2 * 2] = pa;
+                        pf[n / 2][n % 2 * 2 + 1] = pb;
+                        const float2 ra = unpack2<T>(pa), rb = unpack2<T>(pb);
+                        l0 += ra.x + ra.y;
+                        l1 += rb.x + rb.y;
+                    }
                     const uint32_t row = tv + (sub + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128, x = (lane >> 4) ^ (lane & 7);
 #pragma unroll
-                    for (int i2 = 0; i2 < HDP / 16; i2++) {
-                        if (i2 * 16 < wide) {
-                            uint32_t b[4];
-                            ldmatrix_x4_trans(b, row + (i2 >> 2) * BLK + ((((2 * i2) & 7) ^ x) << 4));
-                            mma_k16<T>(o[2 * i2], pf, b[0], b[1]);
-                            mma_k16<T>(o[2 * i2 + 1], pf, b[2], b[3]);
+                    for (int n = 0; n < NT / 2; n++)
+#pragma unroll
+                        for (int i2 = 0; i2 < HDP / 16; i2++) {
+                            if (i2 * 16 < wide) {
+                                uint32_t b[4];
+                                ldmatrix_x4_trans(b, row + n * 2048 + (i2 >> 2) * BLK + ((((2 * i2) & 7) ^ x) << 4));
+                                mma_k16<T>(o[2 * i2], pf[n], b[0], b[1]);
+                                mma_k16<T>(o[2 * i2 + 1], pf[n], b[2], b[3]);
+                            }
                         }
-                    }
                 }
             };
-            // f32: the warp's share of a tile at once (splitting the queries takes as long as
-            // a product, and serves all of the share's positions)
+            // 32 positions at a time where the warp has as many: fewer maxima, and f32 queries
+            // are split once for all of them
             if (busy) {
                 if constexpr (!F) {
-                    for (int sub = ps * 16; sub < here; sub += nps * 16) step(std::integral_constant<int, 2>{}, sub);
+                    if (nps == 4) {
+                        if (ps * 16 < here) step(std::integral_constant<int, 2>{}, ps * 16);
+                    } else {
+                        for (int sub = ps * 32; sub < here; sub += nps * 32) step(std::integral_constant<int, 4>{}, sub);
+                    }
                 } else if (nps == 1) {
                     step(std::integral_constant<int, 4>{}, 0);
                 } else if (nps == 2) {
