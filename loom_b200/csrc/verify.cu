@@ -26,27 +26,16 @@ namespace {
 
 constexpr int V_C = 8, V_W = 16, V_T = V_W * 32;  // CTAs of a cluster, warps of a CTA
 
-// What a row's cluster leaves: every CTA's part, read as one by row_stat
-struct RowParts {
-    double z[V_C];   // sums of e^((l - top) / T)
-    int arg[V_C];    // first index of the largest logit (greedy rows)
-    float top;       // the largest logit that is not NaN; -inf when none is above it
-    int pad[7];
+// One CTA's part of a row; row_stat reads a row's parts as one
+struct RowPart {
+    double z;   // sum of e^((l - top) / T) over its logits
+    float top;  // the row's largest logit, or the part's own (two passes); -inf when none is above it
+    int arg;    // first index of the row's largest among its logits (greedy rows), or 2^31 - 1
 };
 struct RowStat {
     float top, z;
     int arg;
 };
-__device__ __forceinline__ RowStat row_stat(const RowParts *p) {
-    double z = 0.0;
-    int arg = 0x7FFFFFFF;
-#pragma unroll
-    for (int c = 0; c < V_C; c++) {
-        z += p->z[c];
-        arg = min(arg, p->arg[c]);
-    }
-    return {p->top, (float)z, arg == 0x7FFFFFFF ? 0 : arg};
-}
 
 struct VerifyArgs {
     const void *logits;
@@ -55,9 +44,9 @@ struct VerifyArgs {
     const uint32_t *seq_rows;
     int32_t *out, *n_out;
     float *logprobs;
-    RowParts *stat;
+    RowPart *stat;  // [rows][parts]
     int64_t logits_stride, probs_stride;
-    int n_seqs, n_rows, vocab;
+    int n_seqs, n_rows, vocab, parts;
 };
 
 __device__ __forceinline__ float temp_of(const VerifyArgs &a, int b) { return a.temp ? a.temp[b] : 1.0f; }
@@ -92,6 +81,21 @@ __device__ __forceinline__ int seq_of(const VerifyArgs &a, int r) {
         if (a.seq_rows[mid] <= (uint32_t)r) lo = mid; else hi = mid;
     }
     return lo;
+}
+
+// of row r, by a whole warp
+__device__ __forceinline__ RowStat row_stat(const VerifyArgs &a, int r) {
+    const RowPart *p = a.stat + (size_t)r * a.parts;
+    double z = 0.0;
+    float top = -INFINITY;
+    int arg = 0x7FFFFFFF;
+    for (int i = threadIdx.x & 31; i < a.parts; i += 32) {
+        z += p[i].z;
+        top = fmaxf(top, p[i].top);
+        arg = min(arg, p[i].arg);
+    }
+    arg = __reduce_min_sync(0xffffffffu, arg);
+    return {warp_max(top), (float)warp_sum_d(z), arg == 0x7FFFFFFF ? 0 : arg};
 }
 
 // ---- layout of a row over a cluster -----------------------------------------------
@@ -212,12 +216,15 @@ template <class T> struct RowPieces {
         run = (pieces + V_C * V_W * 32 - 1) / (V_C * V_W * 32) * 32;
         first = ((int)cluster_rank() * V_W + (threadIdx.x >> 5)) * run + (threadIdx.x & 31);
     }
-    __device__ __forceinline__ int base(int j) const { return (first + 32 * j) * Piece<T>::N - head; }  // element
+    __device__ __forceinline__ int base(int j) const { return place(first + 32 * j); }  // first element of load(j)
     __device__ __forceinline__ int steps() const { return run / 32; }
-    // the j-th piece of this thread; outside the row -inf, which weighs nothing
-    __device__ __forceinline__ Piece<T> load(int j) const {
+    __device__ __forceinline__ int place(int piece) const { return piece * Piece<T>::N - head; }  // its first element
+    // the j-th piece of this thread
+    __device__ __forceinline__ Piece<T> load(int j) const { return at(first + 32 * j); }
+    // a piece of the row; what is outside the row is -inf, which weighs nothing
+    __device__ __forceinline__ Piece<T> at(int piece) const {
         Piece<T> p;
-        const int i = base(j);
+        const int i = place(piece);
         if (i >= 0 && i + Piece<T>::N <= vocab) {
             p.raw = ld_stream_v4(x + i);
         } else {
@@ -230,10 +237,112 @@ template <class T> struct RowPieces {
     }
 };
 
-// One cluster per row: the largest logit, then every CTA's sum of the weights (the
-// parts meet in row_stat, so the cluster meets once, for the maximum). Reading the
-// logits once would take 14 us for 366 rows of 129,281 bf16; what bounds it is
-// issuing about 20 instructions per logit, half of them e^x.
+// Sum of a thread's weights and the first index of the largest logit (greedy), over
+// pieces j = 0 .. n - 1 that get(j) gives and base(j) places.
+template <class T, class G, class P>
+__device__ __forceinline__ void sum_pieces(int n, float top, float inv, bool greedy, G get, P base, double &z, int &arg) {
+    constexpr int N = Piece<T>::N;
+    if (isfinite(top) && isfinite(inv)) {  // then e^0 is 1 without asking
+        const F2 top2 = f2(-top, -top), inv2 = f2(inv, inv);
+        Sum01 s;
+#pragma unroll
+        for (int j = 0; j < n; j++) {
+            const Piece<T> p = get(j);
+#pragma unroll
+            for (int k = 0; k < N; k += 2) {
+                const float2 x = split((f2(p.get(k), p.get(k + 1)) + top2) * inv2);
+                s.add(f2(fmaxf(expf(x.x), 0.0f), fmaxf(expf(x.y), 0.0f)));  // the maximum drops a NaN
+            }
+        }
+        z += s.get();
+    } else {  // nothing above -inf, an infinite logit, a temperature without a finite inverse
+#pragma unroll
+        for (int j = 0; j < n; j++) {
+            const Piece<T> p = get(j);
+#pragma unroll
+            for (int k = 0; k < N; k++) z += weight(p.get(k), top, inv);
+        }
+    }
+    if (greedy && top > -INFINITY) {
+#pragma unroll
+        for (int j = 0; j < n; j++) {
+            const Piece<T> p = get(j);
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (p.get(k) == top) arg = min(arg, base(j) + k);
+        }
+    }
+}
+
+// ---- many logits: two passes -----------------------------------------------------------
+// A CTA takes V_CH pieces of a row for the row's largest logit, then (in a second
+// kernel) the same pieces for the sum: the weights need the largest of the whole row,
+// and reading again, mostly from the L2 cache, costs less than a cluster's meeting for
+// it once rows take turns on the SMs. 366 rows of 129,281 bf16: the whole call 71 us
+// against 90. Bound by about 25 instructions per logit, most of them e^x.
+constexpr int V_CH = 1024, V_CT = 256;
+
+template <class T> __global__ void __launch_bounds__(V_CT) k_verify_max(VerifyArgs a) {
+    __shared__ float s_top[V_CT / 32];
+    pdl_trigger_();
+    const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const RowPieces<T> row(static_cast<const T *>(a.logits) + r * a.logits_stride, a.vocab);
+    Piece<T> p[V_CH / V_CT];
+#pragma unroll
+    for (int j = 0; j < V_CH / V_CT; j++) p[j] = row.at(blockIdx.x * V_CH + j * V_CT + tid);
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < V_CH / V_CT; j++) top = p[j].max(top);
+    top = warp_max(top);
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    if (warp == 0) {
+        top = warp_max(lane < V_CT / 32 ? s_top[lane] : -INFINITY);
+        if (lane == 0) a.stat[(size_t)r * a.parts + blockIdx.x].top = top;
+    }
+}
+
+template <class T> __global__ void __launch_bounds__(V_CT) k_verify_sum(VerifyArgs a) {
+    __shared__ double s_z[V_CT / 32];
+    __shared__ int s_arg[V_CT / 32];
+    pdl_trigger_();
+    const int r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const RowPieces<T> row(static_cast<const T *>(a.logits) + r * a.logits_stride, a.vocab);
+    Piece<T> p[V_CH / V_CT];
+#pragma unroll
+    for (int j = 0; j < V_CH / V_CT; j++) p[j] = row.at(blockIdx.x * V_CH + j * V_CT + tid);
+    const float temp = temp_of(a, seq_of(a, r));
+    pdl_wait_();
+    RowPart *parts = a.stat + (size_t)r * a.parts;
+    float top = -INFINITY;
+    for (int i = lane; i < a.parts; i += 32) top = fmaxf(top, __ldcg(&parts[i].top));
+    top = warp_max(top);
+    double z = 0.0;
+    int arg = 0x7FFFFFFF;
+    sum_pieces<T>(V_CH / V_CT, top, inv_temp(temp), temp <= 0.0f, [&](int j) { return p[j]; },
+                  [&](int j) { return row.place(blockIdx.x * V_CH + j * V_CT + tid); }, z, arg);
+    z = warp_sum_d(z);
+    arg = __reduce_min_sync(0xffffffffu, arg);
+    if (lane == 0) {
+        s_z[warp] = z;
+        s_arg[warp] = arg;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        z = 0.0;
+        for (int w = 0; w < V_CT / 32; w++) {
+            z += s_z[w];
+            arg = min(arg, s_arg[w]);
+        }
+        parts[blockIdx.x].z = z;
+        parts[blockIdx.x].arg = arg;
+    }
+}
+
+// ---- few logits: one launch, a cluster per row --------------------------------------------
+// The largest logit, then every CTA's sum of the weights, from registers (the parts
+// meet in row_stat, so the cluster meets once, for the maximum). Bound by issuing
+// about 25 instructions per logit, most of them e^x, and by that meeting.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, sizeof(T) == 4 ? 2 : 3) k_verify_rows(VerifyArgs a) {
     __shared__ float s_best[V_W], s_cta;
     __shared__ double s_sum[V_W];
@@ -265,45 +374,19 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     top = warp_max(peer_ldf(peer(&s_cta, lane % V_C)));
     cluster_arrive();  // a peer leaves once all have read its shared memory
     double z = 0.0;
-    if (isfinite(top) && isfinite(inv)) {  // then e^0 is 1 without asking
-        const F2 top2 = f2(-top, -top), inv2 = f2(inv, inv);
-        auto add = [&](Sum01 &s, const Piece<T> &p) {
-#pragma unroll
-            for (int k = 0; k < N; k += 2) {
-                const float2 x = split((f2(p.get(k), p.get(k + 1)) + top2) * inv2);
-                s.add(f2(fmaxf(expf(x.x), 0.0f), fmaxf(expf(x.y), 0.0f)));  // the maximum drops a NaN
-            }
-        };
-        Sum01 s;
+    int arg = 0x7FFFFFFF;
+    const bool greedy = temp <= 0.0f;
+    if (steps >= V_NV) {
+        sum_pieces<T>(V_NV, top, inv, greedy, [&](int j) { return keep[j]; }, [&](int j) { return row.base(j); }, z, arg);
+    } else {
 #pragma unroll
         for (int j = 0; j < V_NV; j++)
-            if (j < steps) add(s, keep[j]);
-        z = s.get();
-        for (int j = V_NV; j < steps; j++) {
-            Sum01 rest;
-            add(rest, row.load(j));
-            z += rest.get();
-        }
-    } else {  // nothing above -inf, an infinite logit, a temperature without a finite inverse
-        for (int j = 0; j < steps; j++) {
-            const Piece<T> p = row.load(j);
-#pragma unroll
-            for (int k = 0; k < N; k++) z += weight(p.get(k), top, inv);
-        }
+            if (j < steps)
+                sum_pieces<T>(1, top, inv, greedy, [&](int) { return keep[j]; }, [&](int) { return row.base(j); }, z, arg);
     }
-    if (temp <= 0.0f && top > -INFINITY) {  // greedy: the first index of the largest
-        int arg = 0x7FFFFFFF;
-        auto find = [&](const Piece<T> &p, int j) {
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                if (p.get(k) == top) arg = min(arg, row.base(j) + k);
-        };
-#pragma unroll
-        for (int j = 0; j < V_NV; j++)
-            if (j < steps) find(keep[j], j);
-        for (int j = V_NV; j < steps; j++) find(row.load(j), j);
-        if (arg != 0x7FFFFFFF) atomicMin(&s_arg, arg);
-    }
+    for (int j = V_NV; j < steps; j++)
+        sum_pieces<T>(1, top, inv, greedy, [&](int) { return row.load(j); }, [&](int) { return row.base(j); }, z, arg);
+    if (arg != 0x7FFFFFFF) atomicMin(&s_arg, arg);
     z = warp_sum_d(z);
     if (lane == 0) s_sum[warp] = z;
     __syncthreads();
@@ -311,10 +394,7 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         z = 0.0;
 #pragma unroll
         for (int w = 0; w < V_W; w++) z += s_sum[w];
-        RowParts &o = a.stat[r];
-        o.z[cluster_rank()] = z;
-        o.arg[cluster_rank()] = s_arg;
-        if (cluster_rank() == 0) o.top = top;
+        a.stat[r * V_C + cluster_rank()] = RowPart{z, top, s_arg};
     }
     cluster_wait();
 }
@@ -325,7 +405,8 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
 // and finds the index. Bound by the chain of such meetings and by reading the row.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_pick(VerifyArgs a) {
     __shared__ double s_sum[V_W], s_all[V_C * V_W];
-    __shared__ int s_stop;
+    __shared__ RowStat s_stat[V_W];
+    __shared__ bool s_no[V_W];
     constexpr int N = Piece<T>::N;
     const int b = blockIdx.x / V_C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cluster_rank();
@@ -343,43 +424,47 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         const float l = to_f32(row_at(r)[tok]);
         return fsub(l == s.top ? 0.0f : fmul(fsub(l, s.top), inv), logf(s.z));
     };
-    // the first refusal: one draft per lane of the first warp
-    if (warp == 0) {
-        int stop = r1 - 1;
-        for (int j = r0; j < r1 - 1; j += 32) {
-            const int r = j + lane;
-            bool no = false;
-            if (r < r1 - 1) {
-                const int d = a.tokens[r + 1];
-                const RowStat s = row_stat(a.stat + r);
-                if (d < 0 || d >= a.vocab)
-                    no = true;
-                else if (greedy)
-                    no = d != s.arg;
-                else
-                    no = !(fmul(a.u[r], a.probs ? a.probs[r * a.probs_stride + d] : 1.0f) <
-                           __fdiv_rn(weight(to_f32(row_at(r)[d]), s.top, inv), s.z));
-                if (rank == 0 && !no) {  // rows after a refusal are written again below
-                    a.out[r] = d;
-                    a.logprobs[r] = logp(s, r, d);
+    // the first refusal: one row per warp, sixteen at a time
+    RowStat s{};
+    int stop = r1 - 1;
+    for (int j0 = r0; j0 < r1; j0 += V_W) {
+        const int r = j0 + warp;
+        if (r < r1) {
+            const RowStat mine = row_stat(a, r);
+            if (lane == 0) {
+                bool no = true;  // the last row ends the search too
+                if (r < r1 - 1) {
+                    const int d = a.tokens[r + 1];
+                    if (d >= 0 && d < a.vocab) {
+                        if (greedy)
+                            no = d != mine.arg;
+                        else
+                            no = !(fmul(a.u[r], a.probs ? a.probs[r * a.probs_stride + d] : 1.0f) <
+                                   __fdiv_rn(weight(to_f32(row_at(r)[d]), mine.top, inv), mine.z));
+                        if (rank == 0 && !no) {  // rows after a refusal are written again below
+                            a.out[r] = d;
+                            a.logprobs[r] = logp(mine, r, d);
+                        }
+                    }
                 }
-            }
-            const uint32_t m = __ballot_sync(0xffffffffu, no);
-            if (m) {
-                stop = j + __ffs(m) - 1;
-                break;
+                s_stat[warp] = mine;
+                s_no[warp] = no;
             }
         }
-        if (lane == 0) s_stop = stop;
+        __syncthreads();
+        const uint32_t m = __ballot_sync(0xffffffffu, lane < V_W && j0 + lane < r1 && s_no[lane % V_W]);
+        if (m) {
+            stop = j0 + __ffs(m) - 1;
+            s = s_stat[__ffs(m) - 1];
+            break;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    const int stop = s_stop;
     if (rank == 0)
         for (int r = stop + 1 + tid; r < r1; r += V_T) {
             a.out[r] = -1;
             a.logprobs[r] = 0.0f;
         }
-    const RowStat s = row_stat(a.stat + stop);
     auto emit = [&](int tok) {
         a.out[stop] = tok;
         a.logprobs[stop] = logp(s, stop, tok);
@@ -536,12 +621,34 @@ const char *check(const loom_verify_desc *d) {
     return nullptr;
 }
 
-size_t ws_bytes_of(const loom_verify_desc *d) { return d->n_rows * sizeof(RowParts); }
+// Two passes for more than 5 MB of logits. On the device they are the faster way from
+// the start (f32 rows of 32,000: 32 rows 11.4 us against 13.1, 128 rows 16 against 30;
+// rows of 151,936 alike up to 78 MB, and slower by a tenth at 156 MB, which the L2
+// cache does not hold), but their third launch costs the host 2.4 us, which up to
+// about 4 MB is more than they save.
+bool two_passes(const loom_verify_desc *d) {
+    return d->n_rows * d->vocab * elem_bytes(d->type) > ((size_t)5 << 20) && d->n_rows <= 65535;
+}
+// CTAs to a row: those of its cluster, or of the two passes
+int parts_of(const loom_verify_desc *d) {
+    if (!two_passes(d)) return V_C;
+    const size_t piece = 16 / elem_bytes(d->type), per = V_CH * piece;
+    return (int)((d->vocab + piece - 1 + per - 1) / per);  // a row may start inside a piece
+}
+size_t ws_bytes_of(const loom_verify_desc *d) { return d->n_rows * (size_t)parts_of(d) * sizeof(RowPart); }
 
-template <class T> cudaError_t launch(const VerifyArgs &a, cudaStream_t st) {
-    k_verify_rows<T><<<(unsigned)a.n_rows * V_C, V_T, 0, st>>>(a);
-    count_launch();
-    const cudaError_t e = cudaGetLastError();
+template <class T> cudaError_t launch(const VerifyArgs &a, bool two, cudaStream_t st) {
+    cudaError_t e;
+    if (two) {
+        const dim3 grid(a.parts, a.n_rows);
+        k_verify_max<T><<<grid, V_CT, 0, st>>>(a);
+        count_launch();
+        if ((e = cudaGetLastError()) == cudaSuccess) e = launch_pdl_(k_verify_sum<T>, grid, dim3(V_CT), 0, st, a);
+    } else {
+        k_verify_rows<T><<<(unsigned)a.n_rows * V_C, V_T, 0, st>>>(a);
+        count_launch();
+        e = cudaGetLastError();
+    }
     return e == cudaSuccess ? launch_pdl_(k_verify_pick<T>, dim3((unsigned)a.n_seqs * V_C), dim3(V_T), 0, st, a) : e;
 }
 
@@ -575,17 +682,18 @@ int loom_cuda_verify(const loom_verify_desc *d, const void *d_logits, const floa
     a.out = d_out;
     a.n_out = d_n_out;
     a.logprobs = d_logprobs;
-    a.stat = static_cast<RowParts *>(d_ws);
+    a.stat = static_cast<RowPart *>(d_ws);
     a.logits_stride = (int64_t)d->logits_stride;
     a.probs_stride = (int64_t)d->probs_stride;
     a.n_seqs = (int)d->n_seqs;
     a.n_rows = (int)d->n_rows;
     a.vocab = (int)d->vocab;
+    a.parts = parts_of(d);
     if (!a.n_rows) {  // every sequence is empty
         const cudaError_t e = cudaMemsetAsync(d_n_out, 0, d->n_seqs * sizeof(int32_t), rt_stream(stream));
         return e == cudaSuccess ? LOOM_CUDA_OK : rt_fail("verify", e);
     }
-    const cudaError_t e = by_type(d->type, [&](auto t) { return launch<decltype(t)>(a, rt_stream(stream)); });
+    const cudaError_t e = by_type(d->type, [&](auto t) { return launch<decltype(t)>(a, two_passes(d), rt_stream(stream)); });
     return e == cudaSuccess ? LOOM_CUDA_OK : rt_fail("verify", e);
 }
 
