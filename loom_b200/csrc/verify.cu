@@ -46,7 +46,7 @@ struct VerifyArgs {
     float *logprobs;
     RowPart *stat;  // [rows][parts]
     int64_t logits_stride, probs_stride;
-    int n_seqs, n_rows, vocab, parts;
+    int n_seqs, n_rows, vocab, parts, two;  // two: the parts are of the two passes
 };
 
 __device__ __forceinline__ float temp_of(const VerifyArgs &a, int b) { return a.temp ? a.temp[b] : 1.0f; }
@@ -400,9 +400,9 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
 }
 
 // One cluster per sequence: the accepted drafts, then one token. The sums of the
-// weights over the runs of all the cluster's warps say in whose run the chosen index
-// lies, that warp's sums over its steps in which of them; it weighs that step again
-// and finds the index. Bound by the chain of such meetings and by reading the row.
+// weights over the runs of all the warps say in whose run the chosen index lies, that
+// warp's sums over its steps in which of them; it weighs that step again and finds the
+// index. Bound by the chain of such meetings and by reading the row.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, 2) k_verify_pick(VerifyArgs a) {
     __shared__ double s_sum[V_W], s_all[V_C * V_W];
     __shared__ RowStat s_stat[V_W];
@@ -478,7 +478,6 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
     const RowPieces<T> row(row_at(stop), a.vocab);
     const float *q = !full && a.probs ? a.probs + stop * a.probs_stride : nullptr;
     const int d = full ? -1 : a.tokens[stop + 1];
-    const int steps = row.steps(), span = (steps + 31) / 32;
     // The weights of the N elements from i on: max(p - q, 0), or without probabilities
     // those of every token but the draft; after the last draft, and when that rest is
     // empty, the target's own.
@@ -510,10 +509,16 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
             for (int k = 0; k < N; k++) w[k] = fmaxf(fsub(__fdiv_rn(w[k], s.z), v[k]), 0.0f);  // of a NaN, 0
         }
     };
-    double slot = 0.0;               // sum of this warp's steps span lane .. span (lane + 1) - 1
-    double upto = 0.0, total = 0.0;  // of the sums of warps 4 lane .. 4 lane + 3, and of all
     constexpr int BATCH = sizeof(T) == 4 ? 4 : 2;
-    for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
+    // The cluster goes through the whole row only for max(p - q, 0). Other weights have
+    // been summed over the row's parts already (the draft's part again, without it), so
+    // one CTA finds the part, and its warps take that.
+    const bool whole = q != nullptr;
+    if (!whole && rank != 0) return;
+    const int per = a.two ? V_CH : V_W * row.run;  // pieces of a part
+    int first = row.first, run = row.run, me = (int)rank * V_W + warp;
+    double origin = 0.0, want = 0.0;  // sum before the pieces that are gone through, threshold
+    auto sum_of = [&](int from, int steps, double &slot, int span) {  // of this warp's steps; a slot of them per lane
         double mine = 0.0;
         slot = 0.0;
         for (int j0 = 0; j0 < steps; j0 += BATCH) {
@@ -521,14 +526,14 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
             float v[BATCH][N];
 #pragma unroll
             for (int j = 0; j < BATCH; j++) {  // past the run: past the row, or unused
-                p[j] = row.load(j0 + j);
-                load_q(v[j], row.base(j0 + j));
+                p[j] = row.at(from + 32 * (j0 + j));
+                load_q(v[j], row.place(from + 32 * (j0 + j)));
             }
 #pragma unroll
             for (int j = 0; j < BATCH; j++) {
                 if (j0 + j >= steps) break;
                 float w[N];
-                weigh(w, p[j], v[j], row.base(j0 + j));
+                weigh(w, p[j], v[j], row.place(from + 32 * (j0 + j)));
                 Sum01 sum;
 #pragma unroll
                 for (int k = 0; k < N; k += 2) sum.add(f2(w[k], w[k + 1]));
@@ -537,23 +542,81 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
                 if ((j0 + j) / span == lane) slot += all;
             }
         }
+        return mine;
+    };
+    if (!whole) {
+        const RowPart *parts = a.stat + (size_t)stop * a.parts;
+        run = per / V_W;
+        int drafts = -1;  // the draft's part
+        double dz = 0.0, unused;
+        if (rest && d >= 0 && d < a.vocab) {
+            drafts = (d + row.head) / N / per;
+            const double mine = sum_of(drafts * per + warp * run + lane, run / 32, unused, 1);
+            if (lane == 0) s_sum[warp] = mine;
+            __syncthreads();
+            for (int k = 0; k < V_W; k++) dz += s_sum[k];
+            __syncthreads();
+        }
+        auto z_of = [&](int i) { return i >= a.parts ? 0.0 : i == drafts ? dz : parts[i].z; };
+        double total = 0.0;
+        for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
+            total = 0.0;
+            for (int i = 0; i < a.parts; i += 32) total += __shfl_sync(0xffffffffu, running(z_of(i + lane)), 31);
+            if (total > 0.0 || !rest) break;
+            rest = false;
+            drafts = -1;
+        }
+        want = (double)a.u[r1 - 1] * total;
+        // the first part whose end exceeds the threshold; the last with weight, should none
+        int part = -1;
+        double at = 0.0;
+        for (int i = 0; i < a.parts; i += 32) {
+            const double z = z_of(i + lane), end = at + running(z);
+            const uint32_t over = __ballot_sync(0xffffffffu, z > 0.0 && end > want), some = __ballot_sync(0xffffffffu, z > 0.0);
+            if (over || some) {
+                const int l = over ? __ffs(over) - 1 : 31 - __clz(some);
+                part = i + l;
+                origin = __shfl_sync(0xffffffffu, end - z, l);
+            }
+            if (over) break;
+            at = __shfl_sync(0xffffffffu, end, 31);
+        }
+        if (part < 0) {  // no weight at all
+            if (tid == 0) emit(0);
+            return;
+        }
+        first = part * per + warp * run + lane;
+        me = warp;
+    }
+    const int steps = run / 32, span = (steps + 31) / 32;
+    double slot = 0.0;  // sum of this warp's steps span lane .. span (lane + 1) - 1
+    double upto = 0.0;  // of the sums of warps 4 lane .. 4 lane + 3
+    for (int pass = 0; pass < 2; pass++) {  // the second when the rest is empty
+        const double mine = sum_of(first, steps, slot, span);
         if (lane == 0) s_sum[warp] = mine;
-        cluster_sync();
-        if (tid < V_C * V_W) s_all[tid] = peer_ldd(peer(&s_sum[tid % V_W], tid / V_W));
-        cluster_sync();
+        if (whole) {
+            cluster_sync();
+            if (tid < V_C * V_W) s_all[tid] = peer_ldd(peer(&s_sum[tid % V_W], tid / V_W));
+            cluster_sync();
+        } else {
+            __syncthreads();
+            if (tid < V_C * V_W) s_all[tid] = tid < V_W ? s_sum[tid] : 0.0;
+            __syncthreads();
+        }
         double four = 0.0;
 #pragma unroll
         for (int k = 0; k < 4; k++) four += s_all[4 * lane + k];
         upto = running(four);
-        total = __shfl_sync(0xffffffffu, upto, 31);
+        if (!whole) break;
+        const double total = __shfl_sync(0xffffffffu, upto, 31);
+        want = (double)a.u[r1 - 1] * total;
         if (total > 0.0 || !rest) break;
         rest = false;
     }
     // the run with the chosen index: the first whose end exceeds the threshold; the
     // last one with weight, should none (a random number of 1)
-    const double want = (double)a.u[r1 - 1] * total;
     double c = __shfl_up_sync(0xffffffffu, upto, 1), before = 0.0;
-    if (lane == 0) c = 0.0;
+    c = lane == 0 ? origin : origin + c;
     int pick = -1, heavy = -1;
     double start = 0.0;
 #pragma unroll
@@ -572,45 +635,46 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
         before = __shfl_sync(0xffffffffu, start, __ffs(m) - 1);
     } else {
         pick = __reduce_max_sync(0xffffffffu, heavy);
-        before = total;
+        before = want;
     }
     if (pick < 0) {  // no weight at all
         if (tid == 0 && rank == 0) emit(0);
         return;
     }
-    if (pick != (int)rank * V_W + warp) return;
+    if (pick != me) return;
     // the same among the run's slots of steps, then step by step within the slot
     const double ends = before + running(slot);
     m = __ballot_sync(0xffffffffu, slot > 0.0 && ends > want);
     const uint32_t some = __ballot_sync(0xffffffffu, slot > 0.0);
     const int at = m ? __ffs(m) - 1 : 31 - __clz(some);
     before = __shfl_sync(0xffffffffu, ends - slot, at);
-    int first = -1, last = -1;
-    for (int j = at * span; j < min((at + 1) * span, steps) && first < 0; j++) {
-        const Piece<T> p = row.load(j);
+    int found = -1, last = -1;
+    for (int j = at * span; j < min((at + 1) * span, steps) && found < 0; j++) {
+        const int i = row.place(first + 32 * j);
+        const Piece<T> p = row.at(first + 32 * j);
         float v[N], e[N];
-        load_q(v, row.base(j));
-        weigh(e, p, v, row.base(j));
+        load_q(v, i);
+        weigh(e, p, v, i);
         double sum = 0.0;
 #pragma unroll
         for (int k = 0; k < N; k++) sum += e[k];
-        const double run = running(sum);
-        double here = before + (run - sum);
-        before += __shfl_sync(0xffffffffu, run, 31);
+        const double ends_at = running(sum);
+        double here = before + (ends_at - sum);
+        before += __shfl_sync(0xffffffffu, ends_at, 31);
         int mine = 0x7FFFFFFF;
 #pragma unroll
         for (int k = 0; k < N; k++) {
             here += e[k];
             if (e[k] > 0.0f) {
-                last = max(last, row.base(j) + k);
-                if (here > want) mine = min(mine, row.base(j) + k);
+                last = max(last, i + k);
+                if (here > want) mine = min(mine, i + k);
             }
         }
         mine = __reduce_min_sync(0xffffffffu, mine);
-        if (mine != 0x7FFFFFFF) first = mine;
+        if (mine != 0x7FFFFFFF) found = mine;
     }
     last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) emit(first >= 0 ? first : max(last, 0));
+    if (lane == 0) emit(found >= 0 ? found : max(last, 0));
 }
 
 const char *check(const loom_verify_desc *d) {
@@ -689,6 +753,7 @@ int loom_cuda_verify(const loom_verify_desc *d, const void *d_logits, const floa
     a.n_rows = (int)d->n_rows;
     a.vocab = (int)d->vocab;
     a.parts = parts_of(d);
+    a.two = two_passes(d);
     if (!a.n_rows) {  // every sequence is empty
         const cudaError_t e = cudaMemsetAsync(d_n_out, 0, d->n_seqs * sizeof(int32_t), rt_stream(stream));
         return e == cudaSuccess ? LOOM_CUDA_OK : rt_fail("verify", e);

@@ -477,6 +477,15 @@ def test_verify_matches_64_bits(sv, ty, probs, vocab):
         assert len(set(cnt.tolist())) > 1
 
 
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [[2, 1], [3] * 12], ids=["few", "many"])
+def test_verify_beyond_the_registers_of_a_cluster(sv, ty, rows):
+    """A vocabulary longer than a cluster keeps, in one launch and in two passes, with and without probabilities."""
+    for probs in (True, False):
+        check_verify(sv, verify_inputs(ty, rows, 400001, [[0.9, 0.0, 1.0][b % 3] for b in range(len(rows))], probs, seed=3,
+                                       std=3.0), rows)
+
+
 def test_verify_many_sequences(sv):
     rows = [1 + (b * 7) % 4 for b in range(300)]
     i = verify_inputs(F32, rows, 513, [[1.0, 0.7, 0.0][b % 3] for b in range(300)], True, seed=1)
