@@ -149,7 +149,7 @@ template <class T> constexpr size_t mma_block() { return mma_tp<T>() * 128; }  /
 template <class T, int HDP> constexpr size_t mma_tile() { return HDP * sizeof(T) / 128 * mma_block<T>(); }
 constexpr size_t maxz(size_t a, size_t b) { return a > b ? a : b; }
 template <class T, int HDP> constexpr size_t mma_smem() {  // stages (or the warps' sums), then f32 queries
-    return maxz(4 * mma_tile<T, HDP>(), (size_t)64 * HDP * 4) + (sizeof(T) == 4 ? (size_t)64 * (HDP + 4) * 4 : 0);
+    return maxz(4 * mma_tile<T, HDP>(), (size_t)64 * (HDP + 8) * 4) + (sizeof(T) == 4 ? (size_t)64 * (HDP + 4) * 4 : 0);
 }
 
 template <class T, int HDP>
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
         return;
     }
     const uint32_t sm0 = smem_u32(smb);
-    float *sq = reinterpret_cast<float *>(smb + maxz(4 * TILE, (size_t)64 * HDP * 4));
+    float *sq = reinterpret_cast<float *>(smb + maxz(4 * TILE, (size_t)64 * (HDP + 8) * 4));
     constexpr int QST = HDP + 4;
     const int blocks = (hd + E - 1) / E, wide = F ? blocks * E : (hd + 15) / 16 * 16;
     const int tiles = (it.p1 - it.p0 + TP - 1) / TP, left = it.p1 - it.p0 - (tiles - 1) * TP;
@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
             s_l[warp][g + 8] = l1;
         }
         __syncthreads();  // the tiles are read: the sums of the warps take their place
-        float *so = reinterpret_cast<float *>(smb) + warp * 16 * HDP;
+        constexpr int SST = HDP + 8;  // rows g and pairs t of a store touch every bank once
+        float *sums = reinterpret_cast<float *>(smb);
         {
             float t0 = -INFINITY, t1 = -INFINITY;
             for (int w = rt * nps; w < (rt + 1) * nps; w++) {
@@ -503,24 +504,48 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
                 t1 = fmaxf(t1, s_m[w][g + 8]);
             }
             const float f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - t0), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - t1);
+            float *so = sums + (warp * 16 + g) * SST + 2 * t;
 #pragma unroll
             for (int i = 0; i < HDP / 8; i++) {
-                *reinterpret_cast<float2 *>(so + g * HDP + i * 8 + 2 * t) = make_float2(o[i][0] * f0, o[i][1] * f0);
-                *reinterpret_cast<float2 *>(so + (g + 8) * HDP + i * 8 + 2 * t) = make_float2(o[i][2] * f1, o[i][3] * f1);
+                *reinterpret_cast<float2 *>(so + i * 8) = make_float2(o[i][0] * f0, o[i][1] * f0);
+                *reinterpret_cast<float2 *>(so + 8 * SST + i * 8) = make_float2(o[i][2] * f1, o[i][3] * f1);
             }
         }
         __syncthreads();
-        for (int j = warp; j < rows; j += 4) {
-            const int w0 = (j / 16) * nps, jr = j % 16;
-            const size_t at = part_at(a, it.slot, rb + j, kvh);
+        if (tid < rows) {
+            const int w0 = (tid / 16) * nps, jr = tid % 16;
             float top = -INFINITY, l = 0.0f;
             for (int w = w0; w < w0 + nps; w++) top = fmaxf(top, s_m[w][jr]);
             for (int w = w0; w < w0 + nps; w++) l += s_l[w][jr] * (s_m[w][jr] == -INFINITY ? 0.0f : ex2(s_m[w][jr] - top));
-            if (lane == 0) a.ml[at] = make_float2(top, l);
-            for (int d = lane; d < hd; d += 32) {
-                float v = 0.0f;
-                for (int w = w0; w < w0 + nps; w++) v += reinterpret_cast<float *>(smb)[(w * 16 + jr) * HDP + d];
-                a.acc[at * hd + d] = v;
+            a.ml[part_at(a, it.slot, rb + tid, kvh)] = make_float2(top, l);
+        }
+        // a warp's rows four at a time (one after the other 32 rows took 3 us more)
+        constexpr int RU = 4, NP = (HDP + 63) / 64;
+        for (int j0 = warp; j0 < rows; j0 += 4 * RU) {
+            float2 v[RU][NP];
+#pragma unroll
+            for (int u = 0; u < RU; u++) {
+                const int j = min(j0 + 4 * u, rows - 1);
+                const float *from = sums + ((j / 16) * nps * 16 + j % 16) * SST + 2 * lane;
+#pragma unroll
+                for (int d = 0; d < NP; d++) {
+                    v[u][d] = make_float2(0.0f, 0.0f);
+                    if (d * 64 + 2 * lane < HDP)
+                        for (int w = 0; w < nps; w++) {
+                            const float2 x = *reinterpret_cast<const float2 *>(from + w * 16 * SST + d * 64);
+                            v[u][d].x += x.x;
+                            v[u][d].y += x.y;
+                        }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < RU; u++) {
+                const int j = j0 + 4 * u;
+                if (j >= rows) break;
+                float *dst = a.acc + part_at(a, it.slot, rb + j, kvh) * hd + 2 * lane;
+#pragma unroll
+                for (int d = 0; d < NP; d++)
+                    if (d * 64 + 2 * lane < hd) *reinterpret_cast<float2 *>(dst + d * 64) = v[u][d];  // hd is even
             }
         }
     }
@@ -707,14 +732,26 @@ const char *check(const loom_attn_shared_desc *d) {
 }
 
 // Whether the prefix goes to attn_prefix.cu, as far as the call's sizes say: 16-bit
-// types, dimensions that fit its tiles, and rows enough for them.
+// types, dimensions that fit its tiles, a quarter of a tile's rows and products enough
+// to make up for its longer start. Both kernels, bf16, 8 query heads to each of 4 KV
+// heads of 128, us of a call: 2^27 products (256 rows, prefix 1,024 / 64 rows, 4,096)
+// 15.9 / 13.5 here and 15.5 / 13.0 there, half of them (256 rows, 512) 12.0 and 14.6,
+// four times (128 rows, 8,192) 20.9 and 17.7, 2^32 (256 rows, 32,768) 84 and 42; 8 and
+// 16 rows over 32,768 positions 18.2 and 19.9 here, 21.1 and 21.3 there, 32 rows 24.6
+// and 22.1. Heads of 64 meet at twice the positions.
 bool prefix_tc(const loom_attn_shared_desc *d) {
-    return d->type != T_F32 && d->head_dim <= 128 && d->head_dim % 8 == 0 && d->scale >= 0.0f && d->prefix_len &&
-           d->n_rows * (d->n_heads / d->n_kv_heads) > 64;
+    const double rows = (double)d->n_rows * (d->n_heads / d->n_kv_heads);
+    return d->type != T_F32 && d->head_dim <= 128 && d->head_dim % 8 == 0 && d->scale >= 0.0f && rows >= 32 &&
+           rows * d->n_kv_heads * d->prefix_len * d->head_dim >= (double)(1 << 28);
 }
 
-// The cut of the positions. Chunks are sized so that prefix and own items
-// together give the GPU a few CTAs per SM, no smaller than 64 positions.
+// The cut of the positions, chunks of 64 or more: the prefix in 3 CTAs per SM, the own
+// caches in 4. More parts cost the join more than the SMs gain (1 row of 8 heads, f32,
+// prefix 8,192: 22 us, at 6 CTAs 28; 70 rows, bf16, own caches of 1,024: 38.8 us, at 6
+// 42.5), fewer leave them idle (128 sequences' own caches of 2,048: 167 us of a call, at
+// 3 174). attn_prefix.cu takes one CTA per SM in one round, of one tile of 128 rows
+// where that leaves it few steps (256 rows over 4,096 positions of 4 heads: 20 us, with
+// two tiles 25.5; 1,024 over 8,192 43.6 and 42.6; 512 over 32,768 62.0 and 59.6).
 void plan(const loom_attn_shared_desc *d, AttnArgs &a) {
     a.n_seqs = (int)d->n_seqs;
     a.n_rows = (int)d->n_rows;
@@ -733,21 +770,20 @@ void plan(const loom_attn_shared_desc *d, AttnArgs &a) {
     a.ohead = (int64_t)d->own_head_stride;
     a.oseq = (int64_t)d->own_seq_stride;
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
-    const int want = 6 * 148;  // 3 to 12 per SM measured alike
     const int64_t rows = std::max<int64_t>((int64_t)a.n_rows * a.group, 1);
-    if (prefix_tc(d)) {  // one CTA per SM, one round of them
-        a.pre_tiles = (int)up(rows, 256);
+    if (prefix_tc(d)) {
+        a.pre_tiles = (int)up(rows, rows * a.nkv * a.prefix <= ((int64_t)1 << 24) ? 128 : 256);
         a.pre_rows = (int)up(rows, a.pre_tiles);
         const int64_t per = std::max<int64_t>(1, 148 / ((int64_t)a.pre_tiles * a.nkv));
         a.pre_chunk = (int)(up(up(std::max(a.prefix, 1), per), 128) * 128);
     } else {
         a.pre_rows = 64;
         a.pre_tiles = (int)up(rows, a.pre_rows);
-        const int64_t per = up(want, (int64_t)a.pre_tiles * a.nkv);
+        const int64_t per = up(3 * 148, (int64_t)a.pre_tiles * a.nkv);
         a.pre_chunk = (int)(up(up(std::max(a.prefix, 1), per), 64) * 64);
     }
     a.n_pre = (int)up(a.prefix, a.pre_chunk);
-    const int64_t own_per = std::max<int64_t>(1, up(want, (int64_t)std::max(a.n_seqs, 1) * a.nkv));
+    const int64_t own_per = std::max<int64_t>(1, up(4 * 148, (int64_t)std::max(a.n_seqs, 1) * a.nkv));
     a.own_chunk = (int)std::max<int64_t>(64, up(up(std::max(a.cap, 1), own_per), 64) * 64);
     a.n_own = a.n_seqs ? (int)up(a.cap, a.own_chunk) : 0;
 }
@@ -814,9 +850,11 @@ cudaError_t launch_items(size_t smem, int items, int threads, const AttnArgs &a,
 
 template <class T, int ND> cudaError_t launch_join(const AttnArgs &a, int items, cudaStream_t st) {
     // Four warps share a (row, head) where one would read many parts in turn and the
-    // rows alone leave SMs idle.
+    // rows alone leave SMs idle (bf16 calls of 32 heads, us with one and with four: 1 row
+    // of prefix 32,768 25.8 and 18.1, 16 rows of 4,096 26.3 and 24.0, 32 rows of 8,192
+    // 29.0 and 30.3, 64 rows of 4,096 32.4 and 37.7).
     const int64_t pairs = (int64_t)a.n_rows * a.nh;
-    const bool few = a.n_pre + a.n_own > 16 && pairs < 4 * 4 * 148;
+    const bool few = a.n_pre + a.n_own > 16 && pairs <= 4 * 148;
     const auto on = [&](int64_t elems) { return elems % 4 == 0; };
     const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0; };
     const bool whole = on(a.hd) && on(a.q_stride) && on(a.opos) && on(a.ohead) && on(a.oseq) && at(a.q) && at(a.ok) && at(a.ov);

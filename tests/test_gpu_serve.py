@@ -111,6 +111,34 @@ def test_attn_matches_64_bits(sv, ty, shape):
     assert rel(out, attn_ref(i, rows, lens)) < ATTN_TOL[ty]
 
 
+# rows and prefix enough for the prefix's own kernel (16-bit types): its tiles of 128
+# rows and steps of 64 positions with edges everywhere
+PREFIXES = {
+    "a quarter of a tile": ([1, 3], [0, 5], 32, 4, 128, 16411, 8),
+    "a tile and a row, hd 80": ([40, 2, 1], [60, 2, 9], 24, 8, 80, 3301, 60),
+    "group of one, hd 48": ([100, 0, 200], [120, 0, 200], 8, 8, 48, 2401, 200),
+    "one kv head": ([5] * 10, [9] * 10, 16, 1, 64, 5301, 16),
+    "two tiles of a CTA": ([4] * 33, list(range(33)), 32, 4, 128, 4099, 40),
+    "hd 8": ([3, 5], [0, 2], 64, 1, 8, 65601, 4),
+}
+
+
+@pytest.mark.parametrize("ty", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("shape", PREFIXES, ids=[s.replace(" ", "_") for s in PREFIXES])
+def test_attn_prefix_of_many_rows(sv, ty, shape):
+    rows, lens, heads, kv, hd, prefix, cap = PREFIXES[shape]
+    for qstd in (1.0, 20.0):  # and scores of +-60
+        i = attn_inputs(ty, rows, lens, heads, kv, hd, prefix, cap, seed=len(shape), qstd=qstd)
+        tol = ATTN_TOL[ty] + (10 * ATTN_TOL[F32] if qstd > 1 else 0)
+        want = attn_ref(i, rows, lens)
+        assert rel(attn(sv, i), want) < tol
+        for k in ("pk", "pv"):  # head-major
+            i[k] = i[k].transpose(0, 1).contiguous().transpose(0, 1)
+        assert rel(attn(sv, i), want) < tol
+    i["pv"][prefix - 1, :, 0] = float("nan")  # a value that every row sees
+    assert torch.isnan(attn(sv, i)[..., 0]).all()
+
+
 @pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
 def test_attn_peaked_scores(sv, ty):
     """Scores of +-60: one position has almost all of the weight, exp must not overflow."""
