@@ -219,10 +219,40 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
         }
         uint32_t qf[KS][4];
         if constexpr (F) {
-            for (int j = warp; j < (rows + 15) / 16 * 16; j += 4) {
-                const float *src = reinterpret_cast<const float *>(q_row(min(rb + j, it.r1 - 1)));
-                for (int d = lane; d < wide; d += 32) sq[j * QST + d] = j < rows && d < hd ? src[d] : 0.0f;
+            // All of a thread's pieces in flight at once. Up to 32 rows are split here, once
+            // for every tile: the first terms in their rows, the second 32 rows further.
+            const int lanes = wide / 4, there = (rows + 15) / 16 * 16;
+            for (int j = tid; j < there * lanes; j += 128) {
+                const int r = j / lanes, d = j % lanes * 4;
+                const float *src = reinterpret_cast<const float *>(q_row(min(rb + r, it.r1 - 1))) + d;
+                float *dst = sq + r * QST + d;
+                if (r >= rows || d >= hd) {
+                    *reinterpret_cast<float4 *>(dst) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                } else if (d + 4 <= hd && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                    cp_async16(smem_u32(dst), src, true);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (d + k < hd)
+                            cp_async4(smem_u32(dst + k), src + k);
+                        else
+                            dst[k] = 0.0f;
+                    }
+                }
             }
+            cp_async_wait_all();
+            if (nps > 1)
+                for (int j = tid; j < there * lanes; j += 128) {  // the thread's own pieces
+                    float4 *p = reinterpret_cast<float4 *>(sq + j / lanes * QST + j % lanes * 4);
+                    const float4 x = *p;
+                    uint4 hi, lo;
+                    split_tf32(x.x, hi.x, lo.x);
+                    split_tf32(x.y, hi.y, lo.y);
+                    split_tf32(x.z, hi.z, lo.z);
+                    split_tf32(x.w, hi.w, lo.w);
+                    *reinterpret_cast<uint4 *>(p) = hi;
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<float *>(p) + 32 * QST) = lo;
+                }
             __syncthreads();
         } else {
             // pairs of dimensions; whole words where rows lie on 4 bytes (hd is even)
@@ -267,28 +297,42 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
                     // for each of four products: any order sums to the same scores
                     // (products that add to one result wait for one another: the tiles and the
                     // two small terms take turns)
-                    float small[2][NT][4];
+                    constexpr int NS = NT == 4 ? 1 : 2;  // four tiles are turns enough
+                    float small[NS][NT][4];
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) small[0][n][j] = small[1][n][j] = 0.0f;
+                        for (int j = 0; j < 4; j++) small[0][n][j] = small[NS - 1][n][j] = 0.0f;
                     const float *qa = sq + (rt * 16 + g) * QST + 8 * t, *qb = qa + 8 * QST;
                     const uint8_t *kr = smb + (tk - sm0) + (sub + g) * 128;
-#pragma unroll 2
+#pragma unroll(HDP > 128 ? 1 : 2)  // within 255 registers: local memory costs a launch 6 us of host time
                     for (int d = 0; d < blocks; d++) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
+                            uint32_t ah[2][4], al[2][4], bh[NT][4], bl[NT][4];
                             const float4 ua = *reinterpret_cast<const float4 *>(qa + d * 32 + h * 4);
                             const float4 ub = *reinterpret_cast<const float4 *>(qb + d * 32 + h * 4);
-                            uint32_t ah[2][4], al[2][4], bh[NT][4], bl[NT][4];
-                            split_tf32(ua.x, ah[0][0], al[0][0]);
-                            split_tf32(ub.x, ah[0][1], al[0][1]);
-                            split_tf32(ua.y, ah[0][2], al[0][2]);
-                            split_tf32(ub.y, ah[0][3], al[0][3]);
-                            split_tf32(ua.z, ah[1][0], al[1][0]);
-                            split_tf32(ub.z, ah[1][1], al[1][1]);
-                            split_tf32(ua.w, ah[1][2], al[1][2]);
-                            split_tf32(ub.w, ah[1][3], al[1][3]);
+                            if constexpr (NT == 4) {
+                                split_tf32(ua.x, ah[0][0], al[0][0]);
+                                split_tf32(ub.x, ah[0][1], al[0][1]);
+                                split_tf32(ua.y, ah[0][2], al[0][2]);
+                                split_tf32(ub.y, ah[0][3], al[0][3]);
+                                split_tf32(ua.z, ah[1][0], al[1][0]);
+                                split_tf32(ub.z, ah[1][1], al[1][1]);
+                                split_tf32(ua.w, ah[1][2], al[1][2]);
+                                split_tf32(ub.w, ah[1][3], al[1][3]);
+                            } else {  // split already
+                                const float4 va = *reinterpret_cast<const float4 *>(qa + 32 * QST + d * 32 + h * 4);
+                                const float4 vb = *reinterpret_cast<const float4 *>(qb + 32 * QST + d * 32 + h * 4);
+                                auto four_of = [](uint32_t (&r)[2][4], const float4 &a4, const float4 &b4) {
+                                    r[0][0] = __float_as_uint(a4.x), r[0][1] = __float_as_uint(b4.x);
+                                    r[0][2] = __float_as_uint(a4.y), r[0][3] = __float_as_uint(b4.y);
+                                    r[1][0] = __float_as_uint(a4.z), r[1][1] = __float_as_uint(b4.z);
+                                    r[1][2] = __float_as_uint(a4.w), r[1][3] = __float_as_uint(b4.w);
+                                };
+                                four_of(ah, ua, ub);
+                                four_of(al, va, vb);
+                            }
                             float e[NT][4];
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
@@ -306,7 +350,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
 #pragma unroll
                                 for (int n = 0; n < NT; n++) mma_tf32(small[0][n], al[u], bh[n][2 * u], bh[n][2 * u + 1]);
 #pragma unroll
-                                for (int n = 0; n < NT; n++) mma_tf32(small[1][n], ah[u], bl[n][2 * u], bl[n][2 * u + 1]);
+                                for (int n = 0; n < NT; n++) mma_tf32(small[NS - 1][n], ah[u], bl[n][2 * u], bl[n][2 * u + 1]);
                             }
 #pragma unroll
                             for (int n = 0; n < NT; n++)
@@ -317,7 +361,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) c[n][j] += small[0][n][j] + small[1][n][j];
+                        for (int j = 0; j < 4; j++) c[n][j] += NS == 1 ? small[0][n][j] : small[0][n][j] + small[NS - 1][n][j];
                 } else {
                     // 16-byte piece c of a row is at c ^ (row % 8) of its block
                     const uint32_t row = tk + (sub + (lane >> 4) * 8 + (lane & 7)) * 128, x = ((lane >> 3) & 1) ^ (lane & 7);
