@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
                         for (int j = 0; j < 4; j++) small[0][n][j] = small[NS - 1][n][j] = 0.0f;
                     const float *qa = sq + (rt * 16 + g) * QST + 8 * t, *qb = qa + 8 * QST;
                     const uint8_t *kr = smb + (tk - sm0) + (sub + g) * 128;
-#pragma unroll(HDP > 128 ? 1 : 2)  // within 255 registers: local memory costs a launch 6 us of host time
+#pragma unroll 1  // two at once miss the instruction cache (32 sequences: 65 us, not 61)
                     for (int d = 0; d < blocks; d++) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
@@ -434,35 +434,44 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
                         l1 += c[n][2] + c[n][3];
                     }
                     const uint8_t *v0 = smb + (tv - sm0) + (sub + 2 * t) * 128 + (g & 3) * 4;
+                    constexpr int NP = NT > 2 ? 2 : NT;  // positions of a turn, in eights
+#pragma unroll 1
+                    for (int n0 = 0; n0 < NT; n0 += NP, v0 += NP * 1024) {
 #pragma unroll
-                    for (int i4 = 0; i4 < HDP / 8; i4 += 4) {  // a block of 32 dimensions, zeros past hd
-                        if (i4 * 8 < hd) {
-                            const uint8_t *v = v0 + (i4 >> 2) * BLK;
-                            float e[4][4];
+                        for (int i4 = 0; i4 < HDP / 8; i4 += 4) {  // a block of 32 dimensions, zeros past hd
+                            if (i4 * 8 < hd) {
+                                const uint8_t *v = v0 + (i4 >> 2) * BLK;
+                                float e[4][4];
 #pragma unroll
-                            for (int i = 0; i < 4; i++) e[i][0] = e[i][1] = e[i][2] = e[i][3] = 0.0f;
+                                for (int i = 0; i < 4; i++) e[i][0] = e[i][1] = e[i][2] = e[i][3] = 0.0f;
 #pragma unroll
-                            for (int n = 0; n < NT; n++) {
-                                uint32_t bh[4][2], bl[4][2];
+                                for (int n = 0; n < NP; n++) {
+                                    uint32_t bh[4][2], bl[4][2];
 #pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const int piece = 2 * i + (g >> 2);
-                                    split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + ((piece ^ (2 * t)) << 4)), bh[i][0], bl[i][0]);
-                                    split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + 128 + ((piece ^ (2 * t + 1)) << 4)),
-                                               bh[i][1], bl[i][1]);
+                                    for (int i = 0; i < 4; i++) {
+                                        const int piece = 2 * i + (g >> 2);
+                                        split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + ((piece ^ (2 * t)) << 4)), bh[i][0],
+                                                   bl[i][0]);
+                                        split_tf32(*reinterpret_cast<const float *>(v + n * 1024 + 128 + ((piece ^ (2 * t + 1)) << 4)),
+                                                   bh[i][1], bl[i][1]);
+                                    }
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) mma_tf32(e[i], al[n], bh[i][0], bh[i][1]);
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) mma_tf32(e[i], ah[n], bl[i][0], bl[i][1]);
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) mma_tf32(e[i], ah[n], bh[i][0], bh[i][1]);
                                 }
 #pragma unroll
-                                for (int i = 0; i < 4; i++) mma_tf32(e[i], al[n], bh[i][0], bh[i][1]);
+                                for (int i = 0; i < 4; i++)
 #pragma unroll
-                                for (int i = 0; i < 4; i++) mma_tf32(e[i], ah[n], bl[i][0], bl[i][1]);
-#pragma unroll
-                                for (int i = 0; i < 4; i++) mma_tf32(e[i], ah[n], bh[i][0], bh[i][1]);
+                                    for (int j = 0; j < 4; j++) o[i4 + i][j] += e[i][j];
                             }
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-#pragma unroll
-                                for (int j = 0; j < 4; j++) o[i4 + i][j] += e[i][j];
                         }
+#pragma unroll
+                        for (int n = 0; n + NP < NT; n++)  // the next turn's weights
+#pragma unroll
+                            for (int j = 0; j < 4; j++) ah[n][j] = ah[n + NP][j], al[n][j] = al[n + NP][j];
                     }
                 } else {
                     uint32_t pf[NT / 2][4];

@@ -249,12 +249,31 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
                     read8(ub, x + 8 * (xst / 4));
                     split_rows(ah, al, ua, ub);
                     const uint8_t *ws = st + l_xtile<T>(nk) + g * wst + (kp * 32 + 8 * t) * (int)sizeof(T);
-                    mma_tiles<T, 2>(c, ah, al, ws, wst);
-                    if (cols > 16) mma_tiles<T, 2>(c + 2, ah, al, ws + 16 * wst, wst);
-                    if (cols > 32) mma_tiles<T, 4>(c + 4, ah, al, ws + 32 * wst, wst);
+                    if (cols > 32) {
+                        mma_tiles<T, 4>(c, ah, al, ws, wst);
+                        mma_tiles<T, 4>(c + 4, ah, al, ws + 32 * wst, wst);
+                    } else if (cols > 16) {
+                        mma_tiles<T, 4>(c, ah, al, ws, wst);
+                    } else {
+                        mma_tiles<T, 2>(c, ah, al, ws, wst);
+                    }
                 }
             }
             cp_async_wait<0>();
+            if (nk == 1) {  // a warp has its rows' whole sums
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int m = mt * 16 + g + 8 * h;
+                    if (m >= gr.rows) continue;
+                    float *p = part + (size_t)s_rows[m] * a.max_rank + k0 + 2 * t;
+#pragma unroll
+                    for (int n = 0; n < L_NB; n++) {
+                        if (n * 8 + 2 * t < cols) p[n * 8] = c[n][2 * h];
+                        if (n * 8 + 2 * t + 1 < cols) p[n * 8 + 1] = c[n][2 * h + 1];
+                    }
+                }
+                continue;
+            }
             __syncthreads();
             float(*s_t)[16][L_NB * 8 + 1] = reinterpret_cast<float(*)[16][L_NB * 8 + 1]>(smem);
 #pragma unroll

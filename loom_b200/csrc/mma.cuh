@@ -32,13 +32,13 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo with hi, lo of 11 significant bits each (tf32): x is kept to
-// 2^-22, so hi*hi' + hi*lo' + lo*hi' stands for an f32 product (what is left
-// out, lo*lo', is below 2^-24 of it).
+// x = hi + lo with hi, lo of 11 significant bits each (tf32): hi to nearest, the rest,
+// which has either sign, cut off, so x is kept to 2^-21 and hi*hi' + hi*lo' + lo*hi'
+// stands for an f32 product (lo*lo', left out, is below 2^-22 of it). Integer
+// operations: the conversion instruction made 53 us of an attention call 61.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float rest = x - __uint_as_float(hi);
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {

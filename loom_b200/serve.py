@@ -12,6 +12,7 @@ in a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import Optional, Sequence
 
 import torch
@@ -60,6 +61,7 @@ def _laid(t, strides) -> bool:
 
 _stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(dev).cuda_stream gives, 1.2 us sooner
 _capturing = torch.cuda.is_current_stream_capturing
+_alone = threading.Lock()
 _kept = {}          # (device, stream) -> scratch of calls on that stream, in their order
 _KEEP = 32 << 20    # bytes of it; calls that need more take theirs from torch's allocator
 
@@ -71,11 +73,12 @@ def _run(op: str, entry, size, desc, args, dev: int, stream: Optional[int]) -> N
     cur = _stream(dev)
     st = cur if stream is None else stream
     if st == cur and not _capturing():
-        ws = _kept.get((dev, cur))
-        if ws is None:
-            ws = _kept[dev, cur] = torch.empty(_KEEP, dtype=torch.uint8, device=dev)
-        if entry(desc, *args, ws.data_ptr(), _KEEP, cur) == _lib.OK:
-            return
+        with _alone:  # launches of two threads on one stream may not mix while they share the buffer
+            ws = _kept.get((dev, cur))
+            if ws is None:
+                ws = _kept[dev, cur] = torch.empty(_KEEP, dtype=torch.uint8, device=dev)
+            if entry(desc, *args, ws.data_ptr(), _KEEP, cur) == _lib.OK:
+                return
     need = size(desc)  # larger, captured, on a stream of the caller's, or refused: then for the reason it names
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     if st != cur and need:
