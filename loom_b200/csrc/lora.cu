@@ -35,9 +35,9 @@ struct LoraArgs {
     const float *x, *scales, *base;
     const void *a, *b;
     const int32_t *ranks, *ids;
-    float *out, *t;  // t: parts [slice][row][max_rank]
+    float *out, *t;  // t: parts [slice][row][t_row]
     int64_t x_stride, base_stride, out_stride, a_row, a_adapter, b_row, b_adapter;
-    int n_rows, n_in, n_out, n_adapters, max_rank;
+    int n_rows, n_in, n_out, n_adapters, max_rank, t_row;  // t_row: max_rank, up to a multiple of 4
     int slice, n_slices;
     int wide_x, wide_a, wide_b, wide_out;  // 16-byte (out: 8-byte) accesses are aligned
 };
@@ -194,7 +194,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
     pdl_trigger_();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int i0 = blockIdx.z * a.slice, i1 = min(i0 + a.slice, a.n_in);
-    float *part = a.t + (size_t)blockIdx.z * a.n_rows * a.max_rank;
+    float *part = a.t + (size_t)blockIdx.z * a.n_rows * a.t_row;
     for (int j = blockIdx.y;; j += gridDim.y) {
         __syncthreads();  // the rows of the group before have been read
         const Group gr = group_of(a, blockIdx.x * L_RB, j, s_rows);
@@ -265,7 +265,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
                 for (int h = 0; h < 2; h++) {
                     const int m = mt * 16 + g + 8 * h;
                     if (m >= gr.rows) continue;
-                    float *p = part + (size_t)s_rows[m] * a.max_rank + k0 + 2 * t;
+                    float *p = part + (size_t)s_rows[m] * a.t_row + k0 + 2 * t;
 #pragma unroll
                     for (int n = 0; n < L_NB; n++) {
                         if (n * 8 + 2 * t < cols) p[n * 8] = c[n][2 * h];
@@ -288,7 +288,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
                 for (int k = lane; k < cols; k += 32) {
                     float s = 0.0f;
                     for (int q = 0; q < nk; q++) s += s_t[(m / 16) * nk + q][m % 16][k];
-                    part[(size_t)s_rows[m] * a.max_rank + k0 + k] = s;
+                    part[(size_t)s_rows[m] * a.t_row + k0 + k] = s;
                 }
         }
     }
@@ -348,6 +348,13 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs
                     c[n][2 * h + 1] = b.y;
                 }
             }
+            auto clear = [&](int deep, int d4) {  // what the tile has beside the sums
+                for (int j = tid; j < (gr.rows + 15) / 16 * 16 * (deep / 4); j += 128) {
+                    const int m = j / (deep / 4), q = j % (deep / 4);
+                    if (m >= gr.rows || q >= d4) *reinterpret_cast<float4 *>(s_x + m * TST + q * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            };
+            if (rank) clear(min((rank + 31) / 32 * 32, L_DEEP), (min(rank, L_DEEP) + 3) / 4);
             pdl_wait_();  // t is there
             for (int k = 0; k < rank; k += L_DEEP) {
                 const int deep = min((rank - k + 31) / 32 * 32, L_DEEP);
@@ -355,33 +362,21 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs
                     __syncthreads();
                     weights(k);
                 }
-                const size_t next = (size_t)a.n_rows * a.max_rank;  // from part to part
-                if (a.max_rank % 4 == 0) {  // 16 ranks a row's quarter warp, four at a time
-                    for (int m = tid >> 4; m < (gr.rows + 15) / 16 * 16; m += 8) {
-                        const int q = (tid & 15) * 4;
-                        if (q >= deep) continue;
-                        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (m < gr.rows && k + q < rank) {
-                            const float *p = a.t + (size_t)s_rows[m] * a.max_rank + k + q;
+                // the parts' sums, four ranks of a row to a thread
+                const size_t next = (size_t)a.n_rows * a.t_row;  // from part to part
+                const int d4 = (min(rank - k, deep) + 3) / 4;
+                if (k) clear(deep, d4);
+                for (int j = tid; j < gr.rows * d4; j += 128) {
+                    const int m = j / d4, q = j % d4 * 4, left = rank - k - q;  // what lies past the rank was not written
+                    const float *p = a.t + (size_t)s_rows[m] * a.t_row + k + q;
+                    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-                            for (int z = 0; z < a.n_slices; z++) {
-                                const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + z * next));
-                                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-                            }
-                        }
-                        const int left = rank - k - q;  // what lies past the rank was not written
-                        *reinterpret_cast<float4 *>(s_x + m * TST + q) =
-                            make_float4(left > 0 ? s.x * scale : 0.0f, left > 1 ? s.y * scale : 0.0f, left > 2 ? s.z * scale : 0.0f,
-                                        left > 3 ? s.w * scale : 0.0f);
+                    for (int z = 0; z < a.n_slices; z++) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + z * next));
+                        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
                     }
-                } else {
-                    for (int m = warp; m < (gr.rows + 15) / 16 * 16; m += 4)
-                        for (int q = lane; q < deep; q += 32) {
-                            float s = 0.0f;
-                            if (m < gr.rows && k + q < rank)
-                                for (int z = 0; z < a.n_slices; z++) s += __ldcg(a.t + z * next + (size_t)s_rows[m] * a.max_rank + k + q);
-                            s_x[m * TST + q] = s * scale;
-                        }
+                    *reinterpret_cast<float4 *>(s_x + m * TST + q) = make_float4(
+                        s.x * scale, left > 1 ? s.y * scale : 0.0f, left > 2 ? s.z * scale : 0.0f, left > 3 ? s.w * scale : 0.0f);
                 }
                 cp_async_wait<0>();
                 __syncthreads();
@@ -440,7 +435,8 @@ int slice_of(const loom_lora_desc *d) {
     return (int)std::max<size_t>(128, ((d->n_in + want - 1) / want + 127) / 128 * 128);
 }
 size_t slices_of(const loom_lora_desc *d) { return (d->n_in + slice_of(d) - 1) / slice_of(d); }
-size_t ws_bytes_of(const loom_lora_desc *d) { return slices_of(d) * d->n_rows * d->max_rank * sizeof(float); }
+size_t t_row_of(const loom_lora_desc *d) { return (d->max_rank + 3) / 4 * 4; }
+size_t ws_bytes_of(const loom_lora_desc *d) { return slices_of(d) * d->n_rows * t_row_of(d) * sizeof(float); }
 
 template <class T> cudaError_t launch(const LoraArgs &a, cudaStream_t st) {
     const unsigned blocks = (a.n_rows + L_RB - 1) / L_RB, most = std::min(std::min(L_RB, a.n_rows), a.n_adapters + 1);
@@ -507,6 +503,7 @@ int loom_cuda_lora(const loom_lora_desc *d, const float *d_x, const void *d_a, c
     a.n_out = (int)d->n_out;
     a.n_adapters = (int)(d->max_rank ? d->n_adapters : 0);
     a.max_rank = (int)d->max_rank;
+    a.t_row = (int)t_row_of(d);
     a.slice = slice_of(d);
     a.n_slices = (int)slices_of(d);
     const size_t size = elem_bytes(d->type);
