@@ -339,7 +339,7 @@ template <class T> __global__ void __launch_bounds__(V_CT) k_verify_sum(VerifyAr
     }
 }
 
-// ---- few logits: one launch, a cluster per row --------------------------------------------
+// ---- few rows: one launch, a cluster per row --------------------------------------------
 // The largest logit, then every CTA's sum of the weights, from registers (the parts
 // meet in row_stat, so the cluster meets once, for the maximum). Bound by issuing
 // about 25 instructions per logit, most of them e^x, and by that meeting.
@@ -687,13 +687,15 @@ const char *check(const loom_verify_desc *d) {
     return nullptr;
 }
 
-// Two passes for more than 5 MB of logits. On the device they are the faster way from
-// the start (f32 rows of 32,000: 32 rows 11.4 us against 13.1, 128 rows 16 against 30;
-// rows of 151,936 alike up to 78 MB, and slower by a tenth at 156 MB, which the L2
-// cache does not hold), but their third launch costs the host 2.4 us, which up to
-// about 4 MB is more than they save.
+// Two passes, or a cluster per row. On the device the passes are the faster way almost
+// from the start (us of a call with probabilities, cluster and passes: f32, 32,000
+// logits, 4 rows 11.9 and 11.5, 21 rows 13.8 and 12.5, 36 rows, more clusters than the
+// GPU holds at once, 18.2 and 13.0, 169 rows 42 and 25; 1 row of 151,936 16.3 and 10.4;
+// bf16, 36 rows of 8,000, 17.1 and 13.3), but their third launch costs the host 2.4 us,
+// which decides for calls shorter than the host's part of them.
 bool two_passes(const loom_verify_desc *d) {
-    return d->n_rows * d->vocab * elem_bytes(d->type) > ((size_t)5 << 20) && d->n_rows <= 65535;
+    const size_t row = d->vocab * elem_bytes(d->type);
+    return (d->n_rows * row > ((size_t)5 << 20) || d->n_rows > 32 || row > ((size_t)400 << 10)) && d->n_rows <= 65535;
 }
 // CTAs to a row: those of its cluster, or of the two passes
 int parts_of(const loom_verify_desc *d) {
