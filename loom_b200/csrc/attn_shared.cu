@@ -43,7 +43,8 @@ __device__ __forceinline__ void after_prefix() {
 // ---- any shape ---------------------------------------------------------------
 // One CTA per chunk of positions and KV head. 32 positions at a time go to
 // shared memory as f32; 16 query rows (row, head of the group) share them, a
-// lane taking one position for the scores and hd / 32 dimensions for the sums.
+// lane taking one position for the scores and hd / 32 dimensions for the sums. Takes
+// what the copy engine cannot: odd head widths, strides off 16 bytes.
 constexpr int G_TP = 32, G_TR = 16, G_WARPS = 4;
 
 template <class T>
@@ -143,7 +144,11 @@ __global__ void __launch_bounds__(G_WARPS * 32) k_attn_shared_any(AttnArgs a) {
 // own rounding) and summed as rounded, so that they still add up to one; f32
 // operands go as three tf32 products (mma.cuh), and each step's leading products
 // are added to the running sums by f32 additions: the tensor core truncates its
-// own, which along a row of 128 dimensions cost 2.1e-6 of the result, not 1e-6.
+// own, which along a row of 128 dimensions cost 2.1e-6 of the result, where this costs
+// 3e-7. Bound by latency and issue at the 8 (16-bit: 12) warps that registers leave an
+// SM, and in long 16-bit caches by reading them: 32 f32 rows of 32 heads over 1,536
+// shared and up to 512 own positions 52 us (0.7 TB/s of caches, issue slots 39 % used,
+// tensor pipe 29 %), the bf16 own caches of 128 sequences, 349 MB, 69 us (5.1 TB/s).
 template <class T> constexpr int mma_tp() { return sizeof(T) == 4 ? 32 : 64; }
 template <class T> constexpr size_t mma_block() { return mma_tp<T>() * 128; }  // 128 bytes of a tile's rows
 template <class T, int HDP> constexpr size_t mma_tile() { return HDP * sizeof(T) / 128 * mma_block<T>(); }
@@ -614,7 +619,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
 // sums a lane each, then the parts weighted by e^(m - M), eight in flight; then the
 // own rows that not every row of the sequence sees, four at a time, and the
 // division. A lane has four dimensions of each 128. A row that sees nothing gives
-// zeros. Bound by reading the parts.
+// zeros. Bound by reading the parts: 128 sequences of up to two rows of 32 heads, 16
+// parts of each, in 20 us.
 // elements d .. d + 3 of a row of n, zeros past it; one access where it is aligned
 template <class T> __device__ __forceinline__ float4 four(const T *p, int d, int n, bool whole) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

@@ -181,7 +181,10 @@ __device__ __forceinline__ void split_rows(uint32_t (&ah)[4][4], uint32_t (&al)[
 // Parts of t: CTA (block of rows, adapter of the block, slice of n_in). A warp has
 // 16 rows; warps left over split the depth of a tile and join in shared memory. x
 // and the weights come in tiles of 32 deep for each of the nk warps that split it,
-// through stages of asynchronous copies.
+// through stages of asynchronous copies. A decode batch is bound by latency (32 rows of
+// 32 adapters of rank 64, 2,048 wide: 12 us cold), a prompt by issue and latency: 2,048
+// f16 rows, 4,096 wide, rank 64 in 41 us (52 TFLOP/s of tf32, issue 43 %). 256 threads
+// to a CTA (75 against 69 us of the call) and tiles twice as deep (80) were slower.
 // bytes of a stage: 64 / nk rows of x and 64 of weights, 32 nk deep; as many stages,
 // up to four, as fit what three CTAs of an SM (f32 weights: two) can have
 template <class T> __host__ __device__ constexpr int l_xtile(int nk) { return 64 / nk * (128 * nk + 16); }
@@ -296,7 +299,9 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
 
 // out: CTA (block of rows, adapter of the block, L_OUT columns). A warp has 16 rows;
 // warps left over split the columns. The weights and the base, which do not wait for
-// t, are asked for before it. Bound by reading the base and writing out.
+// t, are asked for before it. Bound by latency: 2,048 rows and columns of rank 64 in 33
+// us (1 TB/s of base and out); several column chunks to a CTA took 72 us of a call,
+// not 69.
 constexpr int L_DEEP = 64;  // ranks at a time
 template <class T> constexpr size_t l_expand_smem() { return (size_t)L_OUT * w_stride<T>(L_DEEP) + 64 * (L_DEEP * 4 + 16); }
 
@@ -427,7 +432,10 @@ const char *check(const loom_lora_desc *d) {
 
 // Slices of n_in: enough CTAs for the GPU's 148 SMs, at least 128 wide. One block
 // is a decode batch, where about every row brings its own adapter; more blocks
-// are prompts, whose rows come in runs of one.
+// are prompts, whose rows come in runs of one. Two CTAs per SM: at one and at four a
+// prompt of 2,048 rows took 86 and 66 us, here 62, 32 decode rows 21.3 and 17.0, here
+// 17.5. Slices of 128 at the least: of 256, 168 rows of 4,096 took 20.6 us, not 18.6;
+// of 64 19.4, not 17.0.
 int slice_of(const loom_lora_desc *d) {
     const size_t blocks = (d->n_rows + L_RB - 1) / L_RB;
     const size_t groups = blocks > 1 ? blocks : std::max<size_t>(1, std::min(d->n_rows, d->n_adapters));
@@ -442,7 +450,7 @@ template <class T> cudaError_t launch(const LoraArgs &a, cudaStream_t st) {
     const unsigned blocks = (a.n_rows + L_RB - 1) / L_RB, most = std::min(std::min(L_RB, a.n_rows), a.n_adapters + 1);
     // A CTA per adapter of a decode batch's one block; of a prompt's blocks, whose rows
     // come in runs, as many as fill the GPU, each taking several adapters in turn where
-    // there are more.
+    // there are more (at 2, 4, 6 and 12 CTAs per SM 2,048 rows took 67, 67, 62 and 64 us).
     auto groups = [&](unsigned others) { return blocks == 1 ? most : std::min(most, std::max(2u, 6 * 148 / (blocks * others))); };
     cudaError_t e = allow_smem<k_lora_expand<T>>(l_expand_smem<T>());
     if (e != cudaSuccess) return e;

@@ -278,8 +278,9 @@ __device__ __forceinline__ void sum_pieces(int n, float top, float inv, bool gre
 // A CTA takes V_CH pieces of a row for the row's largest logit, then (in a second
 // kernel) the same pieces for the sum: the weights need the largest of the whole row,
 // and reading again, mostly from the L2 cache, costs less than a cluster's meeting for
-// it once rows take turns on the SMs. 366 rows of 129,281 bf16: the whole call 71 us
-// against 90. Bound by about 25 instructions per logit, most of them e^x.
+// it once rows take turns on the SMs. 366 rows of 129,281 bf16: the maxima 18 us (5.2
+// TB/s), the sums 46 (issue slots 75 % used), bound by about 25 instructions per
+// logit, most of them e^x.
 constexpr int V_CH = 1024, V_CT = 256;
 
 template <class T> __global__ void __launch_bounds__(V_CT) k_verify_max(VerifyArgs a) {
@@ -342,7 +343,8 @@ template <class T> __global__ void __launch_bounds__(V_CT) k_verify_sum(VerifyAr
 // ---- few rows: one launch, a cluster per row --------------------------------------------
 // The largest logit, then every CTA's sum of the weights, from registers (the parts
 // meet in row_stat, so the cluster meets once, for the maximum). Bound by issuing
-// about 25 instructions per logit, most of them e^x, and by that meeting.
+// about 25 instructions per logit, most of them e^x, and by that meeting: 5 greedy rows
+// of 32,000 f32, the whole call 7 us.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, sizeof(T) == 4 ? 2 : 3) k_verify_rows(VerifyArgs a) {
     __shared__ float s_best[V_W], s_cta;
     __shared__ double s_sum[V_W];
@@ -402,7 +404,8 @@ template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__
 // One cluster per sequence: the accepted drafts, then one token. The sums of the
 // weights over the runs of all the warps say in whose run the chosen index lies, that
 // warp's sums over its steps in which of them; it weighs that step again and finds the
-// index. Bound by the chain of such meetings and by reading the row.
+// index. Bound by the chain of such meetings and by reading the row: 32 sequences,
+// 151,936 f32 logits and probabilities, 29 us cold.
 // Without a drafter's probabilities nothing needs the whole row and one CTA does it (C = 1):
 // 59 against 65 us for 64 sequences, 366 rows of 129,281 bf16 logits.
 template <class T, int C> __global__ void __cluster_dims__(C, 1, 1) __launch_bounds__(V_T, 2) k_verify_pick(VerifyArgs a) {
