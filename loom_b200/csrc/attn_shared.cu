@@ -616,9 +616,9 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
 
 // ---- join ----------------------------------------------------------------------
 // WPH warps per (row, head), one warp where the parts are few: their maxima and
-// sums a lane each, then the parts weighted by e^(m - M), eight in flight; then the
-// own rows that not every row of the sequence sees, four at a time, and the
-// division. A lane has four dimensions of each 128. A row that sees nothing gives
+// sums a lane each, then the parts weighted by e^(m - M), eight in flight; before
+// them, while the chunk kernels may still run, the own rows that not every row of the
+// sequence sees, four at a time; at the end the division. A lane has four dimensions of each 128. A row that sees nothing gives
 // zeros. Bound by reading the parts: 128 sequences of up to two rows of 32 heads, 16
 // parts of each, in 20 us.
 // elements d .. d + 3 of a row of n, zeros past it; one access where it is aligned
@@ -653,9 +653,11 @@ __device__ __forceinline__ void scale_by(float4 &a, float f) {
     a.w *= f;
 }
 
-// ND: groups of 128 dimensions; whole: rows of parts, queries and own caches lie on
-// four elements
-template <class T, int WPH, int ND> __global__ void __launch_bounds__(128) k_attn_shared_join(AttnArgs a, bool whole) {
+// ND: groups of 128 dimensions; whole, whole_out: rows of queries and own caches, of out
+// lie on four elements. Six CTAs to an SM where registers allow: 64 sequences of up to 5
+// rows, 78.4 us a call, with four 82.2 (f32: 55 with six, 53 as it is).
+template <class T, int WPH, int ND> __global__ void __launch_bounds__(128, sizeof(T) == 2 && WPH == 1 && ND == 1 ? 6 : 1)
+    k_attn_shared_join(AttnArgs a, bool whole, bool whole_out) {
     __shared__ float4 s_acc[WPH > 1 ? 4 : 1][ND * 32];
     __shared__ float2 s_ml[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPH, hd = a.hd;
@@ -683,6 +685,36 @@ template <class T, int WPH, int ND> __global__ void __launch_bounds__(128) k_att
     for (int d = 0; d < ND; d++) {
         acc[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         q[d] = four(static_cast<const T *>(a.q) + r * a.q_stride + (int64_t)h * hd, d * 128 + lane * 4, hd, whole);
+    }
+    // no kernel of the call writes these
+    const T *k0 = static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead, *v0 = static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead;
+    for (int p0 = part ? see : s.common; p0 < see; p0 += 4) {
+        float x[4];
+        float4 v[4][ND];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[j] = 0.0f;
+            const int64_t at = (int64_t)min(p0 + j, see - 1) * a.opos;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const float4 k = four(k0 + at, d * 128 + lane * 4, hd, whole);
+                v[j][d] = four(v0 + at, d * 128 + lane * 4, hd, whole);
+                x[j] = fmaf(q[d].x, k.x, fmaf(q[d].y, k.y, fmaf(q[d].z, k.z, fmaf(q[d].w, k.w, x[j]))));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[j] = warp_sum(x[j]) * a.scale;
+            if (p0 + j >= see || x[j] == -INFINITY) continue;
+            const float mn = fmaxf(m, x[j]), fa = ex2(m - mn), fb = ex2(x[j] - mn);
+            l = l * fa + fb;
+            m = mn;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                scale_by(acc[d], fa);
+                mul_add(acc[d], fb, v[j][d]);
+            }
+        }
     }
     const int64_t step = (int64_t)a.n_rows * a.nh;  // (row, head) pairs from part to part
     pdl_wait_();
@@ -735,44 +767,22 @@ template <class T, int WPH, int ND> __global__ void __launch_bounds__(128) k_att
             for (int d = 0; d < ND; d++) mul_add(acc[d], f, s_acc[w][d * 32 + lane]);
         }
     }
-    const T *k0 = static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead, *v0 = static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead;
-    for (int p0 = s.common; p0 < see; p0 += 4) {
-        float x[4];
-        float4 v[4][ND];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = 0.0f;
-            const int64_t at = (int64_t)min(p0 + j, see - 1) * a.opos;
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                const float4 k = four(k0 + at, d * 128 + lane * 4, hd, whole);
-                v[j][d] = four(v0 + at, d * 128 + lane * 4, hd, whole);
-                x[j] = fmaf(q[d].x, k.x, fmaf(q[d].y, k.y, fmaf(q[d].z, k.z, fmaf(q[d].w, k.w, x[j]))));
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            x[j] = warp_sum(x[j]) * a.scale;
-            if (p0 + j >= see || x[j] == -INFINITY) continue;
-            const float mn = fmaxf(m, x[j]), fa = ex2(m - mn), fb = ex2(x[j] - mn);
-            l = l * fa + fb;
-            m = mn;
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                scale_by(acc[d], fa);
-                mul_add(acc[d], fb, v[j][d]);
-            }
-        }
-    }
     T *out = static_cast<T *>(a.out) + r * a.out_stride + (int64_t)h * hd;
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; d++) {
         const int at = d * 128 + lane * 4;
-        const float e[4] = {acc[d].x, acc[d].y, acc[d].z, acc[d].w};
+        if (at >= hd) continue;
+        T e[4] = {from_f32<T>(0.0f), from_f32<T>(0.0f), from_f32<T>(0.0f), from_f32<T>(0.0f)};
+        if (l != 0.0f) e[0] = from_f32<T>(acc[d].x * inv), e[1] = from_f32<T>(acc[d].y * inv), e[2] = from_f32<T>(acc[d].z * inv), e[3] = from_f32<T>(acc[d].w * inv);
+        if (whole_out) {
+            struct alignas(4 * sizeof(T)) Four { T e[4]; };
+            *reinterpret_cast<Four *>(out + at) = Four{{e[0], e[1], e[2], e[3]}};
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (at + k < hd) out[at + k] = from_f32<T>(l != 0.0f ? e[k] * inv : 0.0f);
+            for (int k = 0; k < 4; k++)
+                if (at + k < hd) out[at + k] = e[k];
+        }
     }
 }
 
@@ -917,11 +927,12 @@ template <class T, int ND> cudaError_t launch_join(const AttnArgs &a, int items,
     const auto on = [&](int64_t elems) { return elems % 4 == 0; };
     const auto at = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0; };
     const bool whole = on(a.hd) && on(a.q_stride) && on(a.opos) && on(a.ohead) && on(a.oseq) && at(a.q) && at(a.ok) && at(a.ov);
+    const bool whole_out = on(a.hd) && on(a.out_stride) && at(a.out);
     const dim3 grid((unsigned)(few ? pairs : (pairs + 3) / 4));
     if (items)
-        return few ? launch_pdl_(k_attn_shared_join<T, 4, ND>, grid, dim3(128), 0, st, a, whole)
-                   : launch_pdl_(k_attn_shared_join<T, 1, ND>, grid, dim3(128), 0, st, a, whole);
-    k_attn_shared_join<T, 1, ND><<<grid, 128, 0, st>>>(a, whole);  // reads seq_rows before its wait: only behind its own kernel
+        return few ? launch_pdl_(k_attn_shared_join<T, 4, ND>, grid, dim3(128), 0, st, a, whole, whole_out)
+                   : launch_pdl_(k_attn_shared_join<T, 1, ND>, grid, dim3(128), 0, st, a, whole, whole_out);
+    k_attn_shared_join<T, 1, ND><<<grid, 128, 0, st>>>(a, whole, whole_out);  // reads seq_rows before its wait: only behind its own kernel
     count_launch();
     return cudaGetLastError();
 }
