@@ -619,8 +619,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
 // sums a lane each, then the parts weighted by e^(m - M), eight in flight; before
 // them, while the chunk kernels may still run, the own rows that not every row of the
 // sequence sees, four at a time; at the end the division. A lane has four dimensions of each 128. A row that sees nothing gives
-// zeros. Bound by reading the parts: 128 sequences of up to two rows of 32 heads, 16
-// parts of each, in 20 us.
+// zeros. Bound by reading the parts: 128 sequences of up to two rows of 32 heads, 26 MB
+// of parts, in 18 us.
 // elements d .. d + 3 of a row of n, zeros past it; one access where it is aligned
 template <class T> __device__ __forceinline__ float4 four(const T *p, int d, int n, bool whole) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

@@ -183,7 +183,7 @@ __device__ __forceinline__ void split_rows(uint32_t (&ah)[4][4], uint32_t (&al)[
 // and the weights come in tiles of 32 deep for each of the nk warps that split it,
 // through stages of asynchronous copies. A decode batch is bound by latency (32 rows of
 // 32 adapters of rank 64, 2,048 wide: 12 us cold), a prompt by issue and latency: 2,048
-// f16 rows, 4,096 wide, rank 64 in 41 us (52 TFLOP/s of tf32, issue 43 %). 256 threads
+// f16 rows, 4,096 wide, rank 64 in 38 to 41 us (about 55 TFLOP/s of tf32 products, issue 42 %). 256 threads
 // to a CTA (75 against 69 us of the call) and tiles twice as deep (80) were slower.
 // bytes of a stage: 64 / nk rows of x and 64 of weights, 32 nk deep; as many stages,
 // up to four, as fit what three CTAs of an SM (f32 weights: two) can have
@@ -299,7 +299,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
 
 // out: CTA (block of rows, adapter of the block, L_OUT columns). A warp has 16 rows;
 // warps left over split the columns. The weights and the base, which do not wait for
-// t, are asked for before it. Bound by latency: 2,048 rows and columns of rank 64 in 33
+// t, are asked for before it. Bound by latency: 2,048 rows and columns of rank 64 in 32
 // us (1 TB/s of base and out); several column chunks to a CTA took 72 us of a call,
 // not 69.
 constexpr int L_DEEP = 64;  // ranks at a time
