@@ -317,6 +317,8 @@ LORA = {
     "rank 300": (20, 300, 200, [300, 257], [r % 2 for r in range(20)]),
     "many adapters": (64, 128, 128, [4] * 500, [(r * 37) % 500 for r in range(64)]),
     "prompt": (2000, 256, 264, [16, 16], [r // 1100 for r in range(2000)]),
+    "many parts": (39, 4096, 200, [67, 2, 65], [0] * 20 + [2] * 10 + [1] * 9),
+    "rows of two blocks, rank 66": (130, 640, 130, [66, 1], [0] * 100 + [1] * 30),
 }
 
 
@@ -642,3 +644,25 @@ def test_verify_refusals(sv):
         j = dict(i, **kw)
         with pytest.raises(LoomCudaError):
             sv.verify(j["logits"], j["tokens"], j["seq_rows"], j["u"], j["temperature"], j["draft_probs"])
+
+
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
+def test_what_scratch_holds_does_not_matter(sv, ty):
+    """The kept buffer full of NaN gives what a fresh one gives, in every operator."""
+    rows, lens = [3, 1, 0, 5] * 4, [70, 300, 9, 5] * 4
+    calls = []
+    for heads, kv, hd, prefix in ((32, 4, 128, 5000), (6, 2, 33, 90)):
+        i = attn_inputs(ty, rows, lens, heads, kv, hd, prefix, 300, seed=2)
+        calls.append(lambda i=i: (attn(sv, i),))
+    for n in (5, 70):
+        j = lora_inputs(ty, n, 700, 130, [67, 2, 0, 33], [r % 5 for r in range(n)], seed=n)
+        calls.append(lambda j=j: (lora(sv, j),))
+    for seqs, probs in ((2, True), (15, False), (15, True)):
+        k = verify_inputs(ty, [3] * seqs, 5003, [1.0] * seqs, probs, seed=4)
+        calls.append(lambda k=k: sv.verify(k["logits"], k["tokens"], k["seq_rows"], k["u"], k["temperature"], k["draft_probs"]))
+    first = [[o.clone() for o in c()] for c in calls]
+    for c, want in zip(calls, first):
+        for ws in sv._kept.values():
+            ws.fill_(255)
+        for o, w in zip(c(), want):
+            assert torch.equal(o, w)
