@@ -6,8 +6,13 @@ All three share one row layout: the rows of sequence b are seq_rows[b] ..
 seq_rows[b + 1] - 1 (cuda int32 [n_seqs + 1]): its last accepted token, then its
 drafts. Buffers are torch cuda tensors; arguments of a wrong type, shape or
 layout raise LoomCudaError before anything runs. A call runs on `stream` (a
-cudaStream_t), or torch's current stream, and only launches: it can be captured
-in a CUDA graph.
+cudaStream_t), or torch's current stream, and only launches. What it allocates,
+scratch and outputs, is allocated on the stream it runs on; as with any second
+stream, the caller orders `stream` after what made the tensors given, keeps them
+until the call is done, and orders what reads the outputs after it. Under
+torch.cuda.graph a call can be captured, on the current stream or on one that has
+joined the capture; a `stream` that is captured by other means is refused, since
+nothing would keep its scratch for the graph.
 """
 from __future__ import annotations
 
@@ -66,6 +71,27 @@ _kept = {}          # (device, stream) -> scratch of calls on that stream, in th
 _KEEP = 32 << 20    # bytes of it; calls that need more take theirs from torch's allocator
 
 
+def _at(dev: int, st: int):
+    """Stream `st` as torch's current one."""
+    return torch.cuda.stream(torch.cuda.ExternalStream(st, device=dev) if st else torch.cuda.default_stream(dev))
+
+
+def _new(op: str, shape, dtype, dev: int, stream: Optional[int], read: bool = True):
+    """An uninitialised tensor for a call on `stream`. Its memory comes from that stream's pool: what the current
+    stream has freed may still be in use by kernels that wait there, which `stream` does not wait for. `read`: on the
+    current stream, later."""
+    cur = _stream(dev)
+    if stream is None or stream == cur:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    joined = _capturing()  # torch's graph is taking the current stream, and `stream` with it if that is captured too
+    with _at(dev, stream):
+        _need(joined or not _capturing(), f"{op}: a stream that is captured must be torch's current one, or have joined its capture")
+        t = torch.empty(shape, dtype=dtype, device=dev)
+    if read and t.numel() and not joined:
+        t.record_stream(torch.cuda.current_stream(dev))
+    return t
+
+
 def _run(op: str, entry, size, desc, args, dev: int, stream: Optional[int]) -> None:
     """One call: its stream (the current one unless given) and scratch, the refusal as LoomCudaError. Small calls on one
     stream share a buffer, as they run one after the other; one that is being captured gets its own, which the graph
@@ -80,9 +106,7 @@ def _run(op: str, entry, size, desc, args, dev: int, stream: Optional[int]) -> N
             if entry(desc, *args, ws.data_ptr(), _KEEP, cur) == _lib.OK:
                 return
     need = size(desc)  # larger, captured, on a stream of the caller's, or refused: then for the reason it names
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    if st != cur and need:
-        ws.record_stream(torch.cuda.ExternalStream(st, device=dev))
+    ws = _new(op, need, torch.uint8, dev, st, read=False)
     _lib.must(entry(desc, *args, ws.data_ptr(), need, st), op)
 
 
@@ -103,7 +127,7 @@ def attn_shared(q, prefix_k, prefix_v, own_k, own_v, seq_rows, seq_len, scale: f
     pre = prefix_k.shape[0]
     _need(ty in TYPES, f"attn_shared: type must be float32, float16 or bfloat16, got {ty}")
     if out is None:
-        out = torch.empty(qs, dtype=ty, device=dev)
+        out = _new("attn_shared", qs, ty, dev, stream)
     pshape, oshape, i32 = (pre, kv, hd), (seqs, cap, kv, hd), torch.int32
     pst, ost, qst, dst = prefix_k.stride(), own_k.stride(), q.stride(), out.stride()
     if not (prefix_k.dtype is ty and prefix_v.dtype is ty and own_k.dtype is ty and own_v.dtype is ty and
@@ -149,7 +173,7 @@ def lora(x, a, b, ranks, scales, ids, base=None, out=None, stream: Optional[int]
     n, nout = x.shape[0], b.shape[1]
     _need(ty in TYPES, f"lora: type must be float32, float16 or bfloat16, got {ty}")
     if out is None:
-        out = torch.empty((n, nout), dtype=f32, device=dev)
+        out = _new("lora", (n, nout), f32, dev, stream)
     xst, ast, bst, dst = x.stride(), a.stride(), b.stride(), out.stride()
     cst = dst if base is None else base.stride()
     bshape, oshape = (na, nout, rank), (n, nout)
@@ -193,8 +217,7 @@ def verify(logits, tokens, seq_rows, u, temperature=None, draft_probs=None, out=
     seqs = seq_rows.numel() - 1
     _need(ty in TYPES, f"verify: type must be float32, float16 or bfloat16, got {ty}")
     if out is None:
-        out = (torch.empty(n, dtype=i32, device=dev), torch.empty(seqs, dtype=i32, device=dev),
-               torch.empty(n, dtype=f32, device=dev))
+        out = tuple(_new("verify", *w, dev, stream) for w in ((n, i32), (seqs, i32), (n, f32)))
     tok, cnt, lp = out
     lst = logits.stride()
     pst = (0, 1) if draft_probs is None else draft_probs.stride()

@@ -1,0 +1,59 @@
+"""GPU tests of the batched-serving operators' edges: streams and captures, values
+and random numbers at the ends of their ranges. Inputs, plain forms and tolerances
+are those of test_gpu_serve.py."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_serve import (ATTN_TOL, BF16, F16, F32, TYPES, attn, attn_inputs, attn_ref, ints, lora, lora_inputs,  # noqa: F401
+                                  lora_ref, rel, sv, verify_inputs)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- streams --------------------------------------------------------------------
+
+def test_a_call_on_another_stream_takes_no_memory_that_pending_kernels_use(sv):
+    """What the current stream has freed is still written by a kernel that waits there; the call on `st` does not."""
+    i = attn_inputs(BF16, [3, 1, 2] * 5, [50, 300, 129] * 5, 32, 4, 128, 1000, 320, seed=8)
+    j = lora_inputs(BF16, 70, 512, 512, [16, 8, 32], [r % 4 - 1 for r in range(70)], seed=6)
+    k = verify_inputs(F32, [3] * 9, 3001, [1.0] * 9, True, seed=4)
+    st = torch.cuda.Stream()
+    for call in (lambda s: (attn(sv, i, stream=s),), lambda s: (lora(sv, j, stream=s),),
+                 lambda s: sv.verify(k["logits"], k["tokens"], k["seq_rows"], k["u"], k["temperature"], k["draft_probs"],
+                                     stream=s)):
+        want = [t.clone() for t in call(None)]
+        torch.cuda.synchronize()
+        old = [torch.empty_like(t) for t in want] + [torch.empty(n << 10, dtype=torch.uint8, device="cuda")
+                                                     for n in (1, 16, 256, 1024, 4096)]
+        torch.cuda._sleep(50_000_000)
+        for t in old:
+            t.fill_(77)
+        ptrs = {t.data_ptr() for t in old}
+        del old, t
+        got = call(st.cuda_stream)
+        torch.cuda.synchronize()
+        assert not ptrs & {g.data_ptr() for g in got}
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_a_captured_call_on_a_joined_stream_keeps_its_scratch(sv):
+    i = attn_inputs(F16, [3, 1, 2] * 5, [50, 300, 129] * 5, 32, 4, 128, 1000, 320, seed=8)
+    j = lora_inputs(F32, 70, 512, 512, [16, 8, 32], [r % 4 - 1 for r in range(70)], seed=6)
+    want = attn(sv, i).clone(), lora(sv, j).clone()
+    torch.cuda.synchronize()
+    out, st, g = [torch.zeros_like(w) for w in want], torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cur = torch.cuda.current_stream()
+        st.wait_stream(cur)
+        attn(sv, i, out=out[0], stream=st.cuda_stream)
+        lora(sv, j, out=out[1], stream=st.cuda_stream)
+        cur.wait_stream(st)
+    room = [torch.full((n << 10,), 255, dtype=torch.uint8, device="cuda") for n in (64, 1024, 4096, 16384) * 4]
+    with torch.cuda.stream(st):
+        more = [torch.full((n << 10,), 255, dtype=torch.uint8, device="cuda") for n in (64, 1024, 4096, 16384) * 4]
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(out, want))
+    assert all(bool((t == 255).all()) for t in room + more)  # the graph writes to none of them

@@ -1,4 +1,5 @@
 """CPU checks of the batched-serving entries: struct layout, refusals that need no device."""
+import contextlib
 import ctypes as C
 import shutil
 import subprocess
@@ -65,3 +66,81 @@ def test_host_tensors_are_refused():
         serve.lora(z(1, 4), z(1, 2, 4), z(1, 3, 2), i[:1], z(1), i[:1])
     with pytest.raises(LoomCudaError, match="cuda"):
         serve.verify(z(1, 4), i[:1], i, z(1))
+
+
+class FakeTorch:
+    """The parts of torch that a call's allocations need: which stream is current when memory is asked for, and which
+    streams are captured."""
+    uint8 = torch.uint8
+
+    def __init__(self, captured=()):
+        self.now, self.made, self.cuda, self.captured = 1, [], self, set(captured)
+
+    def ExternalStream(self, st, device=None):
+        return st
+
+    def default_stream(self, dev):
+        return 0
+
+    def current_stream(self, dev=None):
+        return self.now
+
+    @contextlib.contextmanager
+    def stream(self, st):
+        was, self.now = self.now, st
+        yield
+        self.now = was
+
+    def empty(self, shape, dtype=None, device=None):
+        self.made.append((self.now, shape))
+        return self
+
+    def numel(self):
+        return 1
+
+    def record_stream(self, st):
+        pass
+
+    def data_ptr(self):
+        return 64
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    def use(**kw):
+        f = FakeTorch(**kw)
+        monkeypatch.setattr(serve, "torch", f)
+        monkeypatch.setattr(serve, "_stream", lambda dev: f.now)
+        monkeypatch.setattr(serve, "_capturing", lambda: f.now in f.captured)
+        monkeypatch.setattr(serve, "_kept", {})
+        return f
+    return use
+
+
+def run_on(stream):
+    serve._run("op", lambda *a: _lib.OK, lambda d: 1000, None, (), 0, stream)
+
+
+def test_scratch_belongs_to_the_stream_of_the_call(fake):
+    """Memory of the current stream's pool may still be in use by kernels that wait on it."""
+    f = fake()
+    run_on(7)
+    run_on(0)
+    assert f.made == [(7, 1000), (0, 1000)] and f.now == 1
+    run_on(None)
+    run_on(1)
+    assert f.made[2:] == [(1, serve._KEEP)]
+
+
+def test_scratch_of_captured_calls(fake):
+    """A graph keeps what torch gives the capture; a stream captured behind torch's back has no such memory."""
+    f = fake(captured=[1])
+    run_on(None)
+    assert f.made == [(1, 1000)]
+    f = fake(captured=[1, 7])
+    run_on(7)
+    assert f.made == [(7, 1000)]
+    f = fake(captured=[7])
+    with pytest.raises(LoomCudaError, match="captured"):
+        run_on(7)
+    assert f.made == []
