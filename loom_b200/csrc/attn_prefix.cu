@@ -307,7 +307,7 @@ __global__ void __maxnreg__(112)
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int k = 0; k < 64; k++) x[k & 3] = fmaxf(x[k & 3], __uint_as_float(s[k / 32][k % 32]));
-            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;  // scale >= 0
+            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;  // scale > 0
             if (__any_sync(0xffffffffu, top > m + AP_LAZY || (m == -INFINITY && top > m))) {
                 const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.0f : ex2(m - mn);
                 l0 *= f;

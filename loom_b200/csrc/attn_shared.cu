@@ -801,7 +801,8 @@ const char *check(const loom_attn_shared_desc *d) {
 }
 
 // Whether the prefix goes to attn_prefix.cu, as far as the call's sizes say: 16-bit
-// types, dimensions that fit its tiles, a quarter of a tile's rows and products enough
+// types, a scale above zero (its masked scores are -inf before they are scaled, and its
+// maxima are taken there), dimensions that fit its tiles, a quarter of a tile's rows and products enough
 // to make up for its longer start. Both kernels, bf16, 8 query heads to each of 4 KV
 // heads of 128, us of a call: 2^27 products (256 rows, prefix 1,024 / 64 rows, 4,096)
 // 15.9 / 13.5 here and 15.5 / 13.0 there, half of them (256 rows, 512) 12.0 and 14.6,
@@ -810,7 +811,7 @@ const char *check(const loom_attn_shared_desc *d) {
 // and 22.1. Heads of 64 meet at twice the positions.
 bool prefix_tc(const loom_attn_shared_desc *d) {
     const double rows = (double)d->n_rows * (d->n_heads / d->n_kv_heads);
-    return d->type != T_F32 && d->head_dim <= 128 && d->head_dim % 8 == 0 && d->scale >= 0.0f && rows >= 32 &&
+    return d->type != T_F32 && d->head_dim <= 128 && d->head_dim % 8 == 0 && d->scale > 0.0f && rows >= 32 &&
            rows * d->n_kv_heads * d->prefix_len * d->head_dim >= (double)(1 << 28);
 }
 

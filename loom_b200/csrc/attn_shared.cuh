@@ -98,7 +98,7 @@ __device__ __forceinline__ void attn_arrive(uint64_t *bar) {
 constexpr uint32_t ATTN_POLLS = 64;  // polls of a wait between looks at the CTA's error flag,
 constexpr int ATTN_TRIES = 1 << 14;  // and looks before it gives up
 
-// The prefix items of a 16-bit call (head_dim <= 128, scale >= 0, pre_rows <= 256,
+// The prefix items of a 16-bit call (head_dim <= 128, scale > 0, pre_rows <= 256,
 // pre_chunk a multiple of the box of ATTN_PREFIX_N positions) on the 5th-generation
 // tensor cores.
 constexpr int ATTN_PREFIX_N = 64;

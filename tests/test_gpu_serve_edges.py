@@ -57,3 +57,16 @@ def test_a_captured_call_on_a_joined_stream_keeps_its_scratch(sv):
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(out, want))
     assert all(bool((t == 255).all()) for t in room + more)  # the graph writes to none of them
+
+
+# ---- attention ------------------------------------------------------------------
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-42, -0.05])
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
+def test_attn_scales_without_a_sign(sv, ty, scale):
+    """A scale of zero weighs every position alike, whichever kernel takes the prefix; a negative one turns the order."""
+    for rows, lens, heads, kv, hd, prefix, cap in (([4] * 33, list(range(4, 37)), 32, 4, 128, 4099, 40),
+                                                   ([100, 0, 200], [120, 0, 200], 8, 8, 48, 2401, 200),
+                                                   ([2, 1], [5, 70], 8, 2, 33, 77, 80)):
+        i = dict(attn_inputs(ty, rows, lens, heads, kv, hd, prefix, cap, seed=prefix), scale=scale)
+        assert rel(attn(sv, i), attn_ref(i, rows, lens)) < ATTN_TOL[ty]
