@@ -573,7 +573,9 @@ template <class T, int C> __global__ void __cluster_dims__(C, 1, 1) __launch_bou
         }
         want = (double)a.u[r1 - 1] * total;
         // the first part whose end exceeds the threshold; the last with weight, should none
+        // (a random number of 1), and then the last in it
         int part = -1;
+        bool passed = false;
         double at = 0.0;
         for (int i = 0; i < a.parts; i += 32) {
             const double z = z_of(i + lane), end = at + running(z);
@@ -583,9 +585,13 @@ template <class T, int C> __global__ void __cluster_dims__(C, 1, 1) __launch_bou
                 part = i + l;
                 origin = __shfl_sync(0xffffffffu, end - z, l);
             }
-            if (over) break;
+            if (over) {
+                passed = true;
+                break;
+            }
             at = __shfl_sync(0xffffffffu, end, 31);
         }
+        if (!passed) want = INFINITY;
         if (part < 0) {  // no weight at all
             if (tid == 0) emit(0);
             return;
@@ -619,7 +625,8 @@ template <class T, int C> __global__ void __cluster_dims__(C, 1, 1) __launch_bou
         rest = false;
     }
     // the run with the chosen index: the first whose end exceeds the threshold; the
-    // last one with weight, should none (a random number of 1)
+    // last one with weight, should none (a random number of 1, or a part whose sum came
+    // out a rounding larger than its runs' together), and in it the last index with weight
     double c = __shfl_up_sync(0xffffffffu, upto, 1), before = 0.0;
     c = lane == 0 ? origin : origin + c;
     int pick = -1, heavy = -1;
@@ -640,7 +647,7 @@ template <class T, int C> __global__ void __cluster_dims__(C, 1, 1) __launch_bou
         before = __shfl_sync(0xffffffffu, start, __ffs(m) - 1);
     } else {
         pick = __reduce_max_sync(0xffffffffu, heavy);
-        before = want;
+        want = INFINITY;
     }
     if (pick < 0) {  // no weight at all
         if (tid == 0 && rank == 0) emit(0);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_gpu_serve import (ATTN_TOL, BF16, F16, F32, TYPES, attn, attn_inputs, attn_ref, ints, lora, lora_inputs,  # noqa: F401
-                                  lora_ref, rel, sv, verify_inputs)
+                                  lora_ref, rel, sv, check_verify, verify_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,31 @@ def test_attn_scales_without_a_sign(sv, ty, scale):
                                                    ([2, 1], [5, 70], 8, 2, 33, 77, 80)):
         i = dict(attn_inputs(ty, rows, lens, heads, kv, hd, prefix, cap, seed=prefix), scale=scale)
         assert rel(attn(sv, i), attn_ref(i, rows, lens)) < ATTN_TOL[ty]
+
+
+# ---- verification ---------------------------------------------------------------
+
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("probs", [True, False], ids=["probs", "sure"])
+@pytest.mark.parametrize("vocab,seqs", [(40, 2), (32000, 2), (32000, 40), (151937, 3)])
+def test_verify_random_number_of_one(sv, ty, probs, vocab, seqs):
+    """A uniform number rounded up to 1: no running sum exceeds the whole; the last token with weight is chosen."""
+    rows, last = [2] * seqs, vocab - vocab // 5 - 1
+    i = verify_inputs(ty, rows, vocab, [1.0] * seqs, probs, seed=vocab)
+    i["u"][:] = 1.0
+    i["logits"][:, last + 1:] = float("-inf")
+    i["tokens"][1::2] = 3
+    if probs:  # refuses the draft, and leaves the tokens at the end their weight
+        i["draft_probs"][:, 3] = 1.0
+        i["draft_probs"][:, vocab // 2:] = 0.0
+        i["draft_probs"][2, 3] = 0.5  # but for the second sequence's, whose p rounds to 1: then the token after it
+        i["logits"][2:4, 3] = i["logits"][2:4].float().amax(1).to(ty) + 40
+    tok, cnt, _ = (t.cpu().numpy() for t in sv.verify(i["logits"], i["tokens"], i["seq_rows"], i["u"], i["temperature"],
+                                                       i["draft_probs"]))
+    for b in range(seqs):
+        if probs and b == 1:
+            assert cnt[b] == 2 and tok[2] == 3
+            w = torch.exp(i["logits"][3].float() - i["logits"][3].float().amax())
+            assert tok[3] == int(torch.nonzero(w > 0)[-1])
+        else:
+            assert cnt[b] == 1 and tok[2 * b] == last and tok[2 * b + 1] == -1
