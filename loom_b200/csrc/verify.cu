@@ -103,11 +103,13 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs &a, int r) {
 // cluster's V_C * V_W has the k-th run of `run` 16-byte pieces, its lane l the
 // pieces l, l + 32, ... of the run. So a running sum over the vocabulary is one
 // over the warps, then over groups of 32 pieces, then over lanes. A thread keeps
-// its first v_nv pieces in registers (152,000 f32 logits take 9.3 of them), so the
-// row crosses the memory once although the weights need its maximum; longer rows
-// read the rest again. A row that does not start on 16 bytes is shifted: its first
-// piece holds fewer logits.
-template <class T> constexpr int v_nv() { return sizeof(T) == 4 ? 10 : 5; }
+// its first v_nv pieces in registers, so the row crosses the memory once although the
+// weights need its maximum; what is left is read again. Rows that take one launch have
+// up to 400 KB (two_passes below), 7 pieces a thread: f32 keeps all of them, 16-bit
+// types, twice the logits in each, 5. Only calls of more than 65,535 rows, which the
+// two passes' grid does not hold, bring longer ones. A row that does not start on 16
+// bytes is shifted: its first piece holds fewer logits.
+template <class T> constexpr int v_nv() { return sizeof(T) == 4 ? 7 : 5; }
 
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;

@@ -98,3 +98,37 @@ def test_verify_random_number_of_one(sv, ty, probs, vocab, seqs):
             assert tok[3] == int(torch.nonzero(w > 0)[-1])
         else:
             assert cnt[b] == 1 and tok[2 * b] == last and tok[2 * b + 1] == -1
+
+
+@pytest.mark.parametrize("ty", [F16, BF16], ids=["f16", "bf16"])
+def test_verify_one_launch_beyond_the_registers_of_a_cluster(sv, ty):
+    """The longest rows that take one launch: more than a cluster's CTAs keep in registers."""
+    for vocab in (163841, 190001, 204800):
+        for probs in (True, False):
+            i = verify_inputs(ty, [1, 2], vocab, [0.0, 0.9], probs, seed=vocab, std=3.0)
+            check_verify(sv, i, [1, 2])
+            i["logits"][:, : vocab - 5] = float("-inf")
+            check_verify(sv, i, [1, 2])
+
+
+def test_verify_one_launch_of_very_many_rows(sv):
+    """More rows than the two passes' grid holds, of more logits than registers do: all the same row, each with its
+    own random number."""
+    n, vocab = 65537, 120001
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    l = torch.randn(vocab, generator=g, device="cuda") * 3
+    u = torch.rand(n, generator=g, device="cuda")
+    temp = torch.full((n,), 0.9, device="cuda")
+    temp[::3] = 0.0
+    rows = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    tok, cnt, lp = sv.verify(l.expand(n, vocab), torch.zeros(n, dtype=torch.int32, device="cuda"), rows, u, temp)
+    assert bool((cnt == 1).all()) and bool((tok[::3] == l.argmax()).all())
+    x = torch.log_softmax(l.double() / 0.9, 0)
+    c = x.exp().cumsum(0)
+    t, want = tok.long(), u.double() * c[-1]
+    over = c[t] - want, want - (c[t] - x[t].exp())  # what the choice is above and below the threshold
+    drawn = torch.arange(n, device="cuda") % 3 != 0
+    assert bool((torch.minimum(*over)[drawn] > -1e-5).all())
+    want_lp = torch.where(drawn, x[t], torch.log_softmax(l.double(), 0)[t])
+    assert bool(((lp.double() - want_lp).abs() <= 2e-5 + 2e-6 * want_lp.abs()).all())
