@@ -17,6 +17,11 @@
 // reading the weights. The order of the summed dimension is free, so lane t of a
 // row takes its elements 8t .. 8t + 7 of 32, the four products of which use two
 // each: operands are read from shared memory 16 bytes at a time.
+//
+// The two terms of an infinite operand, or of one that rounds to infinity, are an
+// infinity and a NaN: every sum that such an operand is part of comes out NaN. A CTA of
+// the second kernel that finds a NaN takes its rows again in plain f32, t as well as
+// out, which gives the infinity, the large number or the NaN that it stands for.
 #include <algorithm>
 #include <type_traits>
 
@@ -305,7 +310,37 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
 constexpr int L_DEEP = 64;  // ranks at a time
 template <class T> constexpr size_t l_expand_smem() { return (size_t)L_OUT * w_stride<T>(L_DEEP) + 64 * (L_DEEP * 4 + 16); }
 
-template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs a) {
+// A CTA's rows and columns in plain f32 (s_x: room for L_DEEP of t). A call of its own:
+// inlined, it cost 2,048 rows 2 us.
+template <class T> __device__ __noinline__ void expand_plain(const LoraArgs &a, Group gr, const int *s_rows, float *s_x, int o0) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = lora_rank(a, gr.id), o = o0 + tid;
+    const bool in = o < a.n_out;
+    const T *wa = static_cast<const T *>(a.a) + gr.id * a.a_adapter, *wb = static_cast<const T *>(a.b) + gr.id * a.b_adapter + o * a.b_row;
+    for (int m = 0; m < gr.rows; m++) {
+        const int64_t row = s_rows[m];
+        const float *x = a.x + row * a.x_stride, *t = a.t + row * a.t_row;
+        float s = in && a.base ? a.base[row * a.base_stride + o] : 0.0f;
+        for (int k0 = 0; k0 < rank; k0 += L_DEEP) {
+            const int n = min(rank - k0, L_DEEP);
+            __syncthreads();
+            for (int k = warp; k < n; k += 4) {
+                float v = 0.0f;
+                for (int z = 0; z < a.n_slices; z++) v += __ldcg(t + (size_t)z * a.n_rows * a.t_row + k0 + k);
+                if (v != v) {
+                    v = 0.0f;
+                    for (int i = lane; i < a.n_in; i += 32) v = fmaf(x[i], to_f32(wa[(k0 + k) * a.a_row + i]), v);
+                    v = warp_sum(v);
+                }
+                if (lane == 0) s_x[k] = v * a.scales[gr.id];
+            }
+            __syncthreads();
+            for (int k = 0; k < n && in; k++) s = fmaf(to_f32(wb[k0 + k]), s_x[k], s);
+        }
+        if (in) a.out[row * a.out_stride + o] = s;
+    }
+}
+
+template <class T> __global__ void __launch_bounds__(128) k_lora_expand(const __grid_constant__ LoraArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_rows[L_RB];
     constexpr int WST = w_stride<T>(L_DEEP), TST = L_DEEP + 4;
@@ -396,6 +431,15 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_expand(LoraArgs
                         for (int n = 0; n < NT; n += 4)
                             mma_tiles<T, 4>(c + n, ah, al, smem + (c0 + n * 8 + g) * WST + (q + 8 * t) * (int)sizeof(T), WST);
                     }
+            }
+            bool nan = false;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) nan = nan || c[n][j] != c[n][j];
+            if (__syncthreads_or(nan && rank)) {  // none has written yet: out may be base
+                expand_plain<T>(a, gr, s_rows, s_x, o0);
+                return;
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {

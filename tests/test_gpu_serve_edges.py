@@ -132,3 +132,28 @@ def test_verify_one_launch_of_very_many_rows(sv):
     assert bool((torch.minimum(*over)[drawn] > -1e-5).all())
     want_lp = torch.where(drawn, x[t], torch.log_softmax(l.double(), 0)[t])
     assert bool(((lp.double() - want_lp).abs() <= 2e-5 + 2e-6 * want_lp.abs()).all())
+
+
+# ---- adapters -------------------------------------------------------------------
+
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 20, 40, 150])
+def test_lora_infinite_operands(sv, ty, n):
+    """Infinities and values at the end of the range go where plain arithmetic takes them, and no further."""
+    ranks, ids = [1, 16, 70], [r % 3 for r in range(n)]
+    for k, at, v in (("x", (0, 5), float("inf")), ("x", (n // 2, 600), float("-inf")), ("x", (0, 7), torch.finfo(F32).max),
+                     ("a", (0, 0, 3), float("inf")), ("a", (1 % n, 2, 300), float("-inf")), ("b", (0, 9, 0), float("inf")),
+                     ("b", (1, 100, 15), float("-inf")), ("b", (2, 33, 69), float("inf")), ("b", (2, 40, 68), torch.finfo(ty).max)):
+        i = lora_inputs(ty, n, 700, 130, ranks, ids, seed=n)
+        i["a"] = i["a"] * 2.0 ** -8  # the largest x stays in range
+        i[k][at] = v
+        out, want = lora(sv, i), lora_ref(i)
+        fin = torch.isfinite(want)
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isinf(out), torch.isinf(want))
+        big = torch.isinf(want)
+        assert torch.equal(out[big].double(), want[big])
+        # by rows: those with huge results have a norm of their own
+        for r in range(n):
+            f = fin[r]
+            if f.any():
+                assert float((out[r][f].double() - want[r][f]).abs().max()) <= 2e-5 * float(want[r][f].abs().max())
