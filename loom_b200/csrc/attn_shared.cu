@@ -653,11 +653,50 @@ __device__ __forceinline__ void scale_by(float4 &a, float f) {
     a.w *= f;
 }
 
+// Row r of head h by one warp in plain f32 over everything it sees (`see` own positions
+// of sequence b): the two tf32 terms of an infinite operand are an infinity and a NaN,
+// and a row that came out NaN is taken again so that it has what f32 arithmetic gives.
+template <class T, int ND> __device__ __noinline__ void row_plain(const AttnArgs &a, int r, int h, int b, int see) {
+    const int lane = threadIdx.x & 31, hd = a.hd, kvh = h / a.group;
+    float m = -INFINITY, l = 0.0f;
+    float acc[ND * 4], q[ND * 4];
+    auto at = [&](int i) { return lane + 32 * i; };  // a lane's i-th dimension
+#pragma unroll
+    for (int i = 0; i < ND * 4; i++) {
+        acc[i] = 0.0f;
+        q[i] = at(i) < hd ? to_f32(static_cast<const T *>(a.q)[r * a.q_stride + (int64_t)h * hd + at(i)]) : 0.0f;
+    }
+    auto cache = [&](const T *k0, const T *v0, int n, int64_t pos) {
+        for (int p = 0; p < n; p++) {
+            const T *k = k0 + p * pos, *v = v0 + p * pos;
+            float x = 0.0f, e[ND * 4];
+#pragma unroll
+            for (int i = 0; i < ND * 4; i++) {
+                x = fmaf(q[i], at(i) < hd ? to_f32(k[at(i)]) : 0.0f, x);
+                e[i] = at(i) < hd ? to_f32(v[at(i)]) : 0.0f;
+            }
+            x = warp_sum(x) * a.scale;
+            if (x == -INFINITY) continue;
+            const float mn = fmaxf(m, x), fa = ex2(m - mn), fb = ex2(x - mn);
+            l = l * fa + fb;
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < ND * 4; i++) acc[i] = fmaf(e[i], fb, acc[i] * fa);
+        }
+    };
+    cache(static_cast<const T *>(a.pk) + kvh * a.phead, static_cast<const T *>(a.pv) + kvh * a.phead, a.prefix, a.ppos);
+    cache(static_cast<const T *>(a.ok) + b * a.oseq + kvh * a.ohead, static_cast<const T *>(a.ov) + b * a.oseq + kvh * a.ohead, see, a.opos);
+    T *out = static_cast<T *>(a.out) + r * a.out_stride + (int64_t)h * hd;
+#pragma unroll
+    for (int i = 0; i < ND * 4; i++)
+        if (at(i) < hd) out[at(i)] = from_f32<T>(l != 0.0f ? acc[i] / l : 0.0f);
+}
+
 // ND: groups of 128 dimensions; whole, whole_out: rows of queries and own caches, of out
 // lie on four elements. Six CTAs to an SM where registers allow: 64 sequences of up to 5
 // rows, 78.4 us a call, with four 82.2 (f32: 55 with six, 53 as it is).
 template <class T, int WPH, int ND> __global__ void __launch_bounds__(128, sizeof(T) == 2 && WPH == 1 && ND == 1 ? 6 : 1)
-    k_attn_shared_join(AttnArgs a, bool whole, bool whole_out) {
+    k_attn_shared_join(const __grid_constant__ AttnArgs a, bool whole, bool whole_out) {
     __shared__ float4 s_acc[WPH > 1 ? 4 : 1][ND * 32];
     __shared__ float2 s_ml[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPH, hd = a.hd;
@@ -765,6 +804,15 @@ template <class T, int WPH, int ND> __global__ void __launch_bounds__(128, sizeo
             l += s_ml[w].y * f;
 #pragma unroll
             for (int d = 0; d < ND; d++) mul_add(acc[d], f, s_acc[w][d * 32 + lane]);
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+        bool nan = l != l;
+#pragma unroll
+        for (int d = 0; d < ND; d++) nan = nan || acc[d].x != acc[d].x || acc[d].y != acc[d].y || acc[d].z != acc[d].z || acc[d].w != acc[d].w;
+        if (a.split && __any_sync(0xffffffffu, nan)) {
+            row_plain<T, ND>(a, r, h, b, see);
+            return;
         }
     }
     T *out = static_cast<T *>(a.out) + r * a.out_stride + (int64_t)h * hd;
@@ -957,6 +1005,7 @@ template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         a.first = a.n_pre * a.pre_tiles;
     }
+    a.split = mapped && sizeof(T) == 4;
     if (const int items = all - a.first) {
         if (!mapped)
             e = launch_items<k_attn_shared_any<T>>((size_t)(G_TR * a.hd + G_TP * (a.hd + 1) + G_TP * a.hd + G_TR * G_TP) * 4,

@@ -21,6 +21,7 @@ struct AttnArgs {
     int prefix, cap;
     int pre_chunk, own_chunk, n_pre, n_own, pre_tiles, pre_rows;
     int first;    // first item of a launch that leaves the prefix's to another
+    int split;    // f32 products were made of tf32 terms
     float scale;  // of the scores in base 2: scale * log2(e)
 };
 

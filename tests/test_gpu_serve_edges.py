@@ -72,6 +72,34 @@ def test_attn_scales_without_a_sign(sv, ty, scale):
         assert rel(attn(sv, i), attn_ref(i, rows, lens)) < ATTN_TOL[ty]
 
 
+ENDS = {
+    "few rows": ([2, 1, 3], [40, 65, 9], 8, 2, 128, 150, 72),
+    "many rows": ([4] * 33, list(range(4, 37)), 32, 4, 128, 4099, 40),
+    "more rows of a sequence": ([20, 12], [60, 30], 8, 2, 64, 100, 60),
+    "heads of 200": ([2, 1], [40, 65], 4, 2, 200, 150, 72),
+    "odd heads": ([2, 1], [40, 65], 4, 2, 33, 150, 72),
+}
+
+
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", ENDS, ids=[s.replace(" ", "_") for s in ENDS])
+def test_attn_infinities_that_are_seen(sv, ty, shape):
+    """A key whose score is -inf has no weight, one far below the others neither; an infinite value is the result's."""
+    rows, lens, heads, kv, hd, prefix, cap = ENDS[shape]
+    i = attn_inputs(ty, rows, lens, heads, kv, hd, prefix, cap, seed=3)
+    i["q"][..., 0] = i["q"][..., 0].abs() + 0.25
+    for k, at in (("pk", (7,)), ("pk", (prefix - 1,)), ("ok", (0, 3)), ("ok", (1, 0))):
+        i[k][at][..., 0] = float("-inf")
+    i["pk"][64, :, 0] = -torch.finfo(ty).max
+    assert rel(attn(sv, i), attn_ref(i, rows, lens)) < ATTN_TOL[ty]
+    i["pv"][20, 0, 5] = float("inf")
+    i["ov"][0, 2, -1, 9] = float("-inf")
+    out, want = attn(sv, i), attn_ref(i, rows, lens)
+    assert torch.equal(torch.isinf(out), torch.isinf(want)) and torch.equal(out[torch.isinf(want)].double(), want[torch.isinf(want)])
+    fin = torch.isfinite(want)
+    assert bool(torch.isfinite(out[fin]).all()) and not bool(fin.all()) and rel(out[fin], want[fin]) < ATTN_TOL[ty]
+
+
 # ---- verification ---------------------------------------------------------------
 
 @pytest.mark.parametrize("ty", TYPES, ids=["f32", "f16", "bf16"])
