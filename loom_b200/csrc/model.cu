@@ -18,6 +18,7 @@
 // and one device->host copy.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -146,6 +147,20 @@ template <class T> int dalloc(Model &m, T *&p, size_t n, bool zero = false) {
     return 0;
 }
 
+// A buffer whose contents are not needed: the one before is given back first. Nothing
+// on the device may still use it.
+template <class T> int regrow(Model &m, T *&p, size_t n, bool zero = false) {
+    if (p) {
+        m.allocs.erase(std::find(m.allocs.begin(), m.allocs.end(), static_cast<void *>(p)));
+        MCK(cudaFree(p));
+        p = nullptr;
+    }
+    return dalloc(m, p, n, zero);
+}
+// room for `need` where there is room for `have`: half as much again, so that calls that
+// grow little by little allocate now and then
+size_t grown(size_t need, size_t have) { return std::max(need, have + have / 2); }
+
 void free_model(Model *m) {
     if (m->exec) cudaGraphExecDestroy(m->exec);
     if (m->ab_trace) cudaFree(m->ab_trace);
@@ -216,9 +231,9 @@ void matvec(const Mat &m, const float *xf, const XQW &x256, const XQW &x32, floa
 }
 
 int alloc_xq(Model &m, XQW &q, size_t cols, bool k256) {
-    if (int rc = dalloc(m, q.q, cols)) return rc;
-    if (int rc = dalloc(m, q.d, cols / (k256 ? 256 : 32) + 1)) return rc;
-    return dalloc(m, q.s, cols / (k256 ? 16 : 32) + 1);
+    if (int rc = regrow(m, q.q, cols)) return rc;
+    if (int rc = regrow(m, q.d, cols / (k256 ? 256 : 32) + 1)) return rc;
+    return regrow(m, q.s, cols / (k256 ? 16 : 32) + 1);
 }
 
 // A dense FFN on the streamed matvec: normed x already quantized in m.n256;
@@ -382,12 +397,15 @@ void matmul_rows(const Mat &m, const float *xf, const XQW &x256, const XQW &x32,
 
 int alloc_prefill(Model &m, size_t n) {
     if (n <= m.pf_cap) return 0;
+    MCK(cudaStreamSynchronize(rt_stream(nullptr)));  // all that uses the rows runs there
+    n = grown(n, m.pf_cap);
+    m.pf_cap = 0;
     const size_t dim = m.dim, qd = m.nh * m.hd, kvd = m.nkv * m.hd;
     int rc = 0;
-    if ((rc = dalloc(m, m.pf_x[0], n * dim)) || (rc = dalloc(m, m.pf_x[1], n * dim)) ||
-        (rc = dalloc(m, m.pf_normed, n * dim)) || (rc = dalloc(m, m.pf_q, n * qd)) || (rc = dalloc(m, m.pf_k, n * kvd)) ||
-        (rc = dalloc(m, m.pf_v, n * kvd)) || (rc = dalloc(m, m.pf_att, n * qd)) || (rc = dalloc(m, m.pf_proj, n * dim)) ||
-        (rc = dalloc(m, m.pf_zero, n, true)) || (rc = dalloc(m, m.pf_tok, n)) || (rc = dalloc(m, m.pf_pos, 1)) ||
+    if ((rc = regrow(m, m.pf_x[0], n * dim)) || (rc = regrow(m, m.pf_x[1], n * dim)) ||
+        (rc = regrow(m, m.pf_normed, n * dim)) || (rc = regrow(m, m.pf_q, n * qd)) || (rc = regrow(m, m.pf_k, n * kvd)) ||
+        (rc = regrow(m, m.pf_v, n * kvd)) || (rc = regrow(m, m.pf_att, n * qd)) || (rc = regrow(m, m.pf_proj, n * dim)) ||
+        (rc = regrow(m, m.pf_zero, n, true)) || (rc = regrow(m, m.pf_tok, n)) || (rc = regrow(m, m.pf_pos, 1)) ||
         (rc = alloc_xq(m, m.pf_n256, n * dim, true)) || (rc = alloc_xq(m, m.pf_n32, n * dim, false)) ||
         (rc = alloc_xq(m, m.pf_a256, n * qd, true)) || (rc = alloc_xq(m, m.pf_a32, n * qd, false)))
         return rc;
@@ -487,9 +505,9 @@ int alloc_batch(Model &m, size_t B) {
     if (m.bd_cap) return 0;
     const size_t cache = B * m.n_layers * m.ctx * m.nkv * m.hd;
     int rc = 0;
-    if ((rc = dalloc(m, m.bkc, cache, true)) || (rc = dalloc(m, m.bvc, cache, true)) ||
-        (rc = dalloc(m, m.bd_logits, B * m.vocab)) || (rc = dalloc(m, m.bd_pos, B)) || (rc = dalloc(m, m.bd_next, B)) ||
-        (rc = dalloc(m, m.bd_part, B * attn_part_floats((int)m.nh, (int)m.nkv, (int)m.hd, (int)m.ctx))))
+    if ((rc = regrow(m, m.bkc, cache, true)) || (rc = regrow(m, m.bvc, cache, true)) ||
+        (rc = regrow(m, m.bd_logits, B * m.vocab)) || (rc = regrow(m, m.bd_pos, B)) || (rc = regrow(m, m.bd_next, B)) ||
+        (rc = regrow(m, m.bd_part, B * attn_part_floats((int)m.nh, (int)m.nkv, (int)m.hd, (int)m.ctx))))
         return rc;
     m.bd_cap = B;
     return 0;
@@ -1086,22 +1104,25 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
     if (int rc = alloc_batch(m, n)) return rc;
     int rc = 0;
     const size_t words_in = 5 * rows + 3 * n + 1, words_out = 2 * rows + n;
-    if (rows > m.sh_rows || n > m.sh_seqs) {
-        const size_t r = std::max(rows, m.sh_rows), q = std::max(n, m.sh_seqs);
-        if ((rc = dalloc(m, m.sh_logits, r * m.vocab)) || (rc = dalloc(m, m.sh_in, 5 * r + 3 * q + 1)) ||
-            (rc = dalloc(m, m.sh_out, 2 * r + q)))
+    const bool more = rows > m.sh_rows || n > m.sh_seqs;
+    if (more || ws > m.sh_ws) MCK(cudaStreamSynchronize(rt_stream(nullptr)));
+    if (more) {
+        const size_t r = rows > m.sh_rows ? grown(rows, m.sh_rows) : m.sh_rows, q = n > m.sh_seqs ? grown(n, m.sh_seqs) : m.sh_seqs;
+        m.sh_rows = m.sh_seqs = 0;
+        if ((rc = regrow(m, m.sh_logits, r * m.vocab)) || (rc = regrow(m, m.sh_in, 5 * r + 3 * q + 1)) ||
+            (rc = regrow(m, m.sh_out, 2 * r + q)))
             return rc;
         if (m.sh_host) cudaFreeHost(m.sh_host);
         m.sh_host = nullptr;
-        m.sh_rows = m.sh_seqs = 0;
         MCK(cudaHostAlloc(&m.sh_host, (5 * r + 3 * q + 1) * 4, cudaHostAllocDefault));
         m.sh_rows = r;
         m.sh_seqs = q;
     }
     if (ws > m.sh_ws) {
+        const size_t bytes = grown(ws, m.sh_ws);
         m.sh_ws = 0;
-        if ((rc = dalloc(m, m.sh_scratch, ws))) return rc;
-        m.sh_ws = ws;
+        if ((rc = regrow(m, m.sh_scratch, bytes))) return rc;
+        m.sh_ws = bytes;
     }
     if ((rc = loom_cuda_reserve(rows, m.dim, std::max<size_t>(m.max_ffn, 1), m.max_ne, m.max_nu))) return rc;
     // [tokens][positions][sequence of the row][adapter of the row][random numbers] by row, [first rows][lengths][temperatures]

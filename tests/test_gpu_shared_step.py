@@ -222,3 +222,51 @@ def test_batched_decode_and_prefill_keep_their_results(be):
     finally:
         dev.free()
         other.free()
+
+
+def test_growing_steps_hold_what_the_largest_needs(be):
+    """Steps of 1 to 60 rows: the device memory they hold follows the largest, not all of them together."""
+    spec = small_llama()
+    dev = DeviceModel(spec)
+    other = DeviceModel(spec)
+    rng = np.random.default_rng(7)
+    try:
+        for m in (dev, other):
+            m.prefill([3, 1, 4, 1, 5])
+        toks = rng.integers(1, spec.vocab, size=60).tolist()
+        dev.shared_step(5, [[9]], [1])
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        for n in range(1, 61):
+            _, _, got = dev.shared_step(5, [toks[:n]], [n], logits=True)
+        held = before - torch.cuda.mem_get_info()[0]
+        # logits of 60 rows: 7.7 MB; the layers' rows and the scratch less. Twice that, and whole pages of 2 MB each
+        assert held < 64 << 20, held
+        _, _, want = other.shared_step(5, [toks], [60], logits=True)
+        assert np.array_equal(got, want)
+    finally:
+        dev.free()
+        other.free()
+
+
+def test_the_scratch_follows_the_prompt(be):
+    """Another cut of the prompt, another number of sequences within the first call's: results as in a fresh model."""
+    spec = small_llama(ctx=640)
+    dev, fresh = DeviceModel(spec), None
+    rng = np.random.default_rng(17)
+    try:
+        prompt = rng.integers(1, spec.vocab, size=500).tolist()
+        dev.prefill(prompt)
+        for pre, cuts in ((3, [1, 1, 1]), (500, [3, 1, 2]), (40, [9, 9])):
+            rows = [rng.integers(1, spec.vocab, size=c).tolist() for c in cuts]
+            _, _, got = dev.shared_step(pre, rows, cuts, logits=True)
+            fresh = DeviceModel(spec)
+            fresh.prefill(prompt)
+            _, _, want = fresh.shared_step(pre, rows, cuts, logits=True)
+            assert np.array_equal(got, want)
+            fresh.free()
+            fresh = None
+    finally:
+        dev.free()
+        if fresh is not None:
+            fresh.free()
