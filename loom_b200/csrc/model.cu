@@ -1088,6 +1088,10 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
     if (ad && (!s->adapter_ids || !ad->n_adapters || !ad->max_rank || !ad->d_ranks || !ad->d_scales ||
                (ad->q_a && !ad->q_b) || (ad->v_a && !ad->v_b)))
         return rt_decline("shared_step: adapters need ids, ranks, scales and both of their matrices");
+    for (size_t li = 0; ad && li < m.n_layers; li++) {
+        if ((ad->q_a && ad->q_a[li] && !ad->q_b[li]) || (ad->v_a && ad->v_a[li] && !ad->v_b[li]))
+            return rt_decline("shared_step: a layer's adapters need both of their matrices");
+    }
     const loom_verify_desc vd{LOOM_F32, n, rows, m.vocab, m.vocab, m.vocab};
     const loom_attn_shared_desc adesc = shared_desc(m, n, rows, s->prefix_len);
     size_t ws = std::max(loom_cuda_attn_shared_workspace(&adesc), loom_cuda_verify_workspace(&vd));

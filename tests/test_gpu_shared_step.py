@@ -270,3 +270,26 @@ def test_the_scratch_follows_the_prompt(be):
         dev.free()
         if fresh is not None:
             fresh.free()
+
+
+def test_a_missing_matrix_is_refused_before_anything_runs(be):
+    """A layer with the first matrix of an adapter and not the second."""
+    spec = small_llama()
+    dev = DeviceModel(spec)
+    try:
+        dev.prefill([1, 2, 3])
+        d, q = spec.dim, spec.n_heads * spec.head_dim
+        pair = (torch.zeros((1, 2, d), device="cuda"), torch.zeros((1, q, 2), device="cuda"))
+        ad = Adapters([pair] * spec.n_layers, [pair] * spec.n_layers, [2], [1.0])  # q and v are as wide here
+        step = dict(adapters=ad, adapter_ids=[0, -1])
+        dev.shared_step(3, [[4, 5], [6]], [2, 1], **step)
+        for k in (1, 3):  # B of q, of v
+            was, ad._tables[k][1] = ad._tables[k][1], None
+            launched = be.kernelLaunches()
+            with pytest.raises(LoomCudaError, match="matrices"):
+                dev.shared_step(3, [[4, 5], [6]], [2, 1], **step)
+            assert be.kernelLaunches() == launched
+            ad._tables[k][1] = was
+        dev.shared_step(3, [[4, 5], [6]], [2, 1], **step)
+    finally:
+        dev.free()
