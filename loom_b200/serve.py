@@ -36,13 +36,18 @@ def _need(ok: bool, why: str) -> None:
         raise LoomCudaError(why)
 
 
+def _up(op: str, dev: int) -> None:
+    """Bring-up, unless it is up, or the refusal of a second device."""
+    _lib.must(_lib.lib().loom_cuda_init(dev), op)
+
+
 def _on(op: str, t) -> int:
     """The cuda device of t, on which the backend is up."""
     global _device
     dev = t.get_device() if isinstance(t, torch.Tensor) else -1
     _need(dev >= 0, f"{op}: tensors must be on a cuda device")
-    if dev != _device:  # bring-up, or the refusal of a second device
-        _lib.must(_lib.lib().loom_cuda_init(dev), op)
+    if dev != _device:
+        _up(op, dev)
         _device = dev
     return dev
 
@@ -105,7 +110,10 @@ def _run(op: str, entry, size, desc, args, dev: int, stream: Optional[int]) -> N
                 ws = _kept[dev, cur] = torch.empty(_KEEP, dtype=torch.uint8, device=dev)
             if entry(desc, *args, ws.data_ptr(), _KEEP, cur) == _lib.OK:
                 return
-    need = size(desc)  # larger, captured, on a stream of the caller's, or refused: then for the reason it names
+    # larger, captured, on a stream of the caller's, or refused: then for the reason it names, unless the backend was shut
+    # down since a call here brought it up
+    _up(op, dev)
+    need = size(desc)
     ws = _new(op, need, torch.uint8, dev, st, read=False)
     _lib.must(entry(desc, *args, ws.data_ptr(), need, st), op)
 

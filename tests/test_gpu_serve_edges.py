@@ -1,12 +1,14 @@
 """GPU tests of the batched-serving operators' edges: streams and captures, values
 and random numbers at the ends of their ranges. Inputs, plain forms and tolerances
 are those of test_gpu_serve.py."""
-import numpy as np
+import subprocess
+import sys
+
 import pytest
 import torch
 
-from tests.test_gpu_serve import (ATTN_TOL, BF16, F16, F32, TYPES, attn, attn_inputs, attn_ref, ints, lora, lora_inputs,  # noqa: F401
-                                  lora_ref, rel, sv, check_verify, verify_inputs)
+from tests.test_gpu_serve import (ATTN_TOL, BF16, F16, F32, TYPES, attn, attn_inputs, attn_ref, check_verify, lora,  # noqa: F401
+                                  lora_inputs, lora_ref, rel, sv, verify_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -185,3 +187,22 @@ def test_lora_infinite_operands(sv, ty, n):
             f = fin[r]
             if f.any():
                 assert float((out[r][f].double() - want[r][f]).abs().max()) <= 2e-5 * float(want[r][f].abs().max())
+
+
+# ---- the backend's life ---------------------------------------------------------
+
+def test_calls_after_a_shutdown_bring_the_backend_up_again():
+    code = """
+import torch
+from loom_b200 import _lib, serve
+x, a, b = torch.ones(2, 8, device="cuda"), torch.ones(1, 2, 8, device="cuda"), torch.ones(1, 4, 2, device="cuda")
+ranks, ids, scales = (torch.tensor(v, dtype=t, device="cuda") for v, t in (([2], torch.int32), ([0, -1], torch.int32), ([0.5], torch.float32)))
+for _ in range(2):
+    y = serve.lora(x, a, b, ranks, scales, ids)
+    assert y.tolist() == [[8.0] * 4, [0.0] * 4], y
+    torch.cuda.synchronize()
+    _lib.lib().loom_cuda_shutdown()
+print("up again")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "up again" in r.stdout, r.stderr[-2000:]

@@ -113,6 +113,7 @@ def fake(monkeypatch):
         monkeypatch.setattr(serve, "_stream", lambda dev: f.now)
         monkeypatch.setattr(serve, "_capturing", lambda: f.now in f.captured)
         monkeypatch.setattr(serve, "_kept", {})
+        monkeypatch.setattr(serve, "_up", lambda op, dev: None)
         return f
     return use
 
