@@ -8,6 +8,7 @@
 
 #include "kernels.cuh"
 #include "pdl.cuh"
+#include "smem_limit.h"
 
 namespace loom {
 
@@ -36,19 +37,18 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Let kernel K use `smem` bytes of dynamic shared memory; the driver is asked only
-// when a launch needs more than K's earlier ones on the device did.
+// Let kernel K use `smem` bytes of dynamic shared memory.
 template <auto K> cudaError_t allow_smem(size_t smem) {
-    static size_t most[16] = {};
+    static SmemLimit limit;
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 16 && most[dev] >= smem)) return e;
-    e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    // kernels that are to share an SM need the same split of its memory: all of it shared
-    if (e == cudaSuccess && smem > 48 * 1024)
-        e = cudaFuncSetAttribute(K, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e == cudaSuccess && dev < 16) most[dev] = smem;
-    return e;
+    if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+    return limit.need(dev, smem, [](size_t bytes) {
+        cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        // kernels that are to share an SM need the same split of its memory: all of it shared
+        if (e == cudaSuccess && bytes > 48 * 1024)
+            e = cudaFuncSetAttribute(K, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        return e;
+    });
 }
 
 // f(T{}) with the element type behind a type id (checked by the caller)

@@ -1,6 +1,7 @@
 """CPU checks of the batched-serving entries: struct layout, refusals that need no device."""
 import contextlib
 import ctypes as C
+import os
 import shutil
 import subprocess
 
@@ -145,3 +146,34 @@ def test_scratch_of_captured_calls(fake):
     with pytest.raises(LoomCudaError, match="captured"):
         run_on(7)
     assert f.made == []
+
+
+def test_shared_memory_limit_of_two_threads(tmp_path):
+    """The larger limit stays, whichever thread comes back from the driver last."""
+    if not shutil.which("g++"):
+        pytest.skip("no C++ compiler")
+    (tmp_path / "t.cc").write_text('''
+#include "smem_limit.h"
+#include <chrono>
+#include <cstdio>
+#include <thread>
+int main() {
+    loom::SmemLimit l;
+    size_t set = 0;
+    int asked = 0;
+    auto nap = [](int ms) { std::this_thread::sleep_for(std::chrono::milliseconds(ms)); };
+    std::thread large([&] { l.need(0, 200, [&](size_t n) { set = n; asked++; nap(400); return 0; }); });
+    std::thread small([&] { nap(100); l.need(0, 100, [&](size_t n) { nap(100); set = n; asked++; return 0; }); });
+    large.join();
+    small.join();
+    l.need(0, 200, [&](size_t n) { set = n; asked++; return 0; });
+    const int refused = l.need(0, 300, [&](size_t) { return 7; });
+    const int again = l.need(0, 300, [&](size_t n) { set = n; return 0; });
+    std::printf("%zu %d %d %d\\n", set, asked, refused, again);
+    return set == 300 && asked == 1 && refused == 7 && again == 0 ? 0 : 1;
+}
+''')
+    src = os.path.join(os.path.dirname(_lib.HEADER), "..", "loom_b200", "csrc")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-I", src, "-o", str(tmp_path / "t"), str(tmp_path / "t.cc")], check=True)
+    r = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
