@@ -677,9 +677,15 @@ int loom_cuda_trace_reset(void);
 /* Copy (start, end) pairs of the first n entries; returns entries copied. */
 size_t loom_cuda_trace_read(uint64_t *out, size_t n_kernels);
 /* Bitwise OR of the device error words the kernels raise instead of trapping
- * (1 = a bounded wait on an asynchronous copy gave up); 0 when none, -1 when
- * the stream itself is in error. Synchronizes the backend's stream. */
+ * (1 = a bounded wait on an asynchronous copy gave up; 128 = one of
+ * loom_cuda_attn_shared, on whatever stream, did, and left its rows without a
+ * result); 0 when none, -1 when the stream itself is in error. Synchronizes the
+ * backend's stream. */
 int loom_cuda_device_error(void);
+/* Diagnostic: with on = 1 the waits of the loom_cuda_attn_shared calls that follow
+ * (of this entry or of a model's step) give up once their copies are on the way, as
+ * they do when those do not come; 0: they wait again. Returns the setting before. */
+int loom_cuda_attn_fail_waits(int on);
 /* Synchronize the backend's stream. */
 int loom_cuda_sync(void);
 /* The backend's stream (cudaStream_t). */

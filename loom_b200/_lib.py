@@ -162,6 +162,7 @@ def lib() -> C.CDLL:
         "loom_cuda_tc_exact": (i, [i]),
         "loom_cuda_last_path": (i, []),
         "loom_cuda_device_error": (i, []),
+        "loom_cuda_attn_fail_waits": (i, [i]),
         "loom_cuda_stack_prepare": (i, [vp, sz, C.POINTER(u64)]),
         "loom_cuda_stack_forward": (i, [u64, vp, vp, vp, vp]),
         "loom_cuda_stack_error": (i, [u64]),

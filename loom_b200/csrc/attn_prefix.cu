@@ -51,7 +51,7 @@ struct ApBars {
     int err, issued;  // a wait gave up; copies issued
 };
 
-__device__ int g_ap_err;  // a wait of any launch gave up
+__device__ unsigned g_gave_up;  // CTAs of which a wait gave up
 
 template <int NB> constexpr size_t ap_smem() {  // queries of two tiles, the ring, barriers
     return NB * (2 * AP_QBLOCK + AP_STAGES * AP_BLOCK) + sizeof(ApBars);
@@ -145,7 +145,7 @@ __global__ void __maxnreg__(112)
     const int n = (it.p1 - it.p0 + AP_N - 1) / AP_N, rows = it.r1 - it.r0, tiles = rows > 128 ? 2 : 1;
     volatile int *err = &B.err;
     auto wait = [&](uint64_t *bar, uint32_t parity) {  // false once any wait of the CTA has given up
-        for (int i = 0; i < ATTN_TRIES; i++) {
+        for (int i = 0; i < ATTN_LOOKS; i++) {
             if (mbar_wait(bar, parity, ATTN_POLLS)) return true;
             if (*err) return false;
         }
@@ -290,7 +290,8 @@ __global__ void __maxnreg__(112)
         const int t = warp / 4, row = it.r0 + t * 128 + (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), ts = lanes + t * 128, to = lanes + 256 + t * 128;
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        bool ok = true;
+        bool ok = !a.fail;
+        if (!ok) *err = 1;
         for (int j = 0; j < n && ok; j++) {
             ok = __all_sync(0xffffffffu, wait(&B.s_full[t][j & 1], (j >> 1) & 1));
             if (!ok) break;
@@ -368,12 +369,11 @@ __global__ void __maxnreg__(112)
     }
     __syncthreads();
     if (*err) {  // what was issued ends before the memory it uses is given back
-        if (warp == 9 && lane == 0) {
+        if (warp == 9 && ap_elect()) {  // the lane that issued the products
             umma_commit(&B.drain);
-            mbar_wait_hint(&B.drain, 0, 1u << 12, 2000);
-            for (int i = max(B.issued - AP_STAGES, 0); i < B.issued; i++)
-                mbar_wait_hint(&B.full[i % AP_STAGES], (i / AP_STAGES) & 1, 1u << 12, 2000);
-            atomicOr(&g_ap_err, 128);
+            attn_drain(&B.drain, 0);
+            for (int i = max(B.issued - AP_STAGES, 0); i < B.issued; i++) attn_drain(&B.full[i % AP_STAGES], (i / AP_STAGES) & 1);
+            atomicAdd(&g_gave_up, 1u);
         }
         for (int j = tid; j < rows; j += AP_THREADS) a.ml[part_at(a, it.slot, it.r0 + j, kvh)] = make_float2(NAN, NAN);
         __syncthreads();
@@ -391,9 +391,8 @@ template <class T, int NB> cudaError_t ap_launch(const AttnArgs &a, const AttnMa
 
 }  // namespace
 
-int attn_prefix_error() {
-    int v = 0;
-    return cudaMemcpyFromSymbol(&v, g_ap_err, sizeof v) == cudaSuccess ? v : -1;
+cudaError_t attn_prefix_gave_up(unsigned *v, cudaStream_t st) {
+    return cudaMemcpyFromSymbolAsync(v, g_gave_up, sizeof *v, 0, cudaMemcpyDeviceToHost, st);
 }
 
 cudaError_t attn_prefix_run(int type, const AttnArgs &a, const AttnMaps &maps, cudaStream_t st) {

@@ -19,6 +19,7 @@
 // but that length, and a cache row that a query may not see never meets it, not
 // even as 0 times infinity.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/loom_cuda.h"
@@ -30,7 +31,8 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_HD = 256;
 
-__device__ int g_err;  // a wait for a copy gave up
+__device__ unsigned g_gave_up;  // CTAs of which a wait gave up
+std::atomic<int> g_fail{0};
 
 // The end of a CTA. The chunk kernel may run beside the prefix's (attn_prefix.cu),
 // and the join waits for the chunk kernel alone: so one CTA of it, and with it the
@@ -181,14 +183,16 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
     const int blocks = (hd + E - 1) / E, wide = F ? blocks * E : (hd + 15) / 16 * 16;
     const int tiles = (it.p1 - it.p0 + TP - 1) / TP, left = it.p1 - it.p0 - (tiles - 1) * TP;
     auto wait = [&](uint64_t *bar, uint32_t parity) {  // false once any wait of the CTA has given up
-        for (int i = 0; i < ATTN_TRIES; i++) {
+        for (int i = 0; i < ATTN_LOOKS; i++) {
             if (mbar_wait(bar, parity, ATTN_POLLS)) return true;
             if (*reinterpret_cast<volatile int *>(&s_err)) return false;
         }
         *reinterpret_cast<volatile int *>(&s_err) = 1;
         return false;
     };
+    uint32_t issued = 0;              // tiles asked for (thread 0), over all blocks of rows
     auto fetch = [&](int s, int i) {  // tile i into stage s; what lies outside the cache reads as zero
+        issued++;
         const uint32_t dst = sm0 + s * 2 * TILE;
         mbar_expect_tx(&s_full[s], 2 * blocks * BLK);
         for (int b = 0; b < blocks; b++) {
@@ -217,11 +221,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
                    (int64_t)(kvh * a.group + hr % a.group) * hd;
         };
         fence_async_smem();  // zeros written below, before the copies that follow
-        __syncthreads();
+        if (__syncthreads_or(!ok)) break;
         if (tid == 0) {  // both stages are free: every tile before has been read
             fetch(seen & 1, 0);
             if (tiles > 1) fetch((seen + 1) & 1, 1);
         }
+        if (a.fail) ok = false;
         uint32_t qf[KS][4];
         if constexpr (F) {
             // All of a thread's pieces in flight at once. Up to 32 rows are split here, once
@@ -607,9 +612,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && HDP <= 128 ? 3 : 1) k_a
             }
         }
     }
-    if (!ok || *reinterpret_cast<volatile int *>(&s_err)) {  // a copy that does not come: no result
+    if (__syncthreads_or(!ok)) {  // a copy that does not come: no result
+        if (tid == 0) {
+            for (uint32_t i = max(issued, 2u) - 2; i < issued; i++) attn_drain(&s_full[i & 1], (i >> 1) & 1);
+            atomicAdd(&g_gave_up, 1u);
+        }
         for (int hr = it.r0 + tid; hr < it.r1; hr += 128) a.ml[part_at(a, it.slot, hr, kvh)] = make_float2(NAN, NAN);
-        if (tid == 0) atomicOr(&g_err, 128);
     }
     after_prefix();
 }
@@ -1024,8 +1032,11 @@ template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
 }  // namespace
 
 int attn_shared_error() {
-    int v = 0;
-    return cudaMemcpyFromSymbol(&v, g_err, sizeof v) == cudaSuccess ? v | attn_prefix_error() : -1;
+    unsigned a = 0, b = 0;
+    if (cudaMemcpyFromSymbol(&a, g_gave_up, sizeof a) != cudaSuccess || attn_prefix_gave_up(&b, nullptr) != cudaSuccess ||
+        cudaStreamSynchronize(nullptr) != cudaSuccess)
+        return -1;
+    return a || b ? 128 : 0;
 }
 
 }  // namespace loom
@@ -1065,8 +1076,11 @@ int loom_cuda_attn_shared(const loom_attn_shared_desc *d, const void *d_q, const
     a.seq_len = d_seq_len;
     a.ml = static_cast<float2 *>(d_ws);
     a.acc = reinterpret_cast<float *>(static_cast<uint8_t *>(d_ws) + ml_bytes(a));
+    a.fail = g_fail;
     const cudaError_t e = by_type(d->type, [&](auto t) { return launch<decltype(t)>(a, prefix_tc(d), rt_stream(stream)); });
     return e == cudaSuccess ? LOOM_CUDA_OK : rt_fail("attn_shared", e);
 }
+
+int loom_cuda_attn_fail_waits(int on) { return g_fail.exchange(on != 0); }
 
 }  // extern "C"

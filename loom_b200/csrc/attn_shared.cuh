@@ -22,6 +22,7 @@ struct AttnArgs {
     int pre_chunk, own_chunk, n_pre, n_own, pre_tiles, pre_rows;
     int first;    // first item of a launch that leaves the prefix's to another
     int split;    // f32 products were made of tf32 terms
+    int fail;     // the waits give up (loom_cuda_attn_fail_waits)
     float scale;  // of the scores in base 2: scale * log2(e)
 };
 
@@ -96,15 +97,19 @@ __device__ __forceinline__ void attn_tma(uint32_t dst, const CUtensorMap *map, i
 __device__ __forceinline__ void attn_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// A wait gives up after about a second (a poll that finds nothing sleeps 4 us). The
+// limits are constants: read from the arguments they cost the kernels 1 to 7 %.
 constexpr uint32_t ATTN_POLLS = 64;  // polls of a wait between looks at the CTA's error flag,
-constexpr int ATTN_TRIES = 1 << 14;  // and looks before it gives up
+constexpr int ATTN_LOOKS = 1 << 12;  // and looks before it gives up
+// After a wait gave up: the copies to this CTA's memory that are under way, before that is given back.
+__device__ __forceinline__ void attn_drain(uint64_t *bar, uint32_t parity) { mbar_wait_hint(bar, parity, 1u << 12, 2000); }
 
 // The prefix items of a 16-bit call (head_dim <= 128, scale > 0, pre_rows <= 256,
 // pre_chunk a multiple of the box of ATTN_PREFIX_N positions) on the 5th-generation
 // tensor cores.
 constexpr int ATTN_PREFIX_N = 64;
 cudaError_t attn_prefix_run(int type, const AttnArgs &a, const AttnMaps &maps, cudaStream_t st);
-int attn_prefix_error();  // 128 after a wait of it gave up; -1 when the device is in error
-int attn_shared_error();  // the same of all the operator's kernels
+cudaError_t attn_prefix_gave_up(unsigned *v, cudaStream_t st);  // to v: CTAs of which a wait gave up, ever
+int attn_shared_error();  // 128 after a wait of the operator's kernels gave up; -1 when the device is in error
 
 }  // namespace loom

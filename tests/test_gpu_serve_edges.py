@@ -206,3 +206,38 @@ print("up again")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "up again" in r.stdout, r.stderr[-2000:]
+
+
+def alone(code):
+    """In a process of its own: the word of waits that gave up stays set."""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stdout + r.stderr[-2000:]
+
+
+def test_attn_waits_that_give_up():
+    """No result, the error word, and the next call is right."""
+    alone("""
+import torch
+from loom_b200 import _lib, backend
+from tests.test_gpu_serve import ATTN_TOL, TYPES, attn, attn_inputs, attn_ref, rel
+import loom_b200.serve as sv
+backend.init(0)
+L = _lib.lib()
+assert L.loom_cuda_device_error() == 0
+shapes = (([3, 1, 2] * 5, [50, 300, 129] * 5, 32, 4, 128, 1000, 320), ([4] * 33, list(range(4, 37)), 32, 4, 128, 4099, 40),
+          ([100, 0, 200], [120, 0, 200], 8, 8, 48, 2401, 200), ([2, 2], [64, 20], 16, 4, 256, 130, 70))
+for ty in TYPES:
+    for rows, lens, *rest in shapes:
+        i = attn_inputs(ty, rows, lens, *rest, seed=8)
+        assert rel(attn(sv, i), attn_ref(i, rows, lens)) < ATTN_TOL[ty]
+        assert L.loom_cuda_attn_fail_waits(1) == 0
+        for _ in range(3):
+            out = attn(sv, i)
+        torch.cuda.synchronize()
+        assert L.loom_cuda_device_error() == 128
+        if ty is not torch.float32:  # f32 takes rows that came out NaN again
+            assert bool(torch.isnan(out).all())
+        assert L.loom_cuda_attn_fail_waits(0) == 1
+        assert rel(attn(sv, i), attn_ref(i, rows, lens)) < ATTN_TOL[ty]
+print("done")
+""")
