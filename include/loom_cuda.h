@@ -431,7 +431,9 @@ int loom_cuda_model_decode_batch(uint64_t handle, const uint32_t *tokens, const 
  * d_draft_probs and the adapters. After it a sequence has n_out[b] tokens more than
  * before its rows: the accepted drafts, whose cache rows stand, and the chosen one,
  * the first row of its next step, which starts n_out[b] positions after this one's.
- * Synchronous. Declines MLA models and what the operators decline. */
+ * Synchronous. Declines MLA models and what the operators decline; LOOM_CUDA_ERROR,
+ * without outputs, where a wait of the attention gave up (the rows of this step are
+ * then to be run again). */
 typedef struct {
     int type; /* of the matrices: LOOM_F32, LOOM_F16 or LOOM_BF16 */
     size_t n_adapters, max_rank;

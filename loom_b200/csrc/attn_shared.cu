@@ -1031,12 +1031,15 @@ template <class T> cudaError_t launch(AttnArgs a, bool tc, cudaStream_t st) {
 
 }  // namespace
 
+cudaError_t attn_shared_gave_up(unsigned (&v)[2], cudaStream_t st) {
+    const cudaError_t e = cudaMemcpyFromSymbolAsync(&v[0], g_gave_up, sizeof v[0], 0, cudaMemcpyDeviceToHost, st);
+    return e == cudaSuccess ? attn_prefix_gave_up(&v[1], st) : e;
+}
+
 int attn_shared_error() {
-    unsigned a = 0, b = 0;
-    if (cudaMemcpyFromSymbol(&a, g_gave_up, sizeof a) != cudaSuccess || attn_prefix_gave_up(&b, nullptr) != cudaSuccess ||
-        cudaStreamSynchronize(nullptr) != cudaSuccess)
-        return -1;
-    return a || b ? 128 : 0;
+    unsigned v[2] = {0, 0};
+    if (attn_shared_gave_up(v, nullptr) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) return -1;
+    return v[0] || v[1] ? 128 : 0;
 }
 
 }  // namespace loom

@@ -110,6 +110,7 @@ __device__ __forceinline__ void attn_drain(uint64_t *bar, uint32_t parity) { mba
 constexpr int ATTN_PREFIX_N = 64;
 cudaError_t attn_prefix_run(int type, const AttnArgs &a, const AttnMaps &maps, cudaStream_t st);
 cudaError_t attn_prefix_gave_up(unsigned *v, cudaStream_t st);  // to v: CTAs of which a wait gave up, ever
+cudaError_t attn_shared_gave_up(unsigned (&v)[2], cudaStream_t st);  // the same of all the operator's kernels
 int attn_shared_error();  // 128 after a wait of the operator's kernels gave up; -1 when the device is in error
 
 }  // namespace loom

@@ -29,6 +29,7 @@
 #include "../../include/loom_cuda.h"
 #include "attn.cuh"
 #include "attn_block.cuh"
+#include "attn_shared.cuh"
 #include "gemv.cuh"
 #include "model_kernel.cuh"
 #include "kernels.cuh"
@@ -1118,7 +1119,7 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
             return rc;
         if (m.sh_host) cudaFreeHost(m.sh_host);
         m.sh_host = nullptr;
-        MCK(cudaHostAlloc(&m.sh_host, (5 * r + 3 * q + 1) * 4, cudaHostAllocDefault));
+        MCK(cudaHostAlloc(&m.sh_host, (4 + 5 * r + 3 * q + 1) * 4, cudaHostAllocDefault));
         m.sh_rows = r;
         m.sh_seqs = q;
     }
@@ -1131,7 +1132,8 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
     if ((rc = loom_cuda_reserve(rows, m.dim, std::max<size_t>(m.max_ffn, 1), m.max_ne, m.max_nu))) return rc;
     // [tokens][positions][sequence of the row][adapter of the row][random numbers] by row, [first rows][lengths][temperatures]
     cudaStream_t st = rt_stream(nullptr);
-    uint32_t *h = m.sh_host;
+    unsigned(*gave_up)[2] = reinterpret_cast<unsigned(*)[2]>(m.sh_host);  // before the step and after it
+    uint32_t *h = m.sh_host + 4;
     const float zero = 0.0f;
     std::memcpy(h, s->tokens, rows * 4);
     for (size_t b = 0; b < n; b++)
@@ -1148,6 +1150,7 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
         std::memcpy(h + 5 * rows + 2 * n + 1, s->temperature, n * 4);
     else
         std::memset(h + 5 * rows + 2 * n + 1, 0, n * 4);
+    MCK(attn_shared_gave_up(gave_up[0], st));
     MCK(cudaMemcpyAsync(m.sh_in, h, words_in * 4, cudaMemcpyHostToDevice, st));
     MCK(cudaMemcpyAsync(m.pf_tok, m.sh_in, rows * 4, cudaMemcpyDeviceToDevice, st));
     const uint32_t *in = m.sh_in, *d_rows = in + 5 * rows;
@@ -1160,8 +1163,11 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
                                out, out + rows, reinterpret_cast<float *>(out + rows + n), m.sh_scratch, m.sh_ws, st)))
         return rc;
     MCK(cudaMemcpyAsync(h, m.sh_out, words_out * 4, cudaMemcpyDeviceToHost, st));
+    MCK(attn_shared_gave_up(gave_up[1], st));
     if (s->logits) MCK(cudaMemcpyAsync(s->logits, m.sh_logits, rows * m.vocab * 4, cudaMemcpyDeviceToHost, st));
     MCK(cudaStreamSynchronize(st));
+    if (std::memcmp(gave_up[0], gave_up[1], sizeof gave_up[0]))  // its NaN are not the logits' but look like theirs
+        return rt_fail("shared_step: a wait of the attention gave up, the step has no result", cudaErrorTimeout);
     std::memcpy(s->out, h, rows * 4);
     std::memcpy(s->n_out, h + rows, n * 4);
     if (s->logprobs) std::memcpy(s->logprobs, h + rows + n, rows * 4);

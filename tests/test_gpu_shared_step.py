@@ -7,6 +7,8 @@ Logits are held to 2e-2 relative L2, the tolerance of the model's other fast
 forms: the attention sums in another order, which can move an int8 activation of
 the next matvec."""
 import dataclasses
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -293,3 +295,33 @@ def test_a_missing_matrix_is_refused_before_anything_runs(be):
         dev.shared_step(3, [[4, 5], [6]], [2, 1], **step)
     finally:
         dev.free()
+
+
+def test_a_step_whose_attention_gave_up_is_an_error():
+    """Waits of the attention that give up end the step with an error, not with tokens; the next step is right. (In a
+    process of its own: the word of waits that gave up stays set.)"""
+    code = """
+import numpy as np
+from loom_b200 import LoomCudaError, _lib, backend
+from loom_b200.model import DeviceModel
+from tests.test_gpu_shared_step import small_llama
+backend.init(0)
+dev = DeviceModel(small_llama())
+dev.prefill([3, 1, 4, 1, 5])
+step = dict(prefix_len=5, rows=[[9, 2], [6]], seq_len=[2, 1], logits=True)
+want = dev.shared_step(**step)
+_lib.lib().loom_cuda_attn_fail_waits(1)
+for _ in range(2):
+    try:
+        dev.shared_step(**step)
+        raise SystemExit("no error")
+    except LoomCudaError as e:
+        assert "gave up" in str(e), e
+_lib.lib().loom_cuda_attn_fail_waits(0)
+got = dev.shared_step(**step)
+assert got[0] == want[0] and got[1] == want[1] and np.array_equal(got[2], want[2])
+assert _lib.lib().loom_cuda_device_error() == 128
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stdout + r.stderr[-2000:]
