@@ -422,7 +422,8 @@ int loom_cuda_model_decode_batch(uint64_t handle, const uint32_t *tokens, const 
  * 0 .. prefix_len - 1 of the single-sequence cache (loom_cuda_model_prefill), which
  * all sequences read; sequence b's rows seq_rows[b] .. seq_rows[b + 1] - 1 (at least
  * one: its last token, then its drafts) are the last of its seq_len[b] own
- * positions, which follow the prompt, in the caches of loom_cuda_model_decode_batch.
+ * positions, which follow the prompt, in the caches of loom_cuda_model_decode_batch
+ * (whose number the first call of either entry fixes for the model's life).
  * The drafts are judged and one more token chosen as loom_cuda_verify says, at
  * temperature[b] (NULL: greedy) with the random numbers u (by row; NULL: zeros) and
  * the drafter's probabilities d_draft_probs (device f32 [rows][vocab], NULL: a
@@ -561,7 +562,9 @@ int loom_cuda_ep_a2a_forward_cap(const loom_moe_desc *desc, const float *d_x, si
  * least loom_cuda_*_workspace(desc) bytes, not shared by calls that overlap; its
  * contents need not be kept), so they can be captured in a CUDA graph. Strides
  * count elements; element types are LOOM_F32, LOOM_F16 and LOOM_BF16, sums are
- * f32 or wider. Device-side indices that lie outside the call's sizes are held to
+ * f32 or wider; infinities and NaN that a result depends on go into it as f32
+ * arithmetic has it (which, for f32 attention and for adapters, takes such rows a
+ * slower way). Device-side indices that lie outside the call's sizes are held to
  * them: the result is then meaningless, but nothing outside the buffers is
  * touched. Outputs may not overlap inputs, except where said. */
 
@@ -611,7 +614,8 @@ int loom_cuda_lora(const loom_lora_desc *desc, const float *d_x, const void *d_a
  * accepted in order while d_u[r] * q(draft) < p(draft); at T <= 0 while the draft
  * is the argmax. Then one more token is chosen: after a refusal from max(p - q, 0)
  * (from p when that is zero everywhere), after the last draft from p, at the first
- * index where the running sum exceeds d_u[last row of b] times the whole; at T <= 0
+ * index where the running sum exceeds d_u[last row of b] times the whole (should none,
+ * as for a number rounded up to 1, the last token with weight); at T <= 0
  * the argmax (first maximum, NaN never taken, 0 when nothing is above -inf). d_u is
  * f32 [n_rows] in [0, 1). A draft outside the vocabulary is refused.
  * d_out[r]: the token after row r, for the accepted drafts and the chosen token,

@@ -15,10 +15,11 @@
 //
 // A tile has two S (and a barrier of each kind for each: its threads may be a step
 // ahead of the products), so the products of the next positions are made while its
-// threads are at their exponentials (64 a row and step, 16 an SM and cycle: the
-// bound, beside the products' own 2,048 cycles per 128 positions of two tiles; steps of
-// 128 positions with one S a tile took 131 to 141 us where these take 117, tiles a
-// quarter step apart 125). O
+// threads are at their exponentials. A step of two full tiles is 1,024 cycles of products
+// and, at 16 an SM and cycle, 1,024 of exponentials; it takes about 2,500 (1.3 us), so
+// neither pipe is full (tensor 46 %, issue 35 %): P V of either tile waits for both
+// tiles' P, and the next S for that. Steps of 128 positions with one S a tile took 131 to
+// 141 us where these take 117, tiles a quarter step apart 125. O
 // stays in TMEM; it is scaled when a row's maximum has grown by more than 2^8 over
 // the one in use (the quotient by the sum undoes any common factor, and f32 has
 // room), so after the first positions hardly ever.
@@ -28,7 +29,9 @@
 // each, through a ring of six 16 KB stages), warp 9 the MMAs. The ring's size and
 // 112 registers a thread leave room on the SM for a CTA of the own caches' kernel,
 // which is bound by memory where this one is not. P is rounded to the element type
-// as in attn_shared.cu. 192 rows of 8 heads (128 sequences' drafts) over 32,768 positions
+// for its product, as in attn_shared.cu; its sum is taken before that, since with the
+// weights as rounded the errors are the same (64 rows over 8,192 positions: 2.3e-3 bf16,
+// 2.9e-4 f16) and the call took 166 us, not 162. 192 rows of 8 heads (128 sequences' drafts) over 32,768 positions
 // of 4 KV heads of 128, bf16: 103 GFLOP in 109 to 122 us by the clocks, up to 950
 // TFLOP/s; 64 sequences' 200 rows over 8,192 positions 47 us. Every wait is bounded; one that gives up sets an error word
 // (bit 128 of loom_cuda_device_error), leaves NaN in the CTA's rows and ends.

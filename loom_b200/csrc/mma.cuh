@@ -34,7 +34,9 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
 
 // x = hi + lo with hi, lo of 11 significant bits each (tf32): hi to nearest, the rest,
 // which has either sign, cut off, so x is kept to 2^-21 and hi*hi' + hi*lo' + lo*hi'
-// stands for an f32 product (lo*lo', left out, is below 2^-22 of it). Integer
+// stands for an f32 product (lo*lo', left out, is below 2^-22 of it). Of an infinity,
+// or of what rounds to one, lo is NaN or an infinity of the other sign, so its products
+// come out NaN: who uses this takes sums that are NaN again in plain f32. Integer
 // operations: the conversion instruction made 53 us of an attention call 61.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
