@@ -161,6 +161,13 @@ template <class T> int regrow(Model &m, T *&p, size_t n, bool zero = false) {
 // room for `need` where there is room for `have`: half as much again, so that calls that
 // grow little by little allocate now and then
 size_t grown(size_t need, size_t have) { return std::max(need, have + have / 2); }
+// alloc(more), and where there is no room for that alloc(need)
+template <class F> int fitting(size_t need, size_t more, F alloc) {
+    const int rc = alloc(more);
+    if (!rc || more == need) return rc;
+    cudaGetLastError();  // answered here
+    return alloc(need);
+}
 
 void free_model(Model *m) {
     if (m->exec) cudaGraphExecDestroy(m->exec);
@@ -399,19 +406,20 @@ void matmul_rows(const Mat &m, const float *xf, const XQW &x256, const XQW &x32,
 int alloc_prefill(Model &m, size_t n) {
     if (n <= m.pf_cap) return 0;
     MCK(cudaStreamSynchronize(rt_stream(nullptr)));  // all that uses the rows runs there
-    n = grown(n, m.pf_cap);
+    const size_t dim = m.dim, qd = m.nh * m.hd, kvd = m.nkv * m.hd, more = grown(n, m.pf_cap);
     m.pf_cap = 0;
-    const size_t dim = m.dim, qd = m.nh * m.hd, kvd = m.nkv * m.hd;
-    int rc = 0;
-    if ((rc = regrow(m, m.pf_x[0], n * dim)) || (rc = regrow(m, m.pf_x[1], n * dim)) ||
-        (rc = regrow(m, m.pf_normed, n * dim)) || (rc = regrow(m, m.pf_q, n * qd)) || (rc = regrow(m, m.pf_k, n * kvd)) ||
-        (rc = regrow(m, m.pf_v, n * kvd)) || (rc = regrow(m, m.pf_att, n * qd)) || (rc = regrow(m, m.pf_proj, n * dim)) ||
-        (rc = regrow(m, m.pf_zero, n, true)) || (rc = regrow(m, m.pf_tok, n)) || (rc = regrow(m, m.pf_pos, 1)) ||
-        (rc = alloc_xq(m, m.pf_n256, n * dim, true)) || (rc = alloc_xq(m, m.pf_n32, n * dim, false)) ||
-        (rc = alloc_xq(m, m.pf_a256, n * qd, true)) || (rc = alloc_xq(m, m.pf_a32, n * qd, false)))
-        return rc;
-    m.pf_cap = n;
-    return 0;
+    return fitting(n, more, [&](size_t n) {
+        int rc = 0;
+        if ((rc = regrow(m, m.pf_x[0], n * dim)) || (rc = regrow(m, m.pf_x[1], n * dim)) ||
+            (rc = regrow(m, m.pf_normed, n * dim)) || (rc = regrow(m, m.pf_q, n * qd)) || (rc = regrow(m, m.pf_k, n * kvd)) ||
+            (rc = regrow(m, m.pf_v, n * kvd)) || (rc = regrow(m, m.pf_att, n * qd)) || (rc = regrow(m, m.pf_proj, n * dim)) ||
+            (rc = regrow(m, m.pf_zero, n, true)) || (rc = regrow(m, m.pf_tok, n)) || (rc = regrow(m, m.pf_pos, 1)) ||
+            (rc = alloc_xq(m, m.pf_n256, n * dim, true)) || (rc = alloc_xq(m, m.pf_n32, n * dim, false)) ||
+            (rc = alloc_xq(m, m.pf_a256, n * qd, true)) || (rc = alloc_xq(m, m.pf_a32, n * qd, false)))
+            return rc;
+        m.pf_cap = n;
+        return 0;
+    });
 }
 
 // llama.zig:1698-1825 stepBatch: n tokens at positions pos_base .. pos_base + n - 1 through the
@@ -1112,22 +1120,32 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
     const bool more = rows > m.sh_rows || n > m.sh_seqs;
     if (more || ws > m.sh_ws) MCK(cudaStreamSynchronize(rt_stream(nullptr)));
     if (more) {
-        const size_t r = rows > m.sh_rows ? grown(rows, m.sh_rows) : m.sh_rows, q = n > m.sh_seqs ? grown(n, m.sh_seqs) : m.sh_seqs;
+        const size_t q = std::max(n, m.sh_seqs), r = std::max(rows, m.sh_rows);
+        const size_t more_rows = rows > m.sh_rows ? grown(rows, m.sh_rows) : r;
         m.sh_rows = m.sh_seqs = 0;
-        if ((rc = regrow(m, m.sh_logits, r * m.vocab)) || (rc = regrow(m, m.sh_in, 5 * r + 3 * q + 1)) ||
-            (rc = regrow(m, m.sh_out, 2 * r + q)))
-            return rc;
-        if (m.sh_host) cudaFreeHost(m.sh_host);
-        m.sh_host = nullptr;
-        MCK(cudaHostAlloc(&m.sh_host, (4 + 5 * r + 3 * q + 1) * 4, cudaHostAllocDefault));
-        m.sh_rows = r;
-        m.sh_seqs = q;
+        rc = fitting(r, more_rows, [&](size_t r) {
+            int rc = 0;
+            if ((rc = regrow(m, m.sh_logits, r * m.vocab)) || (rc = regrow(m, m.sh_in, 5 * r + 3 * q + 1)) ||
+                (rc = regrow(m, m.sh_out, 2 * r + q)))
+                return rc;
+            if (m.sh_host) cudaFreeHost(m.sh_host);
+            m.sh_host = nullptr;
+            MCK(cudaHostAlloc(&m.sh_host, (4 + 5 * r + 3 * q + 1) * 4, cudaHostAllocDefault));
+            m.sh_rows = r;
+            m.sh_seqs = q;
+            return 0;
+        });
+        if (rc) return rc;
     }
     if (ws > m.sh_ws) {
         const size_t bytes = grown(ws, m.sh_ws);
         m.sh_ws = 0;
-        if ((rc = regrow(m, m.sh_scratch, bytes))) return rc;
-        m.sh_ws = bytes;
+        rc = fitting(ws, bytes, [&](size_t n) {
+            if (int rc = regrow(m, m.sh_scratch, n)) return rc;
+            m.sh_ws = n;
+            return 0;
+        });
+        if (rc) return rc;
     }
     if ((rc = loom_cuda_reserve(rows, m.dim, std::max<size_t>(m.max_ffn, 1), m.max_ne, m.max_nu))) return rc;
     // [tokens][positions][sequence of the row][adapter of the row][random numbers] by row, [first rows][lengths][temperatures]
