@@ -17,7 +17,7 @@
 // ahead of the products), so the products of the next positions are made while its
 // threads are at their exponentials. A step of two full tiles is 1,024 cycles of products
 // and, at 16 an SM and cycle, 1,024 of exponentials; it takes about 2,500 (1.3 us), so
-// neither pipe is full (tensor 46 %, issue 35 %): P V of either tile waits for both
+// neither pipe is full (tensor 47 %, issue 36 %): P V of either tile waits for both
 // tiles' P, and the next S for that. Steps of 128 positions with one S a tile took 131 to
 // 141 us where these take 117, tiles a quarter step apart 125. O
 // stays in TMEM; it is scaled when a row's maximum has grown by more than 2^8 over

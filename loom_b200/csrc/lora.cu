@@ -304,7 +304,7 @@ template <class T> __global__ void __launch_bounds__(128) k_lora_shrink(LoraArgs
 
 // out: CTA (block of rows, adapter of the block, L_OUT columns). A warp has 16 rows;
 // warps left over split the columns. The weights and the base, which do not wait for
-// t, are asked for before it. Bound by latency: 2,048 rows and columns of rank 64 in 32
+// t, are asked for before it. Bound by latency: 2,048 rows and columns of rank 64 in 33
 // us (1 TB/s of base and out); several column chunks to a CTA took 72 us of a call,
 // not 69.
 constexpr int L_DEEP = 64;  // ranks at a time

@@ -346,7 +346,7 @@ template <class T> __global__ void __launch_bounds__(V_CT) k_verify_sum(VerifyAr
 // The largest logit, then every CTA's sum of the weights, from registers (the parts
 // meet in row_stat, so the cluster meets once, for the maximum). Bound by issuing
 // about 25 instructions per logit, most of them e^x, and by that meeting: 5 greedy rows
-// of 32,000 f32, the whole call 7 us.
+// of 32,000 f32, the whole call 6.1 us.
 template <class T> __global__ void __cluster_dims__(V_C, 1, 1) __launch_bounds__(V_T, sizeof(T) == 4 ? 2 : 3) k_verify_rows(VerifyArgs a) {
     __shared__ float s_best[V_W], s_cta;
     __shared__ double s_sum[V_W];
