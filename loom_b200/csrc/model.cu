@@ -164,9 +164,7 @@ size_t grown(size_t need, size_t have) { return std::max(need, have + have / 2);
 // alloc(more), and where there is no room for that alloc(need)
 template <class F> int fitting(size_t need, size_t more, F alloc) {
     const int rc = alloc(more);
-    if (!rc || more == need) return rc;
-    cudaGetLastError();  // answered here
-    return alloc(need);
+    return rc && more != need ? alloc(need) : rc;
 }
 
 void free_model(Model *m) {

@@ -38,6 +38,7 @@ int fail(const char *what, cudaError_t e) {
     char buf[256];
     snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
     g_err = buf;
+    cudaGetLastError();  // reported here: a later call's check of its launches is not to find it
     return LOOM_CUDA_ERROR;
 }
 int decline(const char *why) {

@@ -14,7 +14,7 @@ import numpy as np
 import pytest
 import torch
 
-from loom_b200 import LoomCudaError
+from loom_b200 import LoomCudaError, _lib
 from loom_b200.model import Adapters, DeviceModel, qwen3_moe, tiny_llama
 from tests.conftest import rel_l2
 
@@ -325,3 +325,21 @@ print("done")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stdout + r.stderr[-2000:]
+
+
+def test_a_step_after_memory_was_refused(be):
+    """An allocation that failed is reported by the call that asked for it, not by the next one."""
+    spec = small_llama()
+    dev = DeviceModel(spec)
+    try:
+        dev.prefill([3, 1, 4, 1, 5])
+        step = dict(prefix_len=5, rows=[[9, 2], [6]], seq_len=[2, 1], logits=True)
+        want = dev.shared_step(**step)
+        plain = dev.decode(7, 5, logits=True)[1].copy()
+        for call, same in ((lambda: dev.shared_step(**step)[2], want[2]), (lambda: dev.decode(7, 5, logits=True)[1], plain),
+                           (lambda: dev.shared_step(**step)[2], want[2])):
+            assert _lib.lib().loom_cuda_reserve(1 << 30, 1 << 16, 1 << 10, 1, 1) == _lib.ERROR  # 2^46 bytes
+            assert "out of memory" in _lib.last_error()
+            assert np.array_equal(call(), same)
+    finally:
+        dev.free()
