@@ -1148,6 +1148,10 @@ int loom_cuda_model_shared_step(uint64_t handle, const loom_shared_step *s) {
     if ((rc = loom_cuda_reserve(rows, m.dim, std::max<size_t>(m.max_ffn, 1), m.max_ne, m.max_nu))) return rc;
     // [tokens][positions][sequence of the row][adapter of the row][random numbers] by row, [first rows][lengths][temperatures]
     cudaStream_t st = rt_stream(nullptr);
+    struct Done {  // also where a launch fails: the next step writes the mirror that the queued copies read
+        cudaStream_t st;
+        ~Done() { cudaStreamSynchronize(st); }
+    } done{st};
     unsigned(*gave_up)[2] = reinterpret_cast<unsigned(*)[2]>(m.sh_host);  // before the step and after it
     uint32_t *h = m.sh_host + 4;
     const float zero = 0.0f;
